@@ -304,6 +304,164 @@ int64_t orth_sieve_hdiag_workspace(int64_t rows, int64_t in_features);
 int orth_sieve_hdiag_hip(const void *x, int32_t x_dtype, int64_t rows, int64_t in_features, float *workspace,
                          int64_t workspace_floats, void *out, int32_t flags, void *stream);
 
+/* Serving many requests at once: what stands between a block's projections.
+ * The reference has no counterpart of these (its only operator is the dual
+ * GEMM, /root/reference/torch_bind/bindings.cpp:9-48); they serve the block
+ * whose projections orth_layers_forward_hip computes.  All pointers are
+ * device memory, strides count elements, and the calls are asynchronous on
+ * `stream`.  Contents of index arrays are checked on the device: an index
+ * outside its range is skipped as each entry says, never followed.
+ *
+ * A paged key-value cache: `pages` pages of `page_size` token slots, each
+ * slot holding kv_heads vectors of head_dim elements in k_cache and in
+ * v_cache.  Slot s of page p, head h starts at p * strides[0] + s *
+ * strides[1] + h * strides[2]; a vector's elements are contiguous.  head_dim
+ * is a multiple of 8, at most 256; pointers are 16-byte aligned and strides
+ * multiples of 8. */
+typedef struct {
+    void *k_cache;
+    void *v_cache;
+    int32_t dtype;           /* orth_dtype_t: ORTH_DT_F16 or ORTH_DT_BF16 */
+    int32_t page_size;       /* >= 1 */
+    int32_t kv_heads;
+    int32_t head_dim;
+    int64_t pages;
+    int64_t k_strides[3];    /* page, slot, head */
+    int64_t v_strides[3];
+} orth_hip_cache_t;
+
+/* Pages, slots and positions of one step's new tokens.  Request r has
+ * lengths[r] tokens in the cache and brings new_tokens[r] (>= 0) more; the
+ * step's arrays have `tokens` places, filled request by request.  With P =
+ * page_size, old = ceil(lengths / P), need = ceil((lengths + new) / P) - old:
+ *   block_table[r, old + j] = the next need[r] entries of free_pages, of
+ *                             which pool[0] are handed out already
+ *   rows[t], positions[t]   = the request and position of token t
+ *   slots[t]                = block_table[r, pos / P] * P + pos % P
+ *   query_start[r]          = the first place of request r (query_start
+ *                             [requests]: the places used), at most `tokens`
+ *   lengths_out = lengths + new_tokens, pool_out[0] = pages handed out after
+ * A request whose tokens exceed the table's width or the places left, whose
+ * numbers are negative or pass 2^31 - 1 together (status bit
+ * ORTH_STEP_NO_ROOM), or whose pages exceed the free ones
+ * (ORTH_STEP_NO_PAGES) is refused whole: it gets no page, its length stays,
+ * its places keep their row with position and slot -1.  pool_out[1] holds
+ * the status bits (0: every request was served).  Places without a token
+ * have row, position and slot -1.  lengths_out and pool_out must not be
+ * the input arrays.  At most ORTH_STEP_REQUESTS requests. */
+#define ORTH_STEP_NO_ROOM 1
+#define ORTH_STEP_NO_PAGES 2
+#define ORTH_STEP_REQUESTS 8192
+typedef struct {
+    const int32_t *lengths;      /* [requests] */
+    const int32_t *new_tokens;   /* [requests] */
+    int32_t *block_table;        /* [requests, table_width], row stride table_stride */
+    const int32_t *free_pages;   /* [free_count] */
+    const int32_t *pool;         /* [2]: pages handed out, ignored */
+    int32_t *lengths_out;        /* [requests] */
+    int32_t *pool_out;           /* [2]: pages handed out, status bits */
+    int32_t *query_start;        /* [requests + 1] */
+    int32_t *rows;               /* [tokens] */
+    int32_t *positions;          /* [tokens] */
+    int64_t *slots;              /* [tokens] */
+    int64_t requests;
+    int64_t table_width;
+    int64_t table_stride;
+    int64_t free_count;
+    int64_t tokens;
+    int32_t page_size;
+    int32_t reserved;
+} orth_hip_step_t;
+int orth_page_step_hip(const orth_hip_step_t *step, void *stream);
+
+/* Writes the new tokens' keys and values to their slots of the cache, the
+ * keys (and the queries, into q_out) turned by rotary positions first.
+ * cos_sin: FP32 [cos_sin_rows, rot], row p holding rot / 2 cosines, then
+ * rot / 2 sines of position p; NULL: no turn, and q must be NULL.  Of the
+ * first rot (even, at most head_dim) elements of a vector, pair i is (i, i +
+ * rot / 2), or (2 i, 2 i + 1) when interleaved; (a, b) becomes (a c - b s,
+ * b c + a s), in FP32, rounded once.  A token whose slot lies outside
+ * [0, pages * page_size) is not written to the cache; one whose position
+ * lies outside [0, cos_sin_rows) is not written either and its q_out is 0.
+ * Two tokens with one slot leave either's values there.  q_out may be q (the
+ * same strides); other overlaps give unspecified values.  q, k, v and q_out
+ * hold the cache's dtype; their strides are [token, head]. */
+typedef struct {
+    const void *q;               /* [tokens, q_heads, head_dim] or NULL */
+    const void *k;               /* [tokens, kv_heads, head_dim] */
+    const void *v;
+    void *q_out;
+    int64_t q_strides[2];
+    int64_t k_strides[2];
+    int64_t v_strides[2];
+    int64_t q_out_strides[2];
+    const int64_t *slots;        /* [tokens] */
+    const int32_t *positions;    /* [tokens]; NULL without cos_sin */
+    const float *cos_sin;
+    int64_t cos_sin_rows;
+    int64_t tokens;
+    int32_t q_heads;
+    int32_t rot;
+    int32_t interleaved;
+    int32_t reserved;
+} orth_hip_append_t;
+int orth_cache_append_hip(const orth_hip_cache_t *cache, const orth_hip_append_t *append, void *stream);
+
+/* Attention of single tokens over the paged cache:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j
+ * over the keys j = 0 .. positions[t] (the last `window` of them when window
+ * > 0) of request rows[t] (NULL: request t), key j in page block_table[row,
+ * j / page_size]; query head h reads key head h / (q_heads / kv_heads).  A
+ * token whose position is negative or whose row lies outside the table gets
+ * zeros; keys past the table's width or in a page outside [0, pages) are not
+ * seen (a token that sees no key gets zeros).  Softmax statistics and sums
+ * are FP32; nothing the mask hides reaches the result, whatever it holds. */
+typedef struct {
+    const void *q;               /* [tokens, q_heads, head_dim], the cache's dtype */
+    void *out;
+    int64_t q_strides[2];        /* token, head */
+    int64_t out_strides[2];
+    const int32_t *block_table;  /* [table_rows, table_width], row stride table_stride */
+    const int32_t *positions;    /* [tokens] */
+    const int32_t *rows;         /* [tokens] or NULL */
+    int64_t table_rows;
+    int64_t table_width;
+    int64_t table_stride;
+    int64_t tokens;
+    int32_t q_heads;
+    int32_t window;              /* 0: every key */
+    float scale;
+    int32_t reserved;
+} orth_hip_attend_t;
+int orth_paged_attention_hip(const orth_hip_cache_t *cache, const orth_hip_attend_t *attend, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[m] = y[m] + scales[i] * (x[m] a[i]^T) b[i]^T,  i = adapters[m]
+ * (out[m] = y[m] where i lies outside [0, count)); a[i] is [rank,
+ * in_features], b[i] [out_features, rank], both contiguous.  Products are
+ * exact, sums FP32, one rounding at the end.  out may be y (the same
+ * stride); other overlaps give unspecified values. */
+#define ORTH_ADAPTER_RANK 256
+typedef struct {
+    const void *x;               /* [tokens, in_features], row stride x_stride */
+    const void *y;               /* [tokens, out_features], row stride y_stride */
+    void *out;                   /* row stride out_stride */
+    const void *a;               /* [count, rank, in_features] */
+    const void *b;               /* [count, out_features, rank] */
+    const int32_t *adapters;     /* [tokens] */
+    const float *scales;         /* [count] or NULL (1) */
+    int64_t x_stride;
+    int64_t y_stride;
+    int64_t out_stride;
+    int64_t tokens;
+    int64_t in_features;
+    int64_t out_features;
+    int64_t count;
+    int32_t rank;                /* 1 .. ORTH_ADAPTER_RANK */
+    int32_t dtype;               /* of x, y, out, a, b: ORTH_DT_F16 or ORTH_DT_BF16 */
+} orth_hip_adapter_t;
+int orth_adapter_add_hip(const orth_hip_adapter_t *adapter, void *stream);
+
 /* Device facts.  Replaces check_tensor_core_support,
  * /root/reference/src/dual_gemm_tensor_core.cu:342-350. */
 typedef struct {

@@ -44,7 +44,8 @@ _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: 
 # forward_group takes make_layer descriptors (OrthoLinear.forward_group wraps it)
 __all__ = ["forward", "forward_planned", "forward_group", "build_plan", "dequant", "pack_base", "pack_csr", "sieve_quantize",
            "sieve_split", "sieve_hdiag", "last_kernel", "last_variant", "set_kernel_policy", "get_kernel_policy", "device_info",
-           "plan_cache_clear", "plan_cache_limit", "plan_cache_info"]
+           "plan_cache_clear", "plan_cache_limit", "plan_cache_info", "page_step", "cache_append", "paged_attention",
+           "adapter_add"]
 
 
 def _req(cond: bool, msg: str) -> None:
@@ -589,6 +590,231 @@ def sieve_hdiag(inputs: torch.Tensor, ieee_div: bool = False) -> torch.Tensor:
     with torch.cuda.device(x.device):
         _lib.check(L.orth_sieve_hdiag_hip(_ptr(x), _DT[x.dtype], n, K, _ptr(ws), ws_n, _ptr(out),
                                           _sieve_flags(ieee_div), _stream(x.device)))
+    return out
+
+
+# ------------------------------------------------- serving many requests at once
+#
+# What stands between a block's projections; none of it has a counterpart in
+# the reference, whose only operator is ``forward``.
+
+def _stride(t: torch.Tensor, d: int) -> int:
+    return int(t.stride(d)) if t.shape[d] > 1 else 0  # one element: no stride
+
+
+def _index(t: torch.Tensor, dev, n, dtype, msg: str) -> None:
+    _req(t.device == dev and t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
+         msg)
+
+
+def _cache(k: torch.Tensor, v: torch.Tensor) -> _lib.OrthHipCache:
+    _req(k.is_cuda and v.device == k.device, "k_cache and v_cache must be on one ROCm GPU")
+    _req(k.dim() == 4 and v.shape == k.shape, "k_cache and v_cache must be [pages, page_size, kv_heads, head_dim]")
+    _req(v.dtype == k.dtype, "k_cache and v_cache must have one dtype")
+    _req(k.stride(3) == 1 and v.stride(3) == 1, "the cache's last dimension must be contiguous")
+    _req(k.dtype in (torch.float16, torch.bfloat16), "the cache must be float16 or bfloat16")
+    _req(k.shape[1] < 1 << 31 and k.shape[2] < 1 << 31, "the cache's page_size or kv_heads is too large")
+    _req(k.shape[3] <= 256, "head_dim must be a multiple of 8, at most 256")
+    return _lib.OrthHipCache(k_cache=_ptr(k), v_cache=_ptr(v), dtype=_DT[k.dtype], page_size=k.shape[1],
+                             kv_heads=k.shape[2], head_dim=k.shape[3], pages=k.shape[0],
+                             k_strides=tuple(_stride(k, d) for d in range(3)),
+                             v_strides=tuple(_stride(v, d) for d in range(3)))
+
+
+def _vectors(t: torch.Tensor, cache: torch.Tensor, tokens: int, msg: str) -> None:
+    _req(t.device == cache.device and t.dtype == cache.dtype and t.dim() == 3 and t.shape[0] == tokens and
+         t.shape[2] == cache.shape[3] and (t.numel() == 0 or t.stride(2) == 1), msg)
+
+
+_LIKE = " must be [tokens, {}, head_dim] of the cache's dtype on its device, vectors contiguous"
+_TABLE = "block_table must be int32 [requests, pages] with contiguous rows that do not overlap"
+
+
+def _table(t: torch.Tensor, dev, rows=None) -> int:
+    """A block table's row stride, checked."""
+    _req(t.device == dev and t.dtype == torch.int32 and t.dim() == 2 and (rows is None or t.shape[0] == rows) and
+         (t.numel() == 0 or (t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]))), _TABLE)
+    return int(t.shape[1] if t.shape[0] < 2 or t.numel() == 0 else t.stride(0))
+
+
+def page_step(lengths, new_tokens, block_table, free_pages, pool, page_size, tokens):
+    """Pages, slots and positions of one step's new tokens, made on the GPU.
+
+    Request r holds ``lengths[r]`` tokens and brings ``new_tokens[r]`` more
+    (int32 [requests]); pages it lacks are taken from ``free_pages`` (int32),
+    of which ``pool[0]`` are handed out already, and written into its row of
+    ``block_table`` (int32 [requests, pages], in place).  ``tokens`` is the
+    number of places in the step's arrays, filled request by request.
+    Returns ``(lengths, pool, query_start, rows, positions, slots)``:
+
+      lengths     int32 [requests], the tokens each request then holds
+      pool        int32 [2], pages handed out, and the step's status: 0, or
+                  bits 1 (a request does not fit the table or the places, or
+                  its numbers are negative) and 2 (the pages ran out)
+      query_start int32 [requests + 1], where each request's places start
+      rows        int32 [tokens], each token's request (-1: an unused place)
+      positions   int32 [tokens], its position in the request (-1: none)
+      slots       int64 [tokens], its cache slot, page * page_size + offset
+
+    A request that does not fit is refused whole: no pages, its length kept,
+    positions and slots -1.  The inputs but ``block_table`` stay as they are,
+    so a repeated call gives the same answer.  The pages of finished requests
+    go back by rewriting ``free_pages`` between steps; at most 8192 requests."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.page_step(lengths, new_tokens, block_table, free_pages, pool, page_size, tokens)
+    _req(lengths.is_cuda, "lengths must be on a ROCm GPU")
+    dev = lengths.device
+    _index(lengths, dev, None, torch.int32, "lengths must be a contiguous int32 vector")
+    R = int(lengths.shape[0])
+    _index(new_tokens, dev, R, torch.int32, "new_tokens must be a contiguous int32 vector as long as lengths")
+    stride = _table(block_table, dev, R)
+    _index(free_pages, dev, None, torch.int32, "free_pages must be a contiguous int32 vector")
+    _index(pool, dev, 2, torch.int32, "pool must be a contiguous int32 vector of 2")
+    _req(1 <= page_size < 1 << 31, "page_size must be positive")
+    _req(0 <= tokens < 1 << 31, "tokens must not be negative, at most 2^31 - 1")
+    out, pool_out, start, rows, positions = (torch.empty(n, dtype=torch.int32, device=dev)
+                                             for n in (R, 2, R + 1, tokens, tokens))
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    s = _lib.OrthHipStep(_ptr(lengths), _ptr(new_tokens), _ptr(block_table), _ptr(free_pages), _ptr(pool), _ptr(out),
+                         _ptr(pool_out), _ptr(start), _ptr(rows), _ptr(positions), _ptr(slots), R,
+                         block_table.shape[1], stride, free_pages.shape[0], tokens, page_size, 0)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_page_step_hip(ctypes.byref(s), _stream(dev)))
+    return out, pool_out, start, rows, positions, slots
+
+
+def cache_append(k, v, k_cache, v_cache, slots, q=None, positions=None, cos_sin=None, interleaved=False, q_out=None):
+    """Writes the new tokens' ``k`` and ``v`` [tokens, kv_heads, head_dim] to
+    their ``slots`` (int64) of the paged cache [pages, page_size, kv_heads,
+    head_dim], in place, and returns ``q`` turned (None without ``q``).
+
+    With ``cos_sin`` (float32 [positions, rot]: each position's rot / 2
+    cosines, then its sines) the first ``rot`` elements of k and q are turned
+    by the rotary angles of ``positions`` (int32): pairs (i, i + rot / 2), or
+    (2 i, 2 i + 1) when ``interleaved``.  ``q_out`` may be ``q`` itself.  A
+    token whose slot is negative or past the cache is not written; one whose
+    position lies outside ``cos_sin`` is not written either, and its q is 0.
+    q, k and v may be strided views (of one projection's output, say) of the
+    cache's dtype, float16 or bfloat16; each vector must be contiguous."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.cache_append(k, v, k_cache, v_cache, slots, q, positions, cos_sin, interleaved, q_out)
+    c = _cache(k_cache, v_cache)
+    dev = k_cache.device
+    _req(k.dim() == 3, "k" + _LIKE.format("kv_heads"))
+    n = int(k.shape[0])
+    _vectors(k, k_cache, n, "k" + _LIKE.format("kv_heads"))
+    _vectors(v, k_cache, n, "v" + _LIKE.format("kv_heads"))
+    _req(k.shape[1] == c.kv_heads and v.shape[1] == c.kv_heads, "k and v must have the cache's kv_heads")
+    _index(slots, dev, n, torch.int64, "slots must be a contiguous int64 vector of tokens")
+    _req(cos_sin is not None or q is None, "q needs cos_sin")
+    _req(q_out is None or q is not None, "q_out needs q")
+    a = _lib.OrthHipAppend(k=_ptr(k), v=_ptr(v), k_strides=(_stride(k, 0), _stride(k, 1)),
+                           v_strides=(_stride(v, 0), _stride(v, 1)), slots=_ptr(slots), tokens=n,
+                           interleaved=int(bool(interleaved)))
+    none = ctypes.c_float()  # an empty table still turns the call: no position lies inside it
+    if cos_sin is not None:
+        _req(positions is not None, "cos_sin needs positions")
+        _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
+        _req(cos_sin.device == dev and cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
+             "cos_sin must be a contiguous float32 [positions, rot]")
+        _req(cos_sin.shape[1] % 2 == 0 and cos_sin.shape[1] <= c.head_dim, "rot must be even and at most head_dim")
+        a.positions = _ptr(positions)
+        a.cos_sin = _ptr(cos_sin) or ctypes.addressof(none)
+        a.cos_sin_rows, a.rot = cos_sin.shape
+    if q is not None:
+        _vectors(q, k_cache, n, "q" + _LIKE.format("q_heads"))
+        _req(1 <= q.shape[1] < 1 << 31, "q must have heads")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _vectors(q_out, k_cache, n, "q_out must be like q")
+        _req(q_out.shape[1] == q.shape[1], "q_out must be like q")
+        a.q, a.q_out, a.q_heads = _ptr(q), _ptr(q_out), q.shape[1]
+        a.q_strides, a.q_out_strides = (_stride(q, 0), _stride(q, 1)), (_stride(q_out, 0), _stride(q_out, 1))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_cache_append_hip(ctypes.byref(c), ctypes.byref(a), _stream(dev)))
+    return q_out
+
+
+def paged_attention(q, k_cache, v_cache, block_table, positions, rows=None, scale=None, window=0, out=None):
+    """Attention of single tokens over the paged cache, [tokens, q_heads,
+    head_dim]: token t sees the keys 0 .. ``positions[t]`` (the last
+    ``window`` of them, when positive) of request ``rows[t]`` (None: request
+    t), key j in page ``block_table[row, j // page_size]``.  q_heads is a
+    multiple of the cache's kv_heads, consecutive query heads sharing one.
+    ``scale`` defaults to head_dim ** -0.5.
+
+    A token at position -1 (or whose row lies outside the table) gets zeros;
+    pages outside the cache and keys past the table are not seen.  Several
+    new tokens of one request may be passed at once, each with its own
+    position, once all their keys are in the cache."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.paged_attention(q, k_cache, v_cache, block_table, positions, rows, scale, window, out)
+    c = _cache(k_cache, v_cache)
+    dev = k_cache.device
+    _req(q.dim() == 3, "q" + _LIKE.format("q_heads"))
+    n = int(q.shape[0])
+    _vectors(q, k_cache, n, "q" + _LIKE.format("q_heads"))
+    _req(c.kv_heads > 0 and 0 < q.shape[1] < 1 << 31 and q.shape[1] % c.kv_heads == 0,
+         "q_heads must be a multiple of kv_heads")
+    stride = _table(block_table, dev)
+    _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
+    if rows is not None:
+        _index(rows, dev, n, torch.int32, "rows must be a contiguous int32 vector of tokens")
+    _req(0 <= window < 1 << 31, "window must not be negative")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _vectors(out, k_cache, n, "out must be like q")
+    _req(out.shape[1] == q.shape[1], "out must be like q")
+    a = _lib.OrthHipAttend(q=_ptr(q), out=_ptr(out), q_strides=(_stride(q, 0), _stride(q, 1)),
+                           out_strides=(_stride(out, 0), _stride(out, 1)), block_table=_ptr(block_table),
+                           positions=_ptr(positions), rows=None if rows is None else _ptr(rows),
+                           table_rows=block_table.shape[0], table_width=block_table.shape[1], table_stride=stride,
+                           tokens=n, q_heads=q.shape[1], window=window,
+                           scale=float(scale) if scale is not None else k_cache.shape[3] ** -0.5)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_paged_attention_hip(ctypes.byref(c), ctypes.byref(a), _stream(dev)))
+    return out
+
+
+def adapter_add(y, x, a, b, adapters, scales=None, out=None):
+    """``out[m] = y[m] + scales[i] * (x[m] @ a[i].T) @ b[i].T`` with i =
+    ``adapters[m]`` (int32; outside the adapters: ``out[m] = y[m]``): the
+    low-rank adapters of many requests beside the output ``y`` [M, N] of a
+    projection they share, ``x`` [M, K] its input.  ``a`` [adapters, rank, K]
+    and ``b`` [adapters, N, rank] are stacked and contiguous, rank at most
+    256 (pad smaller ranks with zeros), ``scales`` float32 [adapters] (None:
+    1).  All of x, y, a and b are float16 or bfloat16.  Returns a new tensor,
+    or ``out``, which may be ``y``."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.adapter_add(y, x, a, b, adapters, scales, out)
+    _req(x.is_cuda, "x must be on a ROCm GPU")
+    dev = x.device
+    _req(x.dtype in (torch.float16, torch.bfloat16), "adapters take float16 or bfloat16 activations")
+    _req(x.dim() == 2 and y.dim() == 2 and y.shape[0] == x.shape[0], "x and y must be 2-D [M, K] / [M, N]")
+    _req(a.dim() == 3 and b.dim() == 3 and b.shape == (a.shape[0], y.shape[1], a.shape[1]) and a.shape[2] == x.shape[1],
+         "a must be [adapters, rank, K] and b [adapters, N, rank]")
+    _req(all(t.device == dev for t in (y, a, b)), "x, y, a and b must be on one device")
+    _req(all(t.dtype == x.dtype for t in (y, a, b)), "x, y, a and b must have one dtype")
+    _req(a.is_contiguous() and b.is_contiguous(), "a and b must be contiguous")
+    n = int(x.shape[0])
+    _req(all(t.numel() == 0 or t.stride(1) == 1 for t in (x, y)), "the rows of x and y must be contiguous")
+    _index(adapters, dev, n, torch.int32, "adapters must be a contiguous int32 vector of tokens")
+    if scales is not None:
+        _index(scales, dev, int(a.shape[0]), torch.float32, "scales must be a contiguous float32 vector of adapters")
+    if out is None:
+        out = torch.empty(y.shape, dtype=y.dtype, device=dev)
+    _req(out.device == dev and out.dtype == x.dtype and out.shape == y.shape and (out.numel() == 0 or out.stride(1) == 1),
+         "out must be like y")
+    _req(1 <= a.shape[1] <= 256, "rank must lie in 1..256")
+    g = _lib.OrthHipAdapter(_ptr(x), _ptr(y), _ptr(out), _ptr(a), _ptr(b), _ptr(adapters),
+                            None if scales is None else _ptr(scales), _stride(x, 0), _stride(y, 0), _stride(out, 0), n,
+                            x.shape[1], y.shape[1], a.shape[0], a.shape[1], _DT[x.dtype])
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_adapter_add_hip(ctypes.byref(g), _stream(dev)))
     return out
 
 

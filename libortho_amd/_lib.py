@@ -53,6 +53,43 @@ class OrthHipDeviceInfo(ctypes.Structure):
                 ("l2_bytes", ctypes.c_int32), ("global_mem_bytes", ctypes.c_int64)]
 
 
+class OrthHipCache(ctypes.Structure):
+    _fields_ = [("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("pages", ctypes.c_int64), ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3)]
+
+
+class OrthHipStep(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("lengths", "new_tokens", "block_table", "free_pages", "pool", "lengths_out",
+                                               "pool_out", "query_start", "rows", "positions", "slots")] + \
+               [(n, ctypes.c_int64) for n in ("requests", "table_width", "table_stride", "free_count", "tokens")] + \
+               [("page_size", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class OrthHipAppend(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_strides", "k_strides", "v_strides", "q_out_strides")] + \
+               [(n, ctypes.c_void_p) for n in ("slots", "positions", "cos_sin")] + \
+               [(n, ctypes.c_int64) for n in ("cos_sin_rows", "tokens")] + \
+               [(n, ctypes.c_int32) for n in ("q_heads", "rot", "interleaved", "reserved")]
+
+
+class OrthHipAttend(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_strides", ctypes.c_int64 * 2),
+                ("out_strides", ctypes.c_int64 * 2)] + \
+               [(n, ctypes.c_void_p) for n in ("block_table", "positions", "rows")] + \
+               [(n, ctypes.c_int64) for n in ("table_rows", "table_width", "table_stride", "tokens")] + \
+               [("q_heads", ctypes.c_int32), ("window", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class OrthHipAdapter(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "out", "a", "b", "adapters", "scales")] + \
+               [(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "out_stride", "tokens", "in_features",
+                                              "out_features", "count")] + \
+               [("rank", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 # every function the header declares, with its ctypes signature
 _P, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 _LP = ctypes.POINTER(OrthHipLayer)
@@ -79,6 +116,10 @@ SIGNATURES = {
                                             _P, _P, _P, _P, _I32, _P]),
     "orth_sieve_hdiag_workspace": (_I64, [_I64, _I64]),
     "orth_sieve_hdiag_hip": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I64, _P, _I32, _P]),
+    "orth_page_step_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipStep), _P]),
+    "orth_cache_append_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipCache), ctypes.POINTER(OrthHipAppend), _P]),
+    "orth_paged_attention_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipCache), ctypes.POINTER(OrthHipAttend), _P]),
+    "orth_adapter_add_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipAdapter), _P]),
     "orth_hip_device_info": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(OrthHipDeviceInfo)]),
     "orth_hip_set_kernel_policy": (ctypes.c_int, [ctypes.c_int]),
     "orth_hip_get_kernel_policy": (ctypes.c_int, []),

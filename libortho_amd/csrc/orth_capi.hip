@@ -21,6 +21,7 @@
 
 #include "orth_common.h"
 #include "orth_general_shape.h"
+#include "orth_host.h"
 #include "orth_skinny_shape.h"
 
 namespace orth {
@@ -689,6 +690,25 @@ int group_forward_impl(const orth_hip_layer_t *const *layers, const void *const 
 }
 
 }  // namespace
+
+// What the serving entry points (orth_serve.hip) share with these: errors,
+// the device check and the workspaces.
+namespace orth {
+int host_fail(int status, const char *message) { return fail(status, "%s", message); }
+int host_fail_hip(hipError_t e, const char *what) { return fail_hip(e, what); }
+void host_begin() { t_error.clear(); }
+int host_device(int *dev, int *cus) {
+    int rc = current_device_ok(dev);
+    if (rc == ORTH_OK) *cus = g_dev[*dev].cus;
+    return rc;
+}
+int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p) {
+    float *f = nullptr;
+    int rc = workspace_for(dev, stream, bytes, &f);
+    *p = f;
+    return rc;
+}
+}  // namespace orth
 
 extern "C" {
 

@@ -1,0 +1,17 @@
+// Host-side services of orth_capi.hip for the entry points in other files:
+// the per-thread error message, the device check and the per-stream
+// workspace (under capture: the memory of captured calls).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace orth {
+
+int host_fail(int status, const char *message);
+int host_fail_hip(hipError_t e, const char *what);
+void host_begin();  // clears the thread's error message
+int host_device(int *dev, int *cus);
+int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p);
+
+}  // namespace orth

@@ -17,7 +17,7 @@
 
 #include "orth_hip.h"
 
-namespace {
+void bind_serving(pybind11::module_ &m);  // torch_serve.cpp
 
 // A failed C-ABI call raises libortho_amd._lib.OrthoError(status, message),
 // as the ctypes path does.
@@ -27,6 +27,8 @@ void check_rc(int rc) {
     PyErr_SetObject(cls.ptr(), py::make_tuple(rc, std::string(orth_hip_last_error())).ptr());
     throw py::error_already_set();
 }
+
+namespace {
 
 void req(bool cond, const std::string &msg) {
     if (!cond) throw std::runtime_error(msg);
@@ -231,5 +233,6 @@ PYBIND11_MODULE(_torch_ops, m) {
           py::arg("plan") = py::none(), py::arg("bias") = py::none());
     m.def("linear_group", &linear_group, "several layers over one 2-D input: the outputs allocated and written",
           py::arg("input"), py::arg("layers"));
+    bind_serving(m);
     m.def("abi_version", &orth_hip_abi_version);
 }
