@@ -1,66 +1,596 @@
 // Attention of single tokens over the paged cache.
+//
+// One pass over the keys with a running maximum m and sum l of the softmax:
+// a tile of 32 keys gives scores s (scaled to base 2), m' = max(m, s), p =
+// 2^(s - m'), and the sums l and o = sum p v are scaled by 2^(m - m') where
+// m rises; the result is o / l.
+//
+// A wave takes a tile from registers alone, as two matrix products over
+// v_mfma_f32_16x16x32 (the query heads that share a key head are the 16
+// columns, zeros where there are fewer):
+//
+//   scores  S^T = K Q^T.  The A operand's row and eight elements are a lane's
+//           16-byte load of one key, so keys go from the cache to the
+//           operand.  Row 4 g + i of product tau is key 8 g + 4 tau + i of the
+//           tile: then the scores a lane gets (rows 4 g + i of its lane group
+//           g, both products) are those of keys 8 g .. 8 g + 7.
+//   values  O^T = V^T P^T.  These eight are the B operand's elements of that
+//           lane, so the weights never leave their lane.  The A operand wants
+//           eight keys of one element per lane: a lane loads 8 keys x EL
+//           elements (a key's vector lies across 16 lanes) and transposes
+//           them in registers, one v_perm_b32 per two values.
+//
+// The weights enter the second product as two 16-bit parts, so that rounding
+// them costs 2^-16 and not as much as the output's own rounding; FP16 ones
+// are held 2^14 times larger, which keeps small weights normal numbers.
+//
+// Bound by reading the cache once.  The work is cut evenly over the resident
+// workgroups by the keys the tokens really see, which only the device knows:
+// every wave sums up the tokens' 128-key units and finds its workgroup's
+// share (of some 100 tokens in one load and one scan).  A share that ends
+// inside a (token, key head) leaves a piece (m, l, o) for a second launch to
+// join; whole ones are written at once.
 #include "orth_serve.h"
 
 namespace orth {
 
 namespace {
 
-// A wave per query head: its lanes hold the head's elements, and the keys go
-// by one at a time through a running maximum and sum.
-template <bool BF>
-__global__ __launch_bounds__(64) void paged_attention_kernel(orth_hip_cache_t c, orth_hip_attend_t a, FastDiv page) {
-    const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, lane = threadIdx.x, D = c.head_dim;
-    const int64_t kh = h / (a.q_heads / c.kv_heads);
-    const uint16_t *q = (const uint16_t *)a.q + t * a.q_strides[0] + h * a.q_strides[1];
-    uint16_t *out = (uint16_t *)a.out + t * a.out_strides[0] + h * a.out_strides[1];
-    const int64_t row = a.rows ? a.rows[t] : t;
-    int64_t end = (int64_t)a.positions[t] + 1;
-    if (row < 0 || row >= a.table_rows) end = 0;
-    int64_t begin = a.window > 0 && end > a.window ? end - a.window : 0;
-    const int64_t held = a.table_width * c.page_size;
-    end = end > held ? held : end;
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -__builtin_inff(), l = 0.f;
-    int64_t seen = 0;
+constexpr int kWaves = 4;
+constexpr int kTile = 32;                // keys a wave takes at a time
+constexpr int kUnit = kTile * kWaves;    // keys a workgroup takes at a time
+constexpr float kLeast = -3.0e38f;       // the maximum of a token that has seen keys, at the least
+
+struct AttendArgs {
+    orth_hip_cache_t c;
+    orth_hip_attend_t a;
+    FastDiv page;
+    float scale2;        // scale * log2(e)
+    int group, gtiles;   // query heads of a key head, and their tiles of 16
+    int gt;              // query heads of a tile: min(group, 16)
+    uint32_t min_units;  // the least share of a workgroup
+    float *part;         // pieces [workgroups * 2][gt][head_dim]
+    float2 *stat;        // (m, l) [workgroups * 2][16]
+    int4 *split;         // [workgroups]: (token, head tile, slot, last workgroup) of the split item that starts there
+};
+
+struct Keys {
+    int begin, end;  // the keys a token sees
+    int tile0, tiles;
+    uint32_t units;
+};
+
+__device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
+    const int64_t row = g.a.rows ? (int64_t)g.a.rows[t] : t;
+    int64_t end = (int64_t)g.a.positions[t] + 1;
+    int64_t begin = g.a.window > 0 && end > g.a.window ? end - g.a.window : 0;
+    const int64_t held = g.a.table_width * g.c.page_size;
+    end = end < held ? end : held;
+    if (row < 0 || row >= g.a.table_rows || end <= begin) begin = end = 0;
+    Keys k;
+    k.begin = (int)begin;
+    k.end = (int)(end > INT32_MAX ? INT32_MAX : end);
+    k.tile0 = k.begin / kTile;
+    k.tiles = (int)(((int64_t)k.end + kTile - 1) / kTile) - k.tile0;
+    k.units = k.tiles > kWaves ? (uint32_t)(k.tiles + kWaves - 1) / kWaves : 1;  // (one that sees nothing is written too)
+    return k;
+}
+
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < D ? load16<BF>(q[lane + 64 * i]) : 0.f;
-    for (int64_t j = begin; j < end; j++) {
-        const int64_t at = quotient((uint32_t)j, page), p = a.block_table[row * a.table_stride + at];
-        if (p < 0 || p >= c.pages) continue;
-        seen++;
-        const int64_t in = j - at * c.page_size;
-        const uint16_t *k = (const uint16_t *)c.k_cache + p * c.k_strides[0] + in * c.k_strides[1] + kh * c.k_strides[2];
-        const uint16_t *v = (const uint16_t *)c.v_cache + p * c.v_strides[0] + in * c.v_strides[1] + kh * c.v_strides[2];
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < D) s += qv[i] * load16<BF>(k[lane + 64 * i]);
-        s = wave_sum(s) * a.scale;
-        const float top = fmaxf(m, s), base = top == -__builtin_inff() ? 0.f : top;
-        const float keep = __expf(m - base), w = __expf(s - base);
-        l = l * keep + w;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            o[i] *= keep;
-            if (lane + 64 * i < D) o[i] += w * load16<BF>(v[lane + 64 * i]);
-        }
-        m = top;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up(v, d, 64);
+        if (lane >= d) v += o;
     }
+    return v;
+}
+
+// Inclusive sums of the units of tokens t0 + 4 lane .. + 3, in u[4].
+__device__ __forceinline__ uint64_t block_units(const AttendArgs &g, int64_t t0, int lane, uint32_t u[4]) {
+    uint64_t s = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < D) out[lane + 64 * i] = store16<BF>(seen ? o[i] / l : 0.f);
+    for (int i = 0; i < 4; i++) {
+        const int64_t t = t0 + 4 * lane + i;
+        u[i] = t < g.a.tokens ? keys_of(g, t).units : 0;
+        s += u[i];
+    }
+    return wave_scan64(s, lane);
+}
+
+// The maximum over the four lanes that hold one column.
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two floats as a pair of 16-bit values plus the pair of what they leave.
+template <bool BF>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t *hi, uint32_t *lo) {
+    if constexpr (BF) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 h = {(__bf16)x, (__bf16)y};
+        *hi = __builtin_bit_cast(uint32_t, h);
+        const bf16x2 r = {(__bf16)(x - __uint_as_float(*hi << 16)), (__bf16)(y - __uint_as_float(*hi & 0xffff0000u))};
+        *lo = __builtin_bit_cast(uint32_t, r);
+    } else {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        *hi = __builtin_bit_cast(uint32_t, h);
+        *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+    }
+}
+
+// KS: steps of 32 elements over head_dim; PG8: page_size is a multiple of 8,
+// so eight keys from a multiple of 8 lie in one page and one table entry
+// serves them; TAIL: head_dim is not KS * 32.
+template <int KS, bool BF, bool PG8, bool TAIL>
+__global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kernel(AttendArgs g) {
+    constexpr int EL = KS <= 2 ? 4 : KS <= 4 ? 8 : 16;  // elements of a value vector per lane
+    constexpr int VW = EL / 2;                          // words of them
+    constexpr bool VTAIL = TAIL || 16 * EL != 32 * KS;
+    constexpr float kShift = BF ? 0.f : 14.f;
+    extern __shared__ float lds[];  // o [waves][gt][16 EL + 4], then (m, l) [waves][16]
+    const int D = g.c.head_dim, row_floats = 16 * EL + 4;
+    float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, lg = lane >> 4;
+    const int heads = g.c.kv_heads * g.gtiles;  // items of a token
+
+    // ------------------------------------------------ this workgroup's share
+    uint32_t mine[4];
+    uint64_t run = 0, incl = 0;
+    for (int64_t t0 = 0; t0 < g.a.tokens; t0 += 256) {
+        incl = block_units(g, t0, lane, mine);
+        run += __shfl(incl, 63, 64);
+    }
+    const uint64_t total = run * heads;
+    uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+    per = per < g.min_units ? g.min_units : per;
+    uint64_t cur = blockIdx.x * per;
+    const uint64_t first = cur, stop = cur + per < total ? cur + per : total;
+    if (threadIdx.x == 0 && g.split) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
+    if (cur >= total) return;
+    const uint64_t want = cur / heads;  // the unit, were the heads one
+    int64_t t = 0;
+    uint64_t before = 0;  // units of the tokens in front of t
+    for (int64_t t0 = 0;; t0 += 256) {
+        if (g.a.tokens > 256) incl = block_units(g, t0, lane, mine);
+        const uint64_t all = __shfl(incl, 63, 64);
+        if (before + all > want) {
+            const uint64_t m = __ballot(before + incl > want);
+            const int l = __ffsll((unsigned long long)m) - 1;
+            uint64_t b = before + __shfl(incl, l, 64);
+            int i = 3;
+#pragma unroll
+            for (int k = 3; k >= 0; k--) {
+                const uint32_t u = __shfl(mine[k], l, 64);
+                if (b > want) {
+                    b -= u;
+                    i = k;
+                }
+            }
+            t = t0 + 4 * l + i;
+            before = b;
+            break;
+        }
+        before += all;
+    }
+    Keys k = keys_of(g, t);
+    const uint64_t inside = cur - before * heads;
+    int item = (int)(inside / k.units);
+    uint32_t unit = (uint32_t)(inside - (uint64_t)item * k.units);
+
+    const int64_t k_slot = g.c.k_strides[1], v_slot = g.c.v_strides[1];
+    const bool q16 = ((reinterpret_cast<uintptr_t>(g.a.q) | (uintptr_t)(g.a.q_strides[0] * 2) | (uintptr_t)(g.a.q_strides[1] * 2)) & 15) == 0;
+    const bool o16 = ((reinterpret_cast<uintptr_t>(g.a.out) | (uintptr_t)(g.a.out_strides[0] * 2) | (uintptr_t)(g.a.out_strides[1] * 2)) & 15) == 0;
+
+    while (cur < stop) {
+        const uint64_t left = stop - cur;
+        const uint32_t n = k.units - unit < left ? k.units - unit : (uint32_t)left;
+        const int kvh = item / g.gtiles, gt0 = (item - kvh * g.gtiles) * 16;  // first query head of the tile
+        const int cols = g.group - gt0 < 16 ? g.group - gt0 : 16;
+        const int64_t q_head = (int64_t)kvh * g.group + gt0;
+
+        // the queries: column col, elements 32 j + 8 lg .. + 7
+        u32x4 q[KS];
+#pragma unroll
+        for (int j = 0; j < KS; j++) {
+            const int d = 32 * j + 8 * lg;
+            q[j] = u32x4{0u, 0u, 0u, 0u};
+            if (col < cols && (!TAIL || d < D)) {
+                const uint16_t *p = (const uint16_t *)g.a.q + t * g.a.q_strides[0] + (q_head + col) * g.a.q_strides[1] + d;
+                if (q16) {
+                    q[j] = *reinterpret_cast<const u32x4 *>(p);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) q[j][e] = (uint32_t)p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
+                }
+            }
+        }
+
+        const int64_t row = g.a.rows ? (int64_t)g.a.rows[t] : t;
+        const int32_t *table = g.a.block_table + row * g.a.table_stride;
+        const uint16_t *kbase = (const uint16_t *)g.c.k_cache + kvh * g.c.k_strides[2];
+        const uint16_t *vbase = (const uint16_t *)g.c.v_cache + kvh * g.c.v_strides[2];
+        const int last = k.end - 1;
+        const int tile_end = k.tile0 + (int)((unit + n) * kWaves < (uint32_t)k.tiles ? (unit + n) * kWaves : (uint32_t)k.tiles);
+        int tile = k.tile0 + (int)(unit * kWaves) + wave;
+
+        f32x4 o[EL];
+        float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+        for (int e = 0; e < EL; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        // a key's page (-1: outside the cache) and its address, in elements
+        // from the head's base; keys past the last are taken as the last
+        auto entry = [&](int key) -> int32_t { return table[quotient((uint32_t)(key < last ? key : last), g.page)]; };
+        auto place = [&](int key, int32_t page, const int64_t *strides) -> int64_t {
+            key = key < last ? key : last;
+            const uint32_t in = (uint32_t)key - quotient((uint32_t)key, g.page) * g.page.d;
+            return ((uint32_t)page < (uint64_t)g.c.pages ? (int64_t)page : 0) * strides[0] + (int64_t)in * strides[1];
+        };
+        // (with PG8 the first key of a group of eight stands for all: the
+        // group lies in its page also where the last key ends inside it)
+        const int last8 = last & ~7;
+        auto entry8 = [&](int key) -> int32_t { return table[quotient((uint32_t)(key < last8 ? key : last8), g.page)]; };
+        auto place8 = [&](int key, int32_t page, const int64_t *strides) -> int64_t {
+            key = key < last8 ? key : last8;
+            const uint32_t in = (uint32_t)key - quotient((uint32_t)key, g.page) * g.page.d;
+            return ((uint32_t)page < (uint64_t)g.c.pages ? (int64_t)page : 0) * strides[0] + (int64_t)in * strides[1];
+        };
+
+        u32x4 kf[2][KS];
+        uint32_t vf[8][VW];
+        uint32_t seen8 = 0xff;  // (without PG8: which of the lane's eight keys lie in a page of the cache)
+        int32_t ke = 0, ve = 0, ve_now = 0;
+
+        auto load_k = [&](int tl, int32_t e) {
+            const int key = tl * kTile + (col >> 2) * 8;
+            const uint16_t *p[2];
+            if constexpr (PG8) {
+                p[0] = kbase + place8(key, e, g.c.k_strides) + (col & 3) * k_slot;
+                p[1] = p[0] + 4 * k_slot;
+            } else {
+#pragma unroll
+                for (int tau = 0; tau < 2; tau++) {
+                    const int x = key + 4 * tau + (col & 3);
+                    p[tau] = kbase + place(x, entry(x), g.c.k_strides);
+                }
+            }
+#pragma unroll
+            for (int tau = 0; tau < 2; tau++)
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    const int d = 32 * j + 8 * lg;
+                    kf[tau][j] = *reinterpret_cast<const u32x4 *>(p[tau] + (!TAIL || d < D ? d : 0));
+                }
+        };
+        auto load_v = [&](int tl, int32_t e) {
+            const int key = tl * kTile + lg * 8;
+            const int d0 = !VTAIL || col * EL < D ? col * EL : 0, d1 = !VTAIL || col * EL + 8 < D ? col * EL + 8 : 0;
+            const uint16_t *p = vbase;
+            if constexpr (PG8) p += place8(key, e, g.c.v_strides);
+            else seen8 = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint16_t *x = p;
+                if constexpr (PG8) {
+                    x += i * v_slot;
+                } else {
+                    const int32_t pg = entry(key + i);
+                    x += place(key + i, pg, g.c.v_strides);
+                    seen8 |= (uint32_t)((uint32_t)pg < (uint64_t)g.c.pages) << i;
+                }
+                if constexpr (EL == 4) {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(x + d0);
+                    vf[i][0] = w.x;
+                    vf[i][1] = w.y;
+                } else {
+                    const u32x4 w = *reinterpret_cast<const u32x4 *>(x + d0);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) vf[i][c] = w[c];
+                    if constexpr (EL == 16) {
+                        const u32x4 z = *reinterpret_cast<const u32x4 *>(x + d1);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) vf[i][4 + c] = z[c];
+                    }
+                }
+            }
+        };
+
+        if (tile < tile_end) {
+            if constexpr (PG8) {
+                ke = entry8(tile * kTile + (col >> 2) * 8);
+                ve = entry8(tile * kTile + lg * 8);
+            }
+            load_k(tile, ke);
+            load_v(tile, ve);
+            ve_now = ve;
+            if constexpr (PG8) {
+                ke = entry8((tile + kWaves) * kTile + (col >> 2) * 8);
+                ve = entry8((tile + kWaves) * kTile + lg * 8);
+            }
+        }
+        for (; tile < tile_end; tile += kWaves) {
+            const bool more = tile + kWaves < tile_end;
+            f32x4 s[2];
+#pragma unroll
+            for (int tau = 0; tau < 2; tau++) {
+                s[tau] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    u32x4 a = kf[tau][j];
+                    if constexpr (TAIL)
+                        if (32 * j + 8 * lg >= D) a = u32x4{0u, 0u, 0u, 0u};
+                    s[tau] = mfma<BF>(a, q[j], s[tau]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            int32_t ve_next = ve;
+            if (more) {
+                load_k(tile + kWaves, ke);
+                if constexpr (PG8) {
+                    ke = entry8((tile + 2 * kWaves) * kTile + (col >> 2) * 8);
+                    ve = entry8((tile + 2 * kWaves) * kTile + lg * 8);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = s[i >> 2][i & 3] * g.scale2;
+            const int key0 = tile * kTile;
+            const bool paged = PG8 ? (uint32_t)ve_now < (uint64_t)g.c.pages : seen8 == 0xff;
+            bool any = true;
+            if (key0 < k.begin || key0 + kTile > k.end || !__all(paged)) {
+                // the keys outside the token's range or the cache: no score,
+                // and zero values (0 times an infinity would be a NaN)
+                bool here = false;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int key = key0 + 8 * lg + i;
+                    const bool in = key >= k.begin && key < k.end && (PG8 ? paged : (seen8 >> i & 1) != 0);
+                    here |= in;
+                    if (!in) {
+                        x[i] = -__builtin_inff();
+#pragma unroll
+                        for (int c = 0; c < VW; c++) vf[i][c] = 0u;
+                    }
+                }
+                any = __any(here);
+            }
+            if (any) {
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = fmaxf(fmaxf(column_max(top), kLeast), m);
+                if (__any(top > m)) {
+                    const float keep = __builtin_amdgcn_exp2f(m - top);
+                    l *= keep;
+#pragma unroll
+                    for (int e = 0; e < EL; e++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[e][i] *= keep;
+                    m = top;
+                }
+                const float base = m - kShift;
+                u32x4 ph, pl;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(x[i] - base), p1 = __builtin_amdgcn_exp2f(x[i + 1] - base);
+                    l += p0 + p1;
+                    uint32_t h, r;
+                    split_pair<BF>(p0, p1, &h, &r);
+                    ph[i >> 1] = h;
+                    pl[i >> 1] = r;
+                }
+#pragma unroll
+                for (int c = 0; c < VW; c++) {
+                    u32x4 a, b;  // elements 2 c and 2 c + 1 of the lane's eight keys
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][c], vf[2 * i][c], 0x05040100u);
+                        b[i] = __builtin_amdgcn_perm(vf[2 * i + 1][c], vf[2 * i][c], 0x07060302u);
+                    }
+                    o[2 * c] = mfma<BF>(a, ph, o[2 * c]);
+                    o[2 * c + 1] = mfma<BF>(b, ph, o[2 * c + 1]);
+                    o[2 * c] = mfma<BF>(a, pl, o[2 * c]);
+                    o[2 * c + 1] = mfma<BF>(b, pl, o[2 * c + 1]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_v(tile + kWaves, ve_next);
+            ve_now = ve_next;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l = column_sum(l);
+
+        // join the four waves
+        if (col < cols) {
+            float *dst = lds + (wave * g.gt + col) * row_floats;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < EL; e += 4)
+                    *reinterpret_cast<f32x4 *>(dst + (4 * lg + i) * EL + e) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+            if (lg == 0) lds_stat[wave * 16 + col] = float2{m, l};
+        }
+        __syncthreads();
+        const bool whole = n == k.units;
+        const int slot = (int)blockIdx.x * 2 + (cur == first ? 0 : 1);
+        const int chunks = D / 8;  // eight elements of one query head a thread
+        for (int x = threadIdx.x; x < cols * chunks; x += 256) {
+            const int h = x / chunks, d = (x - h * chunks) * 8;
+            float top = -__builtin_inff(), sum = 0.f, w[kWaves];
+#pragma unroll
+            for (int v = 0; v < kWaves; v++) top = fmaxf(top, lds_stat[v * 16 + h].x);
+            const float base = top == -__builtin_inff() ? 0.f : top;
+            float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < kWaves; v++) {
+                w[v] = __builtin_amdgcn_exp2f(lds_stat[v * 16 + h].x - base);
+                sum += w[v] * lds_stat[v * 16 + h].y;
+                const float *src = lds + (v * g.gt + h) * row_floats + d;
+#pragma unroll
+                for (int i = 0; i < 8; i++) r[i] += w[v] * src[i];
+            }
+            if (whole) {
+                const bool nothing = top == -__builtin_inff();
+                uint16_t *out = (uint16_t *)g.a.out + t * g.a.out_strides[0] + (q_head + h) * g.a.out_strides[1] + d;
+                uint16_t y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = store16<BF>(nothing ? 0.f : r[i] / sum);
+                if (o16) {
+                    u32x4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = (uint32_t)y[2 * i] | (uint32_t)y[2 * i + 1] << 16;
+                    *reinterpret_cast<u32x4 *>(out) = v;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) out[i] = y[i];
+                }
+            } else {
+                float *dst = g.part + ((int64_t)slot * g.gt + h) * D + d;
+                *reinterpret_cast<f32x4 *>(dst) = f32x4{r[0], r[1], r[2], r[3]};
+                *reinterpret_cast<f32x4 *>(dst + 4) = f32x4{r[4], r[5], r[6], r[7]};
+                if (d == 0) g.stat[slot * 16 + h] = float2{top, sum};
+            }
+        }
+        if (!whole && unit == 0 && threadIdx.x == 0)
+            g.split[blockIdx.x] = int4{(int)t, item, slot, (int)((cur + k.units - 1) / per)};
+        __syncthreads();
+        cur += n;
+        unit = 0;
+        if (++item == heads) {
+            item = 0;
+            t++;
+            if (cur < stop) k = keys_of(g, t);
+        }
+    }
+}
+
+// Joins the pieces of the split item that starts in workgroup blockIdx.x, for
+// query head blockIdx.y of its tile.
+template <bool BF>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
+    const int4 s = g.split[blockIdx.x];
+    if (s.x < 0) return;
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = g.c.head_dim;
+    const int kvh = s.y / g.gtiles, gt0 = (s.y - kvh * g.gtiles) * 16;
+    if (gt0 + h >= g.group) return;
+    const int n = s.w - (int)blockIdx.x + 1;
+    auto slot = [&](int i) -> int64_t { return i == 0 ? s.z : ((int64_t)blockIdx.x + i) * 2; };
+    float top = -__builtin_inff();
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, g.stat[slot(i) * 16 + h].x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    __shared__ f32x4 acc[4][64];
+    __shared__ float sums[4];
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    const bool on = 4 * lane < D;
+#pragma unroll 4
+    for (int i = wave; i < n; i += 4) {
+        const float2 st = g.stat[slot(i) * 16 + h];
+        const float w = __builtin_amdgcn_exp2f(st.x - base);
+        sum += w * st.y;
+        if (on) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(g.part + (slot(i) * g.gt + h) * D + 4 * lane);
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] += w * v[e];
+        }
+    }
+    acc[wave][lane] = r;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (wave == 0 && on) {
+        float den = 0.f;
+        r = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            den += sums[v];
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] += acc[v][lane][e];
+        }
+        const int64_t head = (int64_t)kvh * g.group + gt0 + h;
+        uint16_t *out = (uint16_t *)g.a.out + s.x * g.a.out_strides[0] + head * g.a.out_strides[1] + 4 * lane;
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / den);
+    }
+}
+
+// The resident workgroups, and no more than there can be units.
+int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int gtiles) {
+    const int64_t groups = (int64_t)cus * (c.head_dim > 128 ? 1 : c.head_dim > 64 ? 2 : 3);
+    const int64_t held = a.table_width > kUnit * (int64_t)INT32_MAX / c.page_size ? INT32_MAX : a.table_width * c.page_size;
+    int64_t keys = a.window > 0 && a.window + kTile < held ? a.window + kTile : held;
+    const int64_t units = keys / kUnit + 1, items = a.tokens * c.kv_heads * gtiles;
+    return items > groups / units ? groups : items * units;
+}
+
+template <int KS, bool BF>
+hipError_t attend_launch(const AttendArgs &g, int64_t groups, size_t lds, hipStream_t stream) {
+    const bool pg8 = g.c.page_size % 8 == 0, tail = g.c.head_dim != 32 * KS;
+    auto go = [&](auto kernel) -> hipError_t {
+        if (lds > 48 * 1024) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<dim3((unsigned)groups), 256, lds, stream>>>(g);
+        return hipGetLastError();
+    };
+    if (!pg8) return go(attend_kernel<KS, BF, false, true>);
+    return tail ? go(attend_kernel<KS, BF, true, true>) : go(attend_kernel<KS, BF, true, false>);
+}
+
+template <bool BF>
+hipError_t attend_by_width(const AttendArgs &g, int64_t groups, hipStream_t stream) {
+    const int D = g.c.head_dim, el = D <= 64 ? 4 : D <= 128 ? 8 : 16;
+    const size_t lds = (size_t)kWaves * g.gt * (16 * el + 4) * 4 + kWaves * 16 * sizeof(float2);
+    hipError_t e = D <= 64 ? attend_launch<2, BF>(g, groups, lds, stream)
+                 : D <= 96 ? attend_launch<3, BF>(g, groups, lds, stream)
+                 : D <= 128 ? attend_launch<4, BF>(g, groups, lds, stream)
+                            : attend_launch<8, BF>(g, groups, lds, stream);
+    if (e != hipSuccess) return e;
+    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)g.gt), 256, 0, stream>>>(g);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t attention_workspace_bytes(const orth_hip_cache_t &, const orth_hip_attend_t &, int) { return 0; }
+int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus) {
+    const int group = a.q_heads / c.kv_heads;
+    const int64_t groups = attend_groups(c, a, cus, (group + 15) / 16);
+    return groups * (2 * (group < 16 ? group : 16) * (int64_t)c.head_dim * 4 + 2 * 16 * (int64_t)sizeof(float2) + (int64_t)sizeof(int4));
+}
 
-hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int, void *, hipStream_t stream) {
-    const dim3 grid((unsigned)a.tokens, (unsigned)a.q_heads);
-    const FastDiv page = fast_div((uint32_t)c.page_size);
-    if (c.dtype == ORTH_DT_BF16) paged_attention_kernel<true><<<grid, 64, 0, stream>>>(c, a, page);
-    else paged_attention_kernel<false><<<grid, 64, 0, stream>>>(c, a, page);
-    return hipGetLastError();
+hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work,
+                                  hipStream_t stream) {
+    AttendArgs g;
+    g.c = c;
+    g.a = a;
+    g.page = fast_div((uint32_t)c.page_size);
+    g.scale2 = a.scale * 1.4426950408889634f;
+    g.group = a.q_heads / c.kv_heads;
+    g.gtiles = (g.group + 15) / 16;
+    g.gt = g.group < 16 ? g.group : 16;
+    g.min_units = 2;
+    const int64_t groups = attend_groups(c, a, cus, g.gtiles);
+    g.split = static_cast<int4 *>(work);
+    g.stat = reinterpret_cast<float2 *>(g.split + groups);
+    g.part = reinterpret_cast<float *>(g.stat + groups * 2 * 16);
+    return c.dtype == ORTH_DT_BF16 ? attend_by_width<true>(g, groups, stream) : attend_by_width<false>(g, groups, stream);
 }
 
 }  // namespace orth
