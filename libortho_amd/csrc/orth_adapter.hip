@@ -31,7 +31,6 @@ constexpr int kTokens = 64;    // tokens of a tile, where they are many
 constexpr int kFew = 256;      // up to here, tiles of 16: decode batches, whose adapters differ by token
 constexpr int kUp = 64;        // outputs a wave takes at a time
 constexpr int kDown = 8;       // waves of a down workgroup: steps in flight without more partials to add
-constexpr int kShared = 4;     // adapters of a 64-token tile up to which its tokens are taken together
 
 struct AdapterArgs {
     orth_hip_adapter_t a;
@@ -39,17 +38,20 @@ struct AdapterArgs {
     int tiles;         // of 16 or 64 tokens
     int slices, steps; // slices of in_features, and steps of 32 in each
     int blocks;        // up: blocks of out_features
-    int affine;        // all workgroups of a tile on one XCD
+    int slots;         // down, 16 tokens: adapters of a tile, a workgroup each
+    int chunk;         // tiles of an XCD (0: too few to keep together)
 };
 
-// Workgroup -> (tile, part of it): neighbours in blockIdx go to different
-// XCDs, eight in turn; a tile's partials are read from the L2 they went to.
+// Workgroup -> (tile, part of it).  Neighbours in blockIdx go to different
+// XCDs, eight in turn, so XCD x takes the x-th eighth of the tiles: tiles of
+// one prompt share its adapter in that XCD's L2, and a tile's partials are
+// read from the L2 they were written to.
 __device__ __forceinline__ void place_of(const AdapterArgs &g, int parts, int *tile, int *part) {
     const int b = blockIdx.x;
-    if (g.affine) {
-        const int x = b & 7, q = b >> 3;
-        *tile = (q / parts) * 8 + x;
-        *part = q - (q / parts) * parts;
+    if (g.chunk > 0) {
+        const int x = b & 7, q = b >> 3, at = q / parts;
+        *tile = at < g.chunk ? x * g.chunk + at : g.tiles;
+        *part = q - at * parts;
     } else {
         *tile = b / parts;
         *part = b - *tile * parts;
@@ -99,29 +101,33 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
 
 // ------------------------------------------------------------------------ down
 
-// The waves' sums of 16 RB ranks by 16 tokens, joined in LDS; those of the
-// tokens in `own` are written as this slice's partial.
-template <int RB>
-__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 acc[RB], int64_t m0, uint32_t own, int rank0,
-                                          int slice, float (*lds)[16 * RB][17]) {
+// The workgroup's sum of a product: 16 RB ranks by 16 CB tokens of each wave,
+// joined in LDS ([waves][16 RB][16 CB + 1]); those of the tokens in `own` are
+// written as this slice's partial.
+template <int RB, int CB>
+__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&acc)[CB][RB], int64_t m0, uint64_t own,
+                                          int rank0, int slice, float *lds) {
+    constexpr int kRow = 16 * CB + 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     __syncthreads();  // the last use of lds is over
 #pragma unroll
-    for (int r = 0; r < RB; r++)
+    for (int c = 0; c < CB; c++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) lds[wave][16 * r + 4 * lg + i][col] = acc[r][i];
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) lds[(wave * 16 * RB + 16 * r + 4 * lg + i) * kRow + 16 * c + col] = acc[c][r][i];
     __syncthreads();
-    for (int x = threadIdx.x; x < 256 * RB; x += 64 * kDown) {
+    for (int x = threadIdx.x; x < 256 * RB * CB; x += 64 * kDown) {
         const int j = x % (16 * RB), t = x / (16 * RB);
         if (!(own >> t & 1) || rank0 + j >= g.a.rank) continue;
-        float sum = lds[0][j][t];
+        float sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < kDown; w++) sum += lds[w][j][t];
+        for (int w = 0; w < kDown; w++) sum += lds[(w * 16 * RB + j) * kRow + t];
         g.low[((int64_t)slice * g.a.tokens + m0 + t) * g.a.rank + rank0 + j] = sum;
     }
 }
 
-// The steps of this wave: [s, end) of this slice.
+// The steps of this wave in a slice: [s, end).
 __device__ __forceinline__ void down_steps(const AdapterArgs &g, int slice, int *s, int *end) {
     const int wave = threadIdx.x >> 6, share = (g.steps + kDown - 1) / kDown;
     const int all = (int)((g.a.in_features + 31) / 32), last = (slice + 1) * g.steps;
@@ -131,75 +137,67 @@ __device__ __forceinline__ void down_steps(const AdapterArgs &g, int slice, int 
     if (*end > all) *end = all;
 }
 
-// 16 tokens from m0, every adapter among them.
+// A slice for one of a 16-token tile's adapters: a workgroup reads its part
+// of one A, all of a wave's loads in flight.
 template <int RB, bool BF, int W>
-__device__ __forceinline__ void down16(const AdapterArgs &g, int64_t m0, int rank0, int slice, float (*lds)[16 * RB][17]) {
-    constexpr int U = RB == 1 ? 4 : 2;  // steps whose loads are in flight together
+__device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int id, uint32_t own, int rank0, int slice, float *lds) {
+    constexpr int U = RB == 1 ? 8 : 4;
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
-    const int64_t K = g.a.in_features;
-    const int mine = adapter_of(g, m0 + col);
-    const uint32_t own = (uint32_t)__ballot(mine >= 0) & 0xffffu;
-    const int64_t m = m0 + col < g.a.tokens ? m0 + col : g.a.tokens - 1;
-    const uint16_t *xp = (const uint16_t *)g.a.x + m * g.a.x_stride + 8 * lg;
-    const uint16_t *ap = (const uint16_t *)g.a.a + 8 * lg;
-    f32x4 acc[RB];
+    const int64_t K = g.a.in_features, m = m0 + col < g.a.tokens ? m0 + col : g.a.tokens - 1;
+    const uint16_t *xp = (const uint16_t *)g.a.x + m * g.a.x_stride + 8 * lg, *ap[RB];
 #pragma unroll
-    for (int r = 0; r < RB; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < RB; r++) {
+        const int j = rank0 + 16 * r + col;
+        ap[r] = (const uint16_t *)g.a.a + ((int64_t)id * g.a.rank + (j < g.a.rank ? j : g.a.rank - 1)) * K + 8 * lg;
+    }
+    f32x4 acc[1][RB];
+#pragma unroll
+    for (int r = 0; r < RB; r++) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     int s, end;
     down_steps(g, slice, &s, &end);
     for (; s < end; s += U) {
-        u32x4 xv[U];
-        int64_t left[U];
+        u32x4 x[U], a[U][RB];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            left[u] = s + u < end ? K - (int64_t)(s + u) * 32 - 8 * lg : 0;
-            xv[u] = load8<W>(xp + (int64_t)(s + u) * 32, left[u]);
+            const int64_t k = (int64_t)(s + u) * 32, left = s + u < end ? K - k - 8 * lg : 0;
+            x[u] = load8<W>(xp + k, left);
+#pragma unroll
+            for (int r = 0; r < RB; r++) a[u][r] = load8<W>(ap[r] + k, left);
         }
-        for (uint32_t todo = own; todo;) {
-            const int id = __builtin_amdgcn_readlane(mine, __ffs(todo) - 1);
-            const uint32_t same = (uint32_t)__ballot(mine == id) & 0xffffu;
-            todo &= ~same;
-            f32x4 t[RB];
-            u32x4 av[U][RB];
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const int j = rank0 + 16 * r + col;
-                const uint16_t *p = ap + ((int64_t)id * g.a.rank + (j < g.a.rank ? j : g.a.rank - 1)) * K;
+        for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int u = 0; u < U; u++) av[u][r] = load8<W>(p + (int64_t)(s + u) * 32, left[u]);
-                t[r] = acc[r];
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int r = 0; r < RB; r++) t[r] = mfma<BF>(av[u][r], xv[u], t[r]);
-            if (same >> col & 1) {
-#pragma unroll
-                for (int r = 0; r < RB; r++) acc[r] = t[r];
-            }
-        }
+            for (int r = 0; r < RB; r++) acc[0][r] = mfma<BF>(a[u][r], x[u], acc[0][r]);
     }
-    down_join<RB>(g, acc, m0, own, rank0, slice, lds);
+    down_join<RB, 1>(g, acc, m0, own, rank0, slice, lds);
 }
 
-// 64 tokens from m0, the tokens `own` of one adapter: an adapter's loads
-// serve four products.
+// A slice for 64 tokens and every adapter among them; the loads of the next
+// step's tokens and first adapter go ahead of this one's products.
 template <int RB, bool BF, int W>
-__device__ __forceinline__ void down64(const AdapterArgs &g, int64_t m0, int id, uint64_t own, int rank0, int slice,
-                                       float (*lds)[16 * RB][17]) {
-    constexpr int U = RB == 1 ? 2 : 1;
+__device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int rank0, int slice, float *lds) {
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t K = g.a.in_features;
-    const uint16_t *xp[4], *ap[RB];
+    const int mine = adapter_of(g, m0 + lane);
+    const uint64_t own = __ballot(mine >= 0);
+    if (!own) return;
+    auto take = [&](uint64_t &todo, int &id) -> uint64_t {  // the next adapter and its tokens
+        id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
+        const uint64_t same = __ballot(mine == id);
+        todo &= ~same;
+        return same;
+    };
+    const uint16_t *xp[4];
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const int64_t m = m0 + 16 * c + col;
         xp[c] = (const uint16_t *)g.a.x + (m < g.a.tokens ? m : g.a.tokens - 1) * g.a.x_stride + 8 * lg;
     }
+    int64_t row[RB];
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         const int j = rank0 + 16 * r + col;
-        ap[r] = (const uint16_t *)g.a.a + ((int64_t)id * g.a.rank + (j < g.a.rank ? j : g.a.rank - 1)) * K + 8 * lg;
+        row[r] = (j < g.a.rank ? j : g.a.rank - 1) * K + 8 * lg;
     }
     f32x4 acc[4][RB];
 #pragma unroll
@@ -208,75 +206,92 @@ __device__ __forceinline__ void down64(const AdapterArgs &g, int64_t m0, int id,
         for (int r = 0; r < RB; r++) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     int s, end;
     down_steps(g, slice, &s, &end);
-    u32x4 xv[2][U][4], av[2][U][RB];
-    auto load = [&](int at, u32x4 x[U][4], u32x4 a[U][RB]) {
+    auto load = [&](int at, int id, u32x4 a[RB], u32x4 *x) {
+        const int64_t k = (int64_t)at * 32, left = at < end ? K - k - 8 * lg : 0;
+        const uint16_t *p = (const uint16_t *)g.a.a + (int64_t)id * g.a.rank * K + k;
+        if (x) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t k = (int64_t)(at + u) * 32, left = at + u < end ? K - k - 8 * lg : 0;
-#pragma unroll
-            for (int r = 0; r < RB; r++) a[u][r] = load8<W>(ap[r] + k, left);
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[u][c] = load8<W>(xp[c] + k, left);
+            for (int c = 0; c < 4; c++) x[c] = load8<W>(xp[c] + k, left);
         }
+#pragma unroll
+        for (int r = 0; r < RB; r++) a[r] = load8<W>(p + row[r], left);
     };
-    auto product = [&](const u32x4 x[U][4], const u32x4 a[U][RB]) {
+    auto product = [&](const u32x4 a[RB], const u32x4 x[4], uint64_t same) {
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int c = 0; c < 4; c++) {
+            const uint32_t tokens = (uint32_t)(same >> (16 * c)) & 0xffffu;
+            if (!tokens) continue;
+            if (tokens == 0xffffu) {
 #pragma unroll
-            for (int r = 0; r < RB; r++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[c][r] = mfma<BF>(a[u][r], x[u][c], acc[c][r]);
-    };
-    load(s, xv[0], av[0]);
-    for (; s < end; s += 2 * U) {  // (the next step's loads ahead of this one's products)
-        load(s + U, xv[1], av[1]);
-        product(xv[0], av[0]);
-        load(s + 2 * U, xv[0], av[0]);
-        product(xv[1], av[1]);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const uint32_t o = (uint32_t)(own >> (16 * c)) & 0xffffu;
-        if (o) down_join<RB>(g, acc[c], m0 + 16 * c, o, rank0, slice, lds);
-    }
-}
-
-template <int RB, bool BF, int W, bool FEW>
-__global__ __launch_bounds__(64 * kDown) void adapter_down_kernel(AdapterArgs g) {
-    __shared__ float lds[kDown][16 * RB][17];
-    int tile, slice;
-    place_of(g, g.slices, &tile, &slice);
-    if (tile >= g.tiles) return;
-    if constexpr (FEW) {
-        for (int r = 0; r < g.a.rank; r += 16 * RB) down16<RB, BF, W>(g, (int64_t)tile * 16, r, slice, lds);
-    } else {
-        const int64_t m0 = (int64_t)tile * kTokens;
-        const int mine = adapter_of(g, m0 + (threadIdx.x & 63));
-        const uint64_t all = __ballot(mine >= 0);
-        int distinct = 0;
-        for (uint64_t todo = all; todo; distinct++)
-            todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1));
-        for (int r = 0; r < g.a.rank; r += 16 * RB) {
-            if (distinct > kShared) {
-                for (int c = 0; c < 4 && m0 + 16 * c < g.a.tokens; c++) down16<RB, BF, W>(g, m0 + 16 * c, r, slice, lds);
+                for (int r = 0; r < RB; r++) acc[c][r] = mfma<BF>(a[r], x[c], acc[c][r]);
                 continue;
             }
-            for (uint64_t todo = all; todo;) {
-                const int id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
-                const uint64_t same = __ballot(mine == id);
-                todo &= ~same;
-                down64<RB, BF, W>(g, m0, id, same, r, slice, lds);
+            f32x4 t[RB];
+#pragma unroll
+            for (int r = 0; r < RB; r++) t[r] = mfma<BF>(a[r], x[c], acc[c][r]);
+            if (tokens >> col & 1) {
+#pragma unroll
+                for (int r = 0; r < RB; r++) acc[c][r] = t[r];
             }
         }
+    };
+    u32x4 x[2][4], a[2][RB];
+    int id0;
+    uint64_t rest = own;
+    const uint64_t same0 = take(rest, id0);
+    load(s, id0, a[0], x[0]);
+    auto step = [&](int at, u32x4 an[RB], u32x4 xn[4], const u32x4 ac[RB], const u32x4 xc[4]) {
+        load(at + 1, id0, an, xn);
+        product(ac, xc, same0);
+        for (uint64_t todo = rest; todo;) {
+            int id;
+            u32x4 b[RB];
+            const uint64_t same = take(todo, id);
+            load(at, id, b, nullptr);
+            product(b, xc, same);
+        }
+    };
+    for (; s < end; s += 2) {
+        step(s, a[1], x[1], a[0], x[0]);
+        step(s + 1, a[0], x[0], a[1], x[1]);
+    }
+    down_join<RB, 4>(g, acc, m0, own, rank0, slice, lds);
+}
+
+template <int RB, int CB, bool BF, int W>
+__global__ __launch_bounds__(64 * kDown) void adapter_down_kernel(AdapterArgs g) {
+    extern __shared__ float down_lds[];
+    int tile, part;
+    place_of(g, CB == 1 ? g.slices * g.slots : g.slices, &tile, &part);
+    if (tile >= g.tiles) return;
+    const int64_t m0 = (int64_t)tile * 16 * CB;
+    if constexpr (CB == 1) {
+        // the slot's adapter: the slot-th token that is its adapter's first
+        const int slice = part / g.slots, slot = part - slice * g.slots, col = threadIdx.x & 15;
+        const int mine = adapter_of(g, m0 + col);
+        bool first = mine >= 0;
+#pragma unroll
+        for (int d = 1; d < 16; d++) {
+            const int other = __shfl_up(mine, d, 16);  // (all lanes take part)
+            first &= !(col >= d && other == mine);
+        }
+        uint32_t firsts = (uint32_t)__ballot(first) & 0xffffu;
+        for (int i = 0; i < slot; i++) firsts &= firsts - 1;
+        if (!firsts) return;
+        const int id = __builtin_amdgcn_readlane(mine, __ffs(firsts) - 1);
+        const uint32_t own = (uint32_t)__ballot(mine == id) & 0xffffu;
+        for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m0, id, own, r, slice, down_lds);
+    } else {
+        for (int r = 0; r < g.a.rank; r += 16 * RB) down_all<RB, BF, W>(g, m0, r, part, down_lds);
     }
 }
 
 // -------------------------------------------------------------------------- up
 
 // The sum of slices first, first + step, .. of low[m, j0 .. j0 + 7].
+template <int U>  // slices whose loads are in flight together
 __device__ __forceinline__ void low_sum(const AdapterArgs &g, int64_t m, int j0, int first, int step, f32x4 v[2]) {
     const int r = g.a.rank;
-    constexpr int U = 4;  // slices whose loads are in flight together
     v[0] = v[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s0 = first; s0 < g.slices; s0 += U * step) {
         f32x4 p[U][2];
@@ -348,123 +363,107 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
     return sh;
 }
 
-// One unit of kUp outputs from n0 of 16 tokens from m0: the adapters of the
-// tokens in `own`, every `step`-th of them from `first`.  Product t's row
+// CB 1: 16 tokens a workgroup and one unit of kUp outputs; the waves split
+// the slices to add, and then the adapters.  CB 4: 64 tokens; each wave adds
+// 16 of them up and then takes a unit of its own for all.  Product t's row
 // 4 a + i is output 16 a + 4 t + i of the unit, so a lane (rows 4 lg + i of
-// all four) holds outputs 16 lg .. 16 lg + 15 of its token.  Tokens without
-// an adapter are copied with the first ones.
-template <bool BF, int W, bool YV>
-__device__ __forceinline__ void up_unit(const AdapterArgs &g, int64_t m0, int mine, int sh, int64_t n0, int kks,
-                                        const u32x4 *parts, int first, int step) {
-    const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
-    const int64_t N = g.a.out_features, n = n0 + 16 * lg;
-    const uint32_t own = (uint32_t)__ballot(mine >= 0) & 0xffffu;
-    // this call's tokens
-    uint32_t taken = first == 0 ? ~own & 0xffffu : 0;
-    int k = 0;
-    for (uint32_t todo = own; todo; k++) {
-        const uint32_t same = (uint32_t)__ballot(mine == __builtin_amdgcn_readlane(mine, __ffs(todo) - 1)) & 0xffffu;
-        todo &= ~same;
-        if (k % step == first) taken |= same;
-    }
-    const bool on = (taken >> col & 1) && m0 + col < g.a.tokens;
-    if (!__any(on)) return;
-    const int64_t m = m0 + col < g.a.tokens ? m0 + col : g.a.tokens - 1;
-    const uint16_t *y = (const uint16_t *)g.a.y + m * g.a.y_stride + n;
-    u32x4 yv[2];
-    uint16_t ys[16];
-    if constexpr (YV) {
-        yv[0] = load8<8>(y, on ? N - n : 0);
-        yv[1] = load8<8>(y + 8, on ? N - n - 8 : 0);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) ys[e] = on && n + e < N ? y[e] : 0;
-    }
-    f32x4 acc[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int64_t row[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const int64_t at = n0 + 16 * (col >> 2) + 4 * t + (col & 3);
-        row[t] = (at < N ? at : N - 1) * g.a.rank + 8 * lg;
-    }
-    for (uint32_t todo = own & taken; todo;) {
-        const int id = __builtin_amdgcn_readlane(mine, __ffs(todo) - 1);
-        const uint32_t same = (uint32_t)__ballot(mine == id) & 0xffffu;
-        todo &= ~same;
-        const uint16_t *b = (const uint16_t *)g.a.b + (int64_t)id * N * g.a.rank;
-        f32x4 d[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) d[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-        for (int kk = 0; kk < kks; kk++) {
-            u32x4 bv[4];
-#pragma unroll
-            for (int t = 0; t < 4; t++) bv[t] = load8<W>(b + row[t] + 32 * kk, g.a.rank - 32 * kk - 8 * lg);
-            const u32x4 h = parts[(2 * kk) * 64 + lane], l = parts[(2 * kk + 1) * 64 + lane];
-#pragma unroll
-            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[t], h, d[t]);
-#pragma unroll
-            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[t], l, d[t]);
-        }
-        if (same >> col & 1) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) acc[t] = d[t];
-        }
-    }
-    if (!on) return;
-    uint16_t *out = (uint16_t *)g.a.out + m * g.a.out_stride + n;
-    uint16_t r[16];
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const uint16_t v = YV ? (uint16_t)(yv[e >> 3][(e & 7) >> 1] >> (16 * (e & 1))) : ys[e];
-        const float d = acc[e >> 2][e & 3];
-        r[e] = mine >= 0 ? store16<BF>(load16<BF>(v) + (BF ? d : __builtin_amdgcn_ldexpf(d, -sh))) : v;
-    }
-    if constexpr (YV) {
-#pragma unroll
-        for (int v = 0; v < 2; v++)
-            if (n + 8 * v < N) {
-                u32x4 w;
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = (uint32_t)r[8 * v + 2 * i] | (uint32_t)r[8 * v + 2 * i + 1] << 16;
-                *reinterpret_cast<u32x4 *>(out + 8 * v) = w;
-            }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            if (n + e < N) out[e] = r[e];
-    }
-}
-
-// FEW: 16 tokens a workgroup, one unit, its waves split the slices to add
-// and then the adapters; else 64 tokens, a wave 16 of them to add and then a
-// unit for all of them.
-template <bool BF, int W, bool YV, bool FEW>
-__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs g) {
-    extern __shared__ u32x4 parts[];  // [4][kks][2][64]
+// all four) holds outputs 16 lg .. 16 lg + 15 of its token.  The loads of y
+// and of the first adapters' B go ahead of the low-rank sums.  KB: steps of
+// 32 ranks whose loads are in flight together.
+template <int CB, bool BF, int W, bool YV, int KB>
+__global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
+    constexpr int IDS = CB == 1 ? 4 / KB : 1;  // adapters whose loads are in flight together
+    extern __shared__ u32x4 parts[];           // [4][kks][2][64]
     __shared__ int shifts[kTokens];
     int tile, block;
     place_of(g, g.blocks, &tile, &block);
     if (tile >= g.tiles) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     const int kks = (g.a.rank + 31) / 32, each = kks * 128;
-    const int64_t m0 = (int64_t)tile * (FEW ? 16 : kTokens), mw = FEW ? m0 : m0 + 16 * wave;
-    int mine = adapter_of(g, mw + col);
-    const float scale = mine >= 0 ? (g.a.scales ? g.a.scales[mine] : 1.f) : 0.f;
-    if (__any(mine >= 0)) {
+    const int64_t m0 = (int64_t)tile * 16 * CB, N = g.a.out_features;
+    const int mine = adapter_of(g, m0 + (CB == 1 ? col : lane));
+    const uint64_t own = __ballot(mine >= 0) & (CB == 1 ? 0xffffull : ~0ull);
+    const int64_t left = g.a.tokens - m0;
+    const uint64_t here = left >= 16 * CB ? (CB == 1 ? 0xffffull : ~0ull) : ((uint64_t)1 << left) - 1;
+    auto take = [&](uint64_t &todo, int &id) -> uint64_t {  // the next adapter and its tokens
+        id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
+        const uint64_t same = __ballot(mine == id) & own;
+        todo &= ~same;
+        return same;
+    };
+    // this wave's tokens (those without an adapter are copied) and outputs
+    uint64_t held = here;
+    if constexpr (CB == 1) {
+        held = wave == 0 ? here & ~own : 0;
+        int k = 0, id;
+        for (uint64_t todo = own; todo; k++) {
+            const uint64_t same = take(todo, id);
+            if (k % 4 == wave) held |= same;
+        }
+    }
+    const int64_t n0 = CB == 1 ? (int64_t)block * kUp : ((int64_t)block * 4 + wave) * kUp, n = n0 + 16 * lg;
+    if (n0 >= N) held = 0;
+
+    u32x4 yv[CB][2];
+    uint16_t ys[CB][16];
+#pragma unroll
+    for (int c = 0; c < CB; c++) {
+        const bool on = held >> (16 * c + col) & 1;
+        const uint16_t *y = (const uint16_t *)g.a.y + (on ? m0 + 16 * c + col : m0) * g.a.y_stride + n;
+        if constexpr (YV) {
+            yv[c][0] = load8<8>(y, on ? N - n : 0);
+            yv[c][1] = load8<8>(y + 8, on ? N - n - 8 : 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) ys[c][e] = on && n + e < N ? y[e] : 0;
+        }
+    }
+    int64_t row[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const int64_t at = n0 + 16 * (col >> 2) + 4 * t + (col & 3);
+        row[t] = (at < N ? at : N - 1) * g.a.rank + 8 * lg;
+    }
+    u32x4 bv[IDS][KB][4];
+    int ids[IDS];
+    uint64_t same[IDS], todo = held & own;
+    auto next = [&]() {
+#pragma unroll
+        for (int i = 0; i < IDS; i++) {
+            same[i] = 0;
+            ids[i] = 0;
+            if (todo) same[i] = take(todo, ids[i]);
+        }
+    };
+    auto load_b = [&](int kk0) {
+#pragma unroll
+        for (int i = 0; i < IDS; i++)
+            if (same[i]) {
+                const uint16_t *b = (const uint16_t *)g.a.b + (int64_t)ids[i] * N * g.a.rank + 32 * kk0;
+#pragma unroll
+                for (int k = 0; k < KB; k++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) bv[i][k][t] = load8<W>(b + row[t] + 32 * k, g.a.rank - 32 * (kk0 + k) - 8 * lg);
+            }
+    };
+    next();
+    load_b(0);
+
+    // the low-rank values
+    const int tl = CB == 1 ? mine : __shfl(mine, 16 * wave + col, 64);
+    const float scale = tl >= 0 ? (g.a.scales ? g.a.scales[tl] : 1.f) : 0.f;
+    if (__any(tl >= 0)) {
         for (int kk = 0; kk < kks; kk++) {
             f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            if (mine >= 0) low_sum(g, mw + col, 32 * kk + 8 * lg, FEW ? wave : 0, FEW ? 4 : 1, v);
-            if (!FEW) {
+            if (tl >= 0) low_sum<CB == 1 ? 2 : 4>(g, m0 + (CB == 1 ? 0 : 16 * wave) + col, 32 * kk + 8 * lg, CB == 1 ? wave : 0, CB == 1 ? 4 : 1, v);
+            if (CB > 1) {
                 v[0] *= scale;
                 v[1] *= scale;
             }
             parts[wave * each + (2 * kk) * 64 + lane] = __builtin_bit_cast(u32x4, v[0]);
             parts[wave * each + (2 * kk + 1) * 64 + lane] = __builtin_bit_cast(u32x4, v[1]);
         }
-        if constexpr (FEW) {
+        if constexpr (CB == 1) {
             __syncthreads();
             // (x, the rank words, dealt over the waves)
             for (int x = wave; x < 2 * kks; x += 4) {
@@ -475,20 +474,76 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs g) {
             }
             __syncthreads();
         }
-        if (!FEW || wave == 0) {
-            const int sh = low_parts<BF>(kks, parts + (FEW ? 0 : wave * each));
-            if (lane < 16) shifts[(FEW ? 0 : 16 * wave) + lane] = sh;
+        if (CB > 1 || wave == 0) {
+            const int sh = low_parts<BF>(kks, parts + (CB == 1 ? 0 : wave * each));
+            if (lane < 16) shifts[(CB == 1 ? 0 : 16 * wave) + lane] = sh;
         }
     }
     __syncthreads();
-    if constexpr (FEW) {
-        up_unit<BF, W, YV>(g, m0, mine, shifts[col], (int64_t)block * kUp, kks, parts, wave, 4);
-    } else {
-        const int64_t n0 = ((int64_t)block * 4 + wave) * kUp;
-        if (n0 >= g.a.out_features) return;
-        for (int c = 0; c < 4 && m0 + 16 * c < g.a.tokens; c++) {
-            mine = adapter_of(g, m0 + 16 * c + col);
-            up_unit<BF, W, YV>(g, m0 + 16 * c, mine, shifts[16 * c + col], n0, kks, parts + c * each, 0, 1);
+    if (!held) return;
+
+    f32x4 acc[CB][4];
+#pragma unroll
+    for (int c = 0; c < CB; c++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    while (same[0]) {
+        for (int kk0 = 0; kk0 < kks; kk0 += KB) {
+            if (kk0 > 0) load_b(kk0);
+#pragma unroll
+            for (int i = 0; i < IDS; i++)
+#pragma unroll
+                for (int c = 0; c < CB; c++) {
+                    const uint32_t tokens = (uint32_t)(same[i] >> (16 * c)) & 0xffffu;
+                    if (!tokens) continue;
+                    f32x4 d[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++) d[t] = acc[c][t];
+#pragma unroll
+                    for (int k = 0; k < KB; k++)
+                        if (kk0 + k < kks) {
+                            const u32x4 *p = parts + c * each + (kk0 + k) * 128 + lane;
+                            const u32x4 h = p[0], l = p[64];
+#pragma unroll
+                            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], h, d[t]);
+#pragma unroll
+                            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], l, d[t]);
+                        }
+                    if (tokens >> col & 1) {
+#pragma unroll
+                        for (int t = 0; t < 4; t++) acc[c][t] = d[t];
+                    }
+                }
+        }
+        next();
+        load_b(0);
+    }
+#pragma unroll
+    for (int c = 0; c < CB; c++) {
+        if (!(held >> (16 * c + col) & 1)) continue;
+        const bool add = own >> (16 * c + col) & 1;
+        uint16_t *out = (uint16_t *)g.a.out + (m0 + 16 * c + col) * g.a.out_stride + n;
+        const int sh = !BF && add ? shifts[16 * c + col] : 0;
+        uint16_t r[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const uint16_t v = YV ? (uint16_t)(yv[c][e >> 3][(e & 7) >> 1] >> (16 * (e & 1))) : ys[c][e];
+            const float d = acc[c][e >> 2][e & 3];
+            r[e] = add ? store16<BF>(load16<BF>(v) + (BF ? d : __builtin_amdgcn_ldexpf(d, -sh))) : v;
+        }
+        if constexpr (YV) {
+#pragma unroll
+            for (int v = 0; v < 2; v++)
+                if (n + 8 * v < N) {
+                    u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = (uint32_t)r[8 * v + 2 * i] | (uint32_t)r[8 * v + 2 * i + 1] << 16;
+                    *reinterpret_cast<u32x4 *>(out + 8 * v) = w;
+                }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (n + e < N) out[e] = r[e];
         }
     }
 }
@@ -502,65 +557,77 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     const int wide = a.tokens <= kFew ? 16 : kTokens;
     g.tiles = (int)((a.tokens + wide - 1) / wide);
     const int64_t steps = (a.in_features + 31) / 32;
-    // down: slices for a workgroup of eight waves a CU
-    int64_t slices = (int64_t)cus / g.tiles;
-    if (slices > (steps + kDown - 1) / kDown) slices = (steps + kDown - 1) / kDown;
-    if (slices > 16) slices = 16;
+    // down: slices for a workgroup of eight waves a CU, of four steps at
+    // least; every slice is a partial more that each workgroup of the second
+    // launch adds
+    const bool few = a.tokens <= kFew;
+    int64_t most = a.tokens < 16 ? a.tokens : 16;
+    if (a.count < most) most = a.count < 1 ? 1 : a.count;
+    g.slots = few ? (int)most : 1;
+    int64_t slices = (int64_t)cus / (g.tiles * (int64_t)g.slots);
+    if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;
+    if (slices > 8) slices = 8;
     if (slices < 1) slices = 1;
     g.steps = (int)((steps + slices - 1) / slices);
     g.slices = (int)((steps + g.steps - 1) / g.steps);
-    const int64_t span = a.tokens <= kFew ? kUp : 4 * kUp;
+    const int64_t span = few ? kUp : 4 * kUp;
     g.blocks = (int)((a.out_features + span - 1) / span);
-    g.affine = g.tiles >= 8;
+    g.chunk = g.tiles >= 8 ? (g.tiles + 7) / 8 : 0;
     return g;
 }
 
 bool multiple(const void *p, int64_t stride, int n) { return reinterpret_cast<uintptr_t>(p) % (2 * n) == 0 && stride % n == 0; }
 
-template <int RB, bool BF>
-void down_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
-    const bool few = g.a.tokens <= kFew;
-    if (multiple(g.a.x, g.a.x_stride, 8) && multiple(g.a.a, g.a.in_features, 8)) {
-        if (few) adapter_down_kernel<RB, BF, 8, true><<<groups, 64 * kDown, 0, stream>>>(g);
-        else adapter_down_kernel<RB, BF, 8, false><<<groups, 64 * kDown, 0, stream>>>(g);
-    } else {
-        if (few) adapter_down_kernel<RB, BF, 1, true><<<groups, 64 * kDown, 0, stream>>>(g);
-        else adapter_down_kernel<RB, BF, 1, false><<<groups, 64 * kDown, 0, stream>>>(g);
+// Launches a kernel with dynamic LDS, past the default limit where it asks for more.
+template <class Kernel>
+hipError_t launch_lds(Kernel kernel, unsigned groups, int threads, size_t lds, hipStream_t stream, const AdapterArgs &g) {
+    if (lds > 48 * 1024) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
     }
+    kernel<<<groups, threads, lds, stream>>>(g);
+    return hipGetLastError();
 }
 
-template <bool BF, int W>
+template <int RB, bool BF>
+hipError_t down_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
+    const bool few = g.a.tokens <= kFew, wide = multiple(g.a.x, g.a.x_stride, 8) && multiple(g.a.a, g.a.in_features, 8);
+    const size_t lds = (size_t)kDown * 16 * RB * ((few ? 16 : kTokens) + 1) * sizeof(float);
+    auto go = [&](auto kernel) { return launch_lds(kernel, groups, 64 * kDown, lds, stream, g); };
+    if (few) return wide ? go(adapter_down_kernel<RB, 1, BF, 8>) : go(adapter_down_kernel<RB, 1, BF, 1>);
+    return wide ? go(adapter_down_kernel<RB, 4, BF, 8>) : go(adapter_down_kernel<RB, 4, BF, 1>);
+}
+
+template <int CB, bool BF>
 hipError_t up_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
     const size_t lds = (size_t)4 * ((g.a.rank + 31) / 32) * 128 * sizeof(u32x4);
     const bool yv = g.a.out_features % 8 == 0 && multiple(g.a.y, g.a.y_stride, 8) && multiple(g.a.out, g.a.out_stride, 8);
-    auto go = [&](auto kernel) -> hipError_t {
-        if (lds > 48 * 1024) {
-            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (e != hipSuccess) return e;
-        }
-        kernel<<<groups, 256, lds, stream>>>(g);
-        return hipGetLastError();
-    };
-    if (g.a.tokens <= kFew) return yv ? go(adapter_up_kernel<BF, W, true, true>) : go(adapter_up_kernel<BF, W, false, true>);
-    return yv ? go(adapter_up_kernel<BF, W, true, false>) : go(adapter_up_kernel<BF, W, false, false>);
+    const bool one = g.a.rank <= 32;  // one step of ranks: more adapters' loads at a time
+    auto go = [&](auto kernel) { return launch_lds(kernel, groups, 256, lds, stream, g); };
+    if (multiple(g.a.b, g.a.rank, 8)) {
+        if (yv) return one ? go(adapter_up_kernel<CB, BF, 8, true, 1>) : go(adapter_up_kernel<CB, BF, 8, true, 2>);
+        return one ? go(adapter_up_kernel<CB, BF, 8, false, 1>) : go(adapter_up_kernel<CB, BF, 8, false, 2>);
+    }
+    if (multiple(g.a.b, g.a.rank, 4)) {
+        if (yv) return one ? go(adapter_up_kernel<CB, BF, 4, true, 1>) : go(adapter_up_kernel<CB, BF, 4, true, 2>);
+        return go(adapter_up_kernel<CB, BF, 4, false, 2>);
+    }
+    return go(adapter_up_kernel<CB, BF, 1, false, 2>);
 }
 
 template <bool BF>
 hipError_t adapter_launch(const AdapterArgs &g, hipStream_t stream) {
-    const int64_t padded = g.affine ? ((int64_t)g.tiles + 7) / 8 * 8 : g.tiles;
-    if (padded * (g.blocks > g.slices ? g.blocks : g.slices) > INT32_MAX) return hipErrorInvalidConfiguration;
-    const unsigned down = (unsigned)(padded * g.slices), up = (unsigned)(padded * g.blocks);
+    const int64_t padded = g.chunk > 0 ? (int64_t)g.chunk * 8 : g.tiles, parts = (int64_t)g.slices * g.slots;
+    if (padded * (g.blocks > parts ? g.blocks : parts) > INT32_MAX) return hipErrorInvalidConfiguration;
+    const unsigned down = (unsigned)(padded * parts), up = (unsigned)(padded * g.blocks);
     if (g.a.count > 0) {
-        if (g.a.rank <= 16) down_launch<1, BF>(g, down, stream);
-        else if (g.a.rank <= 32) down_launch<2, BF>(g, down, stream);
-        else down_launch<4, BF>(g, down, stream);
-        hipError_t e = hipGetLastError();
+        hipError_t e = g.a.rank <= 16 ? down_launch<1, BF>(g, down, stream)
+                     : g.a.rank <= 32 ? down_launch<2, BF>(g, down, stream)
+                                      : down_launch<4, BF>(g, down, stream);
         if (e != hipSuccess) return e;
     }
-    if (multiple(g.a.b, g.a.rank, 8)) return up_launch<BF, 8>(g, up, stream);
-    if (multiple(g.a.b, g.a.rank, 4)) return up_launch<BF, 4>(g, up, stream);
-    return up_launch<BF, 1>(g, up, stream);
+    return g.a.tokens <= kFew ? up_launch<1, BF>(g, up, stream) : up_launch<4, BF>(g, up, stream);
 }
 
 }  // namespace
