@@ -65,29 +65,38 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs &g, int64_t m) {
     return i >= 0 && i < g.a.count ? i : -1;
 }
 
-// Eight 16-bit elements from p; those from `left` on are zero.  W: elements
-// of a load that pointers and row lengths allow.
+// Eight 16-bit elements from p; those from `left` on are zero, and nothing
+// past them is read (`safe` stands in).  W: elements of a load that pointers
+// and row lengths allow.  The loads are not behind branches: a branch would
+// make the waves wait for every load in flight.
 template <int W>
-__device__ __forceinline__ u32x4 load8(const uint16_t *p, int64_t left) {
+__device__ __forceinline__ u32x4 load8(const uint16_t *p, int64_t left, const uint16_t *safe) {
     u32x4 v = {0u, 0u, 0u, 0u};
     if constexpr (W == 8) {
-        if (left > 0) v = *reinterpret_cast<const u32x4 *>(p);
+        v = *reinterpret_cast<const u32x4 *>(left > 0 ? p : safe);
+        if (!(left > 0)) v = u32x4{0u, 0u, 0u, 0u};
     } else if constexpr (W == 4) {
-        if (left > 0) {
-            const uint2 a = *reinterpret_cast<const uint2 *>(p);
-            v[0] = a.x;
-            v[1] = a.y;
-        }
-        if (left > 4) {
-            const uint2 b = *reinterpret_cast<const uint2 *>(p + 4);
-            v[2] = b.x;
-            v[3] = b.y;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint2 a = *reinterpret_cast<const uint2 *>(left > 4 * h ? p + 4 * h : safe);
+            v[2 * h] = left > 4 * h ? a.x : 0u;
+            v[2 * h + 1] = left > 4 * h ? a.y : 0u;
         }
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
             if (e < left) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
     }
+    return v;
+}
+
+// The same with all eight there.
+template <int W>
+__device__ __forceinline__ u32x4 load8(const uint16_t *p) {
+    if constexpr (W == 8) return *reinterpret_cast<const u32x4 *>(p);
+    u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
     return v;
 }
 
@@ -127,14 +136,16 @@ __device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&ac
     }
 }
 
-// The steps of this wave in a slice: [s, end).
-__device__ __forceinline__ void down_steps(const AdapterArgs &g, int slice, int *s, int *end) {
-    const int wave = threadIdx.x >> 6, share = (g.steps + kDown - 1) / kDown;
-    const int all = (int)((g.a.in_features + 31) / 32), last = (slice + 1) * g.steps;
+// The whole steps of this wave in a slice: [s, end); true where the step that
+// in_features ends inside follows them.
+__device__ __forceinline__ bool down_steps(const AdapterArgs &g, int slice, int *s, int *end) {
+    const int wave = threadIdx.x >> 6, share = (g.steps + kDown - 1) / kDown, last = (slice + 1) * g.steps;
+    const int whole = (int)(g.a.in_features / 32);
     *s = slice * g.steps + wave * share;
-    *end = *s + share;
-    if (*end > last) *end = last;
-    if (*end > all) *end = all;
+    int e = *s + share;
+    e = e < last ? e : last;
+    *end = e < whole ? e : whole;
+    return g.a.in_features % 32 != 0 && *s <= whole && whole < e;
 }
 
 // A slice for one of a 16-token tile's adapters: a workgroup reads its part
@@ -154,20 +165,28 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int i
 #pragma unroll
     for (int r = 0; r < RB; r++) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     int s, end;
-    down_steps(g, slice, &s, &end);
+    const bool tail = down_steps(g, slice, &s, &end);
+    const u32x4 zero = {0u, 0u, 0u, 0u};
     for (; s < end; s += U) {
         u32x4 x[U], a[U][RB];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t k = (int64_t)(s + u) * 32, left = s + u < end ? K - k - 8 * lg : 0;
-            x[u] = load8<W>(xp + k, left);
+            const int64_t k = (int64_t)(s + u < end ? s + u : end - 1) * 32;
+            x[u] = load8<W>(xp + k);
 #pragma unroll
-            for (int r = 0; r < RB; r++) a[u][r] = load8<W>(ap[r] + k, left);
+            for (int r = 0; r < RB; r++) a[u][r] = load8<W>(ap[r] + k);
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int r = 0; r < RB; r++) acc[0][r] = mfma<BF>(a[u][r], x[u], acc[0][r]);
+            for (int r = 0; r < RB; r++)
+                acc[0][r] = mfma<BF>(s + u < end ? a[u][r] : zero, s + u < end ? x[u] : zero, acc[0][r]);
+    }
+    if (tail) {
+        const int64_t k = K / 32 * 32, left = K - k - 8 * lg;
+        const u32x4 x = load8<W>(xp + k, left, xp - 8 * lg);
+#pragma unroll
+        for (int r = 0; r < RB; r++) acc[0][r] = mfma<BF>(load8<W>(ap[r] + k, left, ap[r] - 8 * lg), x, acc[0][r]);
     }
     down_join<RB, 1>(g, acc, m0, own, rank0, slice, lds);
 }
@@ -204,56 +223,85 @@ __device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int r
     for (int c = 0; c < 4; c++)
 #pragma unroll
         for (int r = 0; r < RB; r++) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int s, end;
-    down_steps(g, slice, &s, &end);
-    auto load = [&](int at, int id, u32x4 a[RB], u32x4 *x) {
-        const int64_t k = (int64_t)at * 32, left = at < end ? K - k - 8 * lg : 0;
-        const uint16_t *p = (const uint16_t *)g.a.a + (int64_t)id * g.a.rank * K + k;
-        if (x) {
+    int s, end, id0;
+    const bool tail = down_steps(g, slice, &s, &end);
+    auto stack = [&](int id) { return (const uint16_t *)g.a.a + (int64_t)id * g.a.rank * K; };
+    auto load_x = [&](int at, u32x4 x[4]) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) x[c] = load8<W>(xp[c] + k, left);
-        }
-#pragma unroll
-        for (int r = 0; r < RB; r++) a[r] = load8<W>(p + row[r], left);
+        for (int c = 0; c < 4; c++) x[c] = load8<W>(xp[c] + (int64_t)at * 32);
     };
-    auto product = [&](const u32x4 a[RB], const u32x4 x[4], uint64_t same) {
+    auto load_a = [&](int at, const uint16_t *p, u32x4 a[RB]) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint32_t tokens = (uint32_t)(same >> (16 * c)) & 0xffffu;
-            if (!tokens) continue;
-            if (tokens == 0xffffu) {
-#pragma unroll
-                for (int r = 0; r < RB; r++) acc[c][r] = mfma<BF>(a[r], x[c], acc[c][r]);
-                continue;
-            }
-            f32x4 t[RB];
-#pragma unroll
-            for (int r = 0; r < RB; r++) t[r] = mfma<BF>(a[r], x[c], acc[c][r]);
-            if (tokens >> col & 1) {
-#pragma unroll
-                for (int r = 0; r < RB; r++) acc[c][r] = t[r];
-            }
-        }
+        for (int r = 0; r < RB; r++) a[r] = load8<W>(p + row[r] + (int64_t)at * 32);
     };
-    u32x4 x[2][4], a[2][RB];
-    int id0;
+    auto product = [&](const u32x4 a[RB], const u32x4 x[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int r = 0; r < RB; r++) acc[c][r] = mfma<BF>(a[r], x[c], acc[c][r]);
+    };
+    auto product_of = [&](const u32x4 a[RB], const u32x4 x[4], uint64_t same) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                const f32x4 t = mfma<BF>(a[r], x[c], acc[c][r]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[c][r][i] = same >> (16 * c + col) & 1 ? t[i] : acc[c][r][i];
+            }
+    };
     uint64_t rest = own;
     const uint64_t same0 = take(rest, id0);
-    load(s, id0, a[0], x[0]);
-    auto step = [&](int at, u32x4 an[RB], u32x4 xn[4], const u32x4 ac[RB], const u32x4 xc[4]) {
-        load(at + 1, id0, an, xn);
-        product(ac, xc, same0);
-        for (uint64_t todo = rest; todo;) {
-            int id;
-            u32x4 b[RB];
-            const uint64_t same = take(todo, id);
-            load(at, id, b, nullptr);
-            product(b, xc, same);
+    const uint16_t *a0 = stack(id0);
+    u32x4 x[2][4], a[2][RB];
+    if (s < end) {
+        load_x(s, x[0]);
+        load_a(s, a0, a[0]);
+    }
+    if (!rest) {  // (one adapter: the other columns are not written)
+        while (s < end) {
+            const int n1 = s + 1 < end ? s + 1 : s;
+            load_x(n1, x[1]);
+            load_a(n1, a0, a[1]);
+            product(a[0], x[0]);
+            if (++s == end) break;
+            const int n0 = s + 1 < end ? s + 1 : s;
+            load_x(n0, x[0]);
+            load_a(n0, a0, a[0]);
+            product(a[1], x[1]);
+            s++;
         }
-    };
-    for (; s < end; s += 2) {
-        step(s, a[1], x[1], a[0], x[0]);
-        step(s + 1, a[0], x[0], a[1], x[1]);
+    } else {
+        for (; s < end; s++) {
+            const int n = s + 1 < end ? s + 1 : s;
+            load_x(n, x[1]);
+            load_a(n, a0, a[1]);
+            product_of(a[0], x[0], same0);
+            for (uint64_t todo = rest; todo;) {
+                int id;
+                u32x4 b[RB];
+                const uint64_t same = take(todo, id);
+                load_a(s, stack(id), b);
+                product_of(b, x[0], same);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) x[0][c] = x[1][c];
+#pragma unroll
+            for (int r = 0; r < RB; r++) a[0][r] = a[1][r];
+        }
+    }
+    if (tail) {
+        const int64_t k = K / 32 * 32, left = K - k - 8 * lg;
+#pragma unroll
+        for (int c = 0; c < 4; c++) x[0][c] = load8<W>(xp[c] + k, left, xp[c] - 8 * lg);
+        for (uint64_t todo = own; todo;) {
+            int id;
+            const uint64_t same = take(todo, id);
+            const uint16_t *p = stack(id);
+#pragma unroll
+            for (int r = 0; r < RB; r++) a[0][r] = load8<W>(p + row[r] + k, left, p);
+            product_of(a[0], x[0], same);
+        }
     }
     down_join<RB, 4>(g, acc, m0, own, rank0, slice, lds);
 }
@@ -411,8 +459,9 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
         const bool on = held >> (16 * c + col) & 1;
         const uint16_t *y = (const uint16_t *)g.a.y + (on ? m0 + 16 * c + col : m0) * g.a.y_stride + n;
         if constexpr (YV) {
-            yv[c][0] = load8<8>(y, on ? N - n : 0);
-            yv[c][1] = load8<8>(y + 8, on ? N - n - 8 : 0);
+            // (a token that is not this wave's: the first's, not used)
+            yv[c][0] = load8<8>(y, N - n, (const uint16_t *)g.a.y);
+            yv[c][1] = load8<8>(y + 8, N - n - 8, (const uint16_t *)g.a.y);
         } else {
 #pragma unroll
             for (int e = 0; e < 16; e++) ys[c][e] = on && n + e < N ? y[e] : 0;
@@ -431,23 +480,23 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
 #pragma unroll
         for (int i = 0; i < IDS; i++) {
             same[i] = 0;
-            ids[i] = 0;
+            ids[i] = i > 0 ? ids[0] : 0;  // (none left: the first's loads again)
             if (todo) same[i] = take(todo, ids[i]);
         }
     };
     auto load_b = [&](int kk0) {
 #pragma unroll
-        for (int i = 0; i < IDS; i++)
-            if (same[i]) {
-                const uint16_t *b = (const uint16_t *)g.a.b + (int64_t)ids[i] * N * g.a.rank + 32 * kk0;
+        for (int i = 0; i < IDS; i++) {
+            const uint16_t *b = (const uint16_t *)g.a.b + (int64_t)ids[i] * N * g.a.rank;
 #pragma unroll
-                for (int k = 0; k < KB; k++)
+            for (int k = 0; k < KB; k++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++) bv[i][k][t] = load8<W>(b + row[t] + 32 * k, g.a.rank - 32 * (kk0 + k) - 8 * lg);
-            }
+                for (int t = 0; t < 4; t++)
+                    bv[i][k][t] = load8<W>(b + row[t] + 32 * (kk0 + k), g.a.rank - 32 * (kk0 + k) - 8 * lg, b);
+        }
     };
     next();
-    load_b(0);
+    if (same[0]) load_b(0);
 
     // the low-rank values
     const int tl = CB == 1 ? mine : __shfl(mine, 16 * wave + col, 64);
@@ -516,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
                 }
         }
         next();
-        load_b(0);
+        if (same[0]) load_b(0);
     }
 #pragma unroll
     for (int c = 0; c < CB; c++) {

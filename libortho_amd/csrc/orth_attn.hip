@@ -30,6 +30,8 @@
 // share (of some 100 tokens in one load and one scan).  A share that ends
 // inside a (token, key head) leaves a piece (m, l, o) for a second launch to
 // join; whole ones are written at once.
+#include <type_traits>
+
 #include "orth_serve.h"
 
 namespace orth {
@@ -38,7 +40,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                // keys a wave takes at a time
-constexpr int kUnit = kTile * kWaves;    // keys a workgroup takes at a time
 constexpr float kLeast = -3.0e38f;       // the maximum of a token that has seen keys, at the least
 
 struct AttendArgs {
@@ -48,10 +49,11 @@ struct AttendArgs {
     float scale2;        // scale * log2(e)
     int group, gtiles;   // query heads of a key head, and their tiles of 16
     int gt;              // query heads of a tile: min(group, 16)
+    int nh, nsub;        // head tiles a workgroup takes at once, and the waves of each: nh * nsub = 4
     uint32_t min_units;  // the least share of a workgroup
-    float *part;         // pieces [workgroups * 2][gt][head_dim]
-    float2 *stat;        // (m, l) [workgroups * 2][16]
-    int4 *split;         // [workgroups]: (token, head tile, slot, last workgroup) of the split item that starts there
+    float *part;         // pieces [workgroups * 2][nh][gt][head_dim]
+    float2 *stat;        // (m, l) [workgroups * 2][nh][16]
+    int4 *split;         // [workgroups]: (token, item, slot, last workgroup) of the split item that starts there
 };
 
 struct Keys {
@@ -72,35 +74,44 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     k.end = (int)(end > INT32_MAX ? INT32_MAX : end);
     k.tile0 = k.begin / kTile;
     k.tiles = (int)(((int64_t)k.end + kTile - 1) / kTile) - k.tile0;
-    k.units = k.tiles > kWaves ? (uint32_t)(k.tiles + kWaves - 1) / kWaves : 1;  // (one that sees nothing is written too)
+    k.units = k.tiles > g.nsub ? (uint32_t)(k.tiles + g.nsub - 1) / g.nsub : 1;  // (one that sees nothing is written too)
     return k;
 }
 
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+// Inclusive sums over the wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    auto add = [&](auto ctrl, auto rows) {
+        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15, 31
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
     return v;
 }
 
-// Inclusive sums of the units of tokens t0 + 4 lane .. + 3, in u[4].
-__device__ __forceinline__ uint64_t block_units(const AttendArgs &g, int64_t t0, int lane, uint32_t u[4]) {
-    uint64_t s = 0;
+// Inclusive sums of the units of tokens t0 + 2 lane, + 1, in u[2].  (32 bits
+// hold them: a token has at most 2^24 units of four tiles, or of one tile
+// where the launch has seen that its table holds no more than 2^28 keys.)
+constexpr int kScan = 128;
+__device__ __forceinline__ uint32_t block_units(const AttendArgs &g, int64_t t0, int lane, uint32_t u[2]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int64_t t = t0 + 4 * lane + i;
+    for (int i = 0; i < 2; i++) {
+        const int64_t t = t0 + 2 * lane + i;
         u[i] = t < g.a.tokens ? keys_of(g, t).units : 0;
-        s += u[i];
     }
-    return wave_scan64(s, lane);
+    return wave_scan(u[0] + u[1]);
 }
 
 // The maximum over the four lanes that hold one column.
 __device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const uint32_t u = __float_as_uint(v);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1])));
+    const auto q = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor(v, 16, 64);
@@ -143,51 +154,45 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     extern __shared__ float lds[];  // o [waves][gt][16 EL + 4], then (m, l) [waves][16]
     const int D = g.c.head_dim, row_floats = 16 * EL + 4;
     float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, lg = lane >> 4;
-    const int heads = g.c.kv_heads * g.gtiles;  // items of a token
+    const int items = g.c.kv_heads * g.gtiles / g.nh;  // items of a token
+    const int hw = wave / g.nsub, sub = wave - hw * g.nsub;
 
     // ------------------------------------------------ this workgroup's share
-    uint32_t mine[4];
-    uint64_t run = 0, incl = 0;
-    for (int64_t t0 = 0; t0 < g.a.tokens; t0 += 256) {
+    uint32_t mine[2], incl = 0;
+    uint64_t run = 0;
+    for (int64_t t0 = 0; t0 < g.a.tokens; t0 += kScan) {
         incl = block_units(g, t0, lane, mine);
-        run += __shfl(incl, 63, 64);
+        run += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
-    const uint64_t total = run * heads;
+    const uint64_t total = run * items;
     uint64_t per = (total + gridDim.x - 1) / gridDim.x;
     per = per < g.min_units ? g.min_units : per;
     uint64_t cur = blockIdx.x * per;
     const uint64_t first = cur, stop = cur + per < total ? cur + per : total;
-    if (threadIdx.x == 0 && g.split) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
+    if (threadIdx.x == 0) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
     if (cur >= total) return;
-    const uint64_t want = cur / heads;  // the unit, were the heads one
+    const uint64_t want = cur / items;  // the unit, were a token one item
     int64_t t = 0;
     uint64_t before = 0;  // units of the tokens in front of t
-    for (int64_t t0 = 0;; t0 += 256) {
-        if (g.a.tokens > 256) incl = block_units(g, t0, lane, mine);
-        const uint64_t all = __shfl(incl, 63, 64);
+    for (int64_t t0 = 0;; t0 += kScan) {
+        if (g.a.tokens > kScan) incl = block_units(g, t0, lane, mine);
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
         if (before + all > want) {
-            const uint64_t m = __ballot(before + incl > want);
-            const int l = __ffsll((unsigned long long)m) - 1;
-            uint64_t b = before + __shfl(incl, l, 64);
-            int i = 3;
-#pragma unroll
-            for (int k = 3; k >= 0; k--) {
-                const uint32_t u = __shfl(mine[k], l, 64);
-                if (b > want) {
-                    b -= u;
-                    i = k;
-                }
-            }
-            t = t0 + 4 * l + i;
-            before = b;
+            const uint32_t at = (uint32_t)(want - before);
+            const int l = __ffsll((unsigned long long)__ballot(incl > at)) - 1;
+            const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)incl, l);
+            const uint32_t u1 = (uint32_t)__builtin_amdgcn_readlane((int)mine[1], l), u0 = (uint32_t)__builtin_amdgcn_readlane((int)mine[0], l);
+            const bool second = end - u1 <= at;
+            t = t0 + 2 * l + (second ? 1 : 0);
+            before += second ? end - u1 : end - u1 - u0;
             break;
         }
         before += all;
     }
     Keys k = keys_of(g, t);
-    const uint64_t inside = cur - before * heads;
+    const uint64_t inside = cur - before * items;
     int item = (int)(inside / k.units);
     uint32_t unit = (uint32_t)(inside - (uint64_t)item * k.units);
 
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     while (cur < stop) {
         const uint64_t left = stop - cur;
         const uint32_t n = k.units - unit < left ? k.units - unit : (uint32_t)left;
-        const int kvh = item / g.gtiles, gt0 = (item - kvh * g.gtiles) * 16;  // first query head of the tile
+        const int ht = item * g.nh + hw, kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;  // first query head of the tile
         const int cols = g.group - gt0 < 16 ? g.group - gt0 : 16;
         const int64_t q_head = (int64_t)kvh * g.group + gt0;
 
@@ -224,8 +229,9 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         const uint16_t *kbase = (const uint16_t *)g.c.k_cache + kvh * g.c.k_strides[2];
         const uint16_t *vbase = (const uint16_t *)g.c.v_cache + kvh * g.c.v_strides[2];
         const int last = k.end - 1;
-        const int tile_end = k.tile0 + (int)((unit + n) * kWaves < (uint32_t)k.tiles ? (unit + n) * kWaves : (uint32_t)k.tiles);
-        int tile = k.tile0 + (int)(unit * kWaves) + wave;
+        const uint64_t upto = (uint64_t)(unit + n) * g.nsub;
+        const int step = g.nsub, tile_end = k.tile0 + (int)(upto < (uint64_t)k.tiles ? upto : (uint64_t)k.tiles);
+        int tile = k.tile0 + (int)unit * g.nsub + sub;
 
         f32x4 o[EL];
         float m = -__builtin_inff(), l = 0.f;
@@ -318,12 +324,12 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             load_v(tile, ve);
             ve_now = ve;
             if constexpr (PG8) {
-                ke = entry8((tile + kWaves) * kTile + (col >> 2) * 8);
-                ve = entry8((tile + kWaves) * kTile + lg * 8);
+                ke = entry8((tile + step) * kTile + (col >> 2) * 8);
+                ve = entry8((tile + step) * kTile + lg * 8);
             }
         }
-        for (; tile < tile_end; tile += kWaves) {
-            const bool more = tile + kWaves < tile_end;
+        for (; tile < tile_end; tile += step) {
+            const bool more = tile + step < tile_end;
             f32x4 s[2];
 #pragma unroll
             for (int tau = 0; tau < 2; tau++) {
@@ -339,10 +345,10 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             __builtin_amdgcn_sched_barrier(0);
             int32_t ve_next = ve;
             if (more) {
-                load_k(tile + kWaves, ke);
+                load_k(tile + step, ke);
                 if constexpr (PG8) {
-                    ke = entry8((tile + 2 * kWaves) * kTile + (col >> 2) * 8);
-                    ve = entry8((tile + 2 * kWaves) * kTile + lg * 8);
+                    ke = entry8((tile + 2 * step) * kTile + (col >> 2) * 8);
+                    ve = entry8((tile + 2 * step) * kTile + lg * 8);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -408,13 +414,13 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_v(tile + kWaves, ve_next);
+            if (more) load_v(tile + step, ve_next);
             ve_now = ve_next;
             __builtin_amdgcn_sched_barrier(0);
         }
         l = column_sum(l);
 
-        // join the four waves
+        // join the waves of each head tile
         if (col < cols) {
             float *dst = lds + (wave * g.gt + col) * row_floats;
 #pragma unroll
@@ -428,24 +434,25 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         const bool whole = n == k.units;
         const int slot = (int)blockIdx.x * 2 + (cur == first ? 0 : 1);
         const int chunks = D / 8;  // eight elements of one query head a thread
-        for (int x = threadIdx.x; x < cols * chunks; x += 256) {
-            const int h = x / chunks, d = (x - h * chunks) * 8;
-            float top = -__builtin_inff(), sum = 0.f, w[kWaves];
-#pragma unroll
-            for (int v = 0; v < kWaves; v++) top = fmaxf(top, lds_stat[v * 16 + h].x);
-            const float base = top == -__builtin_inff() ? 0.f : top;
+        for (int x = threadIdx.x; x < g.nh * g.gt * chunks; x += 256) {
+            const int hx = x / chunks, d = (x - hx * chunks) * 8, hh = hx / g.gt, h = hx - hh * g.gt;
+            const int tile_x = item * g.nh + hh, kv = tile_x / g.gtiles, head0 = (tile_x - kv * g.gtiles) * 16;
+            if (head0 + h >= g.group) continue;
+            float top = -__builtin_inff(), sum = 0.f;
             float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int v = 0; v < kWaves; v++) {
-                w[v] = __builtin_amdgcn_exp2f(lds_stat[v * 16 + h].x - base);
-                sum += w[v] * lds_stat[v * 16 + h].y;
+            for (int v = hh * g.nsub; v < (hh + 1) * g.nsub; v++) top = fmaxf(top, lds_stat[v * 16 + h].x);
+            const float base = top == -__builtin_inff() ? 0.f : top;
+            for (int v = hh * g.nsub; v < (hh + 1) * g.nsub; v++) {
+                const float2 st = lds_stat[v * 16 + h];
+                const float w = __builtin_amdgcn_exp2f(st.x - base);
+                sum += w * st.y;
                 const float *src = lds + (v * g.gt + h) * row_floats + d;
 #pragma unroll
-                for (int i = 0; i < 8; i++) r[i] += w[v] * src[i];
+                for (int i = 0; i < 8; i++) r[i] += w * src[i];
             }
             if (whole) {
                 const bool nothing = top == -__builtin_inff();
-                uint16_t *out = (uint16_t *)g.a.out + t * g.a.out_strides[0] + (q_head + h) * g.a.out_strides[1] + d;
+                uint16_t *out = (uint16_t *)g.a.out + t * g.a.out_strides[0] + ((int64_t)kv * g.group + head0 + h) * g.a.out_strides[1] + d;
                 uint16_t y[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) y[i] = store16<BF>(nothing ? 0.f : r[i] / sum);
@@ -459,10 +466,11 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                     for (int i = 0; i < 8; i++) out[i] = y[i];
                 }
             } else {
-                float *dst = g.part + ((int64_t)slot * g.gt + h) * D + d;
+                const int64_t piece = (int64_t)slot * g.nh + hh;
+                float *dst = g.part + (piece * g.gt + h) * D + d;
                 *reinterpret_cast<f32x4 *>(dst) = f32x4{r[0], r[1], r[2], r[3]};
                 *reinterpret_cast<f32x4 *>(dst + 4) = f32x4{r[4], r[5], r[6], r[7]};
-                if (d == 0) g.stat[slot * 16 + h] = float2{top, sum};
+                if (d == 0) g.stat[piece * 16 + h] = float2{top, sum};
             }
         }
         if (!whole && unit == 0 && threadIdx.x == 0)
@@ -470,7 +478,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         __syncthreads();
         cur += n;
         unit = 0;
-        if (++item == heads) {
+        if (++item == items) {
             item = 0;
             t++;
             if (cur < stop) k = keys_of(g, t);
@@ -478,64 +486,150 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     }
 }
 
-// Joins the pieces of the split item that starts in workgroup blockIdx.x, for
-// query head blockIdx.y of its tile.
+// Joins the pieces of the split item that starts in workgroup blockIdx.x.  Up
+// to kFewPieces: a thread takes four elements of all pieces.  More (few
+// tokens, long): a workgroup a query head, a thread four elements of every
+// 256 / (head_dim / 4)-th piece, eight in flight.
+constexpr int kFewPieces = 16;
 template <bool BF>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
     const int4 s = g.split[blockIdx.x];
     if (s.x < 0) return;
-    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = g.c.head_dim;
-    const int kvh = s.y / g.gtiles, gt0 = (s.y - kvh * g.gtiles) * 16;
-    if (gt0 + h >= g.group) return;
-    const int n = s.w - (int)blockIdx.x + 1;
-    auto slot = [&](int i) -> int64_t { return i == 0 ? s.z : ((int64_t)blockIdx.x + i) * 2; };
-    float top = -__builtin_inff();
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, g.stat[slot(i) * 16 + h].x);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = g.c.head_dim, quads = D / 4, at_once = 256 / quads;
+    const int n = s.w - (int)blockIdx.x + 1, p0 = tid / quads, q = tid - p0 * quads;
+    if (n <= kFewPieces) {
+        for (int x = blockIdx.y * 256 + tid; x < g.nh * g.gt * quads; x += gridDim.y * 256) {
+            const int hx = x / quads, e4 = (x - hx * quads) * 4, hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
+            const int kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;
+            if (gt0 + h >= g.group) continue;
+            auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)blockIdx.x + i) * 2) * g.nh + hh; };
+            f32x4 r = {0.f, 0.f, 0.f, 0.f};
+            float top = -__builtin_inff(), sum = 0.f;
+            for (int i0 = 0; i0 < n; i0 += 4) {
+                f32x4 v[4];
+                float2 st[4];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    __shared__ f32x4 acc[4][64];
-    __shared__ float sums[4];
-    f32x4 r = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    const bool on = 4 * lane < D;
-#pragma unroll 4
-    for (int i = wave; i < n; i += 4) {
-        const float2 st = g.stat[slot(i) * 16 + h];
-        const float w = __builtin_amdgcn_exp2f(st.x - base);
-        sum += w * st.y;
-        if (on) {
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(g.part + (slot(i) * g.gt + h) * D + 4 * lane);
+                for (int u = 0; u < 4; u++) {
+                    const int64_t p = piece(i0 + u < n ? i0 + u : n - 1);
+                    st[u] = g.stat[p * 16 + h];
+                    v[u] = *reinterpret_cast<const f32x4 *>(g.part + (p * g.gt + h) * D + e4);
+                }
+                float most = top;
 #pragma unroll
-            for (int e = 0; e < 4; e++) r[e] += w * v[e];
+                for (int u = 0; u < 4; u++) most = fmaxf(most, st[u].x);  // (the last one again where there are fewer)
+                const float base = most == -__builtin_inff() ? 0.f : most, keep = __builtin_amdgcn_exp2f(top - base);
+                sum *= keep;
+#pragma unroll
+                for (int e = 0; e < 4; e++) r[e] *= keep;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if (i0 + u >= n) continue;
+                    const float w = __builtin_amdgcn_exp2f(st[u].x - base);
+                    sum += w * st[u].y;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) r[e] += w * v[u][e];
+                }
+                top = most;
+            }
+            const int64_t head = (int64_t)kvh * g.group + gt0 + h;
+            uint16_t *out = (uint16_t *)g.a.out + s.x * g.a.out_strides[0] + head * g.a.out_strides[1] + e4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / sum);
         }
+        return;
     }
-    acc[wave][lane] = r;
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (wave == 0 && on) {
-        float den = 0.f;
-        r = f32x4{0.f, 0.f, 0.f, 0.f};
+    __shared__ f32x4 acc[256];
+    __shared__ float weight[256], red[8];
+    for (int hx = blockIdx.y; hx < g.nh * g.gt; hx += gridDim.y) {
+        const int hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
+        const int kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;
+        if (gt0 + h >= g.group) continue;
+        auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)blockIdx.x + i) * 2) * g.nh + hh; };
+        float top = -__builtin_inff();
+        for (int i = tid; i < n; i += 256) top = fmaxf(top, g.stat[piece(i) * 16 + h].x);
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-            den += sums[v];
+        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        f32x4 r = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+        for (int i0 = 0; i0 < n; i0 += 256) {  // 256 weights at a time
+            if (i0 > 0) __syncthreads();
+            if (i0 + tid < n) {
+                const float2 st = g.stat[piece(i0 + tid) * 16 + h];
+                const float w = __builtin_amdgcn_exp2f(st.x - base);
+                weight[tid] = w;
+                sum += w * st.y;
+            }
+            __syncthreads();
+            const int m = n - i0 < 256 ? n - i0 : 256;
+            if (p0 < at_once)
+                for (int i = p0; i < m; i += 8 * at_once) {
+                    f32x4 v[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) r[e] += acc[v][lane][e];
+                    for (int u = 0; u < 8; u++) {
+                        const int x = i + u * at_once < m ? i + u * at_once : i;
+                        v[u] = *reinterpret_cast<const f32x4 *>(g.part + (piece(i0 + x) * g.gt + h) * D + 4 * q);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const float w = i + u * at_once < m ? weight[i + u * at_once] : 0.f;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) r[e] += i + u * at_once < m ? w * v[u][e] : 0.f;
+                    }
+                }
         }
-        const int64_t head = (int64_t)kvh * g.group + gt0 + h;
-        uint16_t *out = (uint16_t *)g.a.out + s.x * g.a.out_strides[0] + head * g.a.out_strides[1] + 4 * lane;
+        acc[tid] = r;
 #pragma unroll
-        for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / den);
+        for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if (lane == 0) red[4 + wave] = sum;
+        __syncthreads();
+        if (tid < quads) {
+            const float den = (red[4] + red[5]) + (red[6] + red[7]);
+            for (int p = 1; p < at_once; p++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) r[e] += acc[p * quads + tid][e];
+            const int64_t head = (int64_t)kvh * g.group + gt0 + h;
+            uint16_t *out = (uint16_t *)g.a.out + s.x * g.a.out_strides[0] + head * g.a.out_strides[1] + 4 * tid;
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / den);
+        }
+        __syncthreads();
     }
 }
 
 // The resident workgroups, and no more than there can be units.
-int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int gtiles) {
+int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, const AttendArgs &g) {
     const int64_t groups = (int64_t)cus * (c.head_dim > 128 ? 1 : c.head_dim > 64 ? 2 : 3);
-    const int64_t held = a.table_width > kUnit * (int64_t)INT32_MAX / c.page_size ? INT32_MAX : a.table_width * c.page_size;
-    int64_t keys = a.window > 0 && a.window + kTile < held ? a.window + kTile : held;
-    const int64_t units = keys / kUnit + 1, items = a.tokens * c.kv_heads * gtiles;
+    const int64_t held = a.table_width > INT32_MAX / c.page_size ? INT32_MAX : a.table_width * c.page_size;
+    const int64_t keys = a.window > 0 && (int64_t)a.window + kTile < held ? (int64_t)a.window + kTile : held;
+    const int64_t units = keys / (kTile * g.nsub) + 1, items = a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh);
     return items > groups / units ? groups : items * units;
+}
+
+// What both the workspace and the launch go by.
+AttendArgs attend_args(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups) {
+    AttendArgs g;
+    g.c = c;
+    g.a = a;
+    g.page = fast_div((uint32_t)c.page_size);
+    g.scale2 = a.scale * 1.4426950408889634f;
+    g.group = a.q_heads / c.kv_heads;
+    g.gtiles = (g.group + 15) / 16;
+    g.gt = g.group < 16 ? g.group : 16;
+    // Four or two head tiles a workgroup where there are items enough: its
+    // waves then read neighbouring heads of the same keys and need no join.
+    // Few items are cut along the keys instead, so that their pieces are few.
+    const int64_t tiles = (int64_t)c.kv_heads * g.gtiles;
+    g.nh = 1;
+    const bool few_keys = a.table_width <= ((int64_t)1 << 28) / c.page_size;  // (block_units)
+    while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && a.tokens * (tiles / (2 * g.nh)) >= cus / 4) g.nh *= 2;
+    g.nsub = kWaves / g.nh;
+    g.min_units = 2;
+    *groups = attend_groups(c, a, cus, g);
+    return g;
 }
 
 template <int KS, bool BF>
@@ -563,33 +657,29 @@ hipError_t attend_by_width(const AttendArgs &g, int64_t groups, hipStream_t stre
                  : D <= 128 ? attend_launch<4, BF>(g, groups, lds, stream)
                             : attend_launch<8, BF>(g, groups, lds, stream);
     if (e != hipSuccess) return e;
-    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)g.gt), 256, 0, stream>>>(g);
+    // many items have few pieces each: the workgroups that 256 threads a
+    // four elements make; few items have many: one a head
+    const int64_t items = g.a.tokens * (g.c.kv_heads * (int64_t)g.gtiles / g.nh), heads = g.nh * g.gt;
+    const int64_t y = items * kFewPieces >= groups ? (heads * (D / 4) + 255) / 256 : heads;
+    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)y), 256, 0, stream>>>(g);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus) {
-    const int group = a.q_heads / c.kv_heads;
-    const int64_t groups = attend_groups(c, a, cus, (group + 15) / 16);
-    return groups * (2 * (group < 16 ? group : 16) * (int64_t)c.head_dim * 4 + 2 * 16 * (int64_t)sizeof(float2) + (int64_t)sizeof(int4));
+    int64_t groups = 0;
+    const AttendArgs g = attend_args(c, a, cus, &groups);
+    return groups * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2)) + (int64_t)sizeof(int4));
 }
 
 hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work,
                                   hipStream_t stream) {
-    AttendArgs g;
-    g.c = c;
-    g.a = a;
-    g.page = fast_div((uint32_t)c.page_size);
-    g.scale2 = a.scale * 1.4426950408889634f;
-    g.group = a.q_heads / c.kv_heads;
-    g.gtiles = (g.group + 15) / 16;
-    g.gt = g.group < 16 ? g.group : 16;
-    g.min_units = 2;
-    const int64_t groups = attend_groups(c, a, cus, g.gtiles);
+    int64_t groups = 0;
+    AttendArgs g = attend_args(c, a, cus, &groups);
     g.split = static_cast<int4 *>(work);
     g.stat = reinterpret_cast<float2 *>(g.split + groups);
-    g.part = reinterpret_cast<float *>(g.stat + groups * 2 * 16);
+    g.part = reinterpret_cast<float *>(g.stat + groups * 2 * g.nh * 16);
     return c.dtype == ORTH_DT_BF16 ? attend_by_width<true>(g, groups, stream) : attend_by_width<false>(g, groups, stream);
 }
 
