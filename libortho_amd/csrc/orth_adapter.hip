@@ -28,8 +28,9 @@ namespace orth {
 namespace {
 
 constexpr int kTokens = 64;    // tokens of a tile, where they are many
-constexpr int kFew = 256;      // up to here, tiles of 16: decode batches, whose adapters differ by token
+constexpr int kFew = 512;      // up to here, tiles of 16: decode batches, whose adapters differ by token
 constexpr int kUp = 64;        // outputs a wave takes at a time
+constexpr int kShared = 4;     // adapters of a 64-token tile up to which each has a pass of its own
 constexpr int kDown = 8;       // waves of a down workgroup: steps in flight without more partials to add
 
 struct AdapterArgs {
@@ -38,7 +39,7 @@ struct AdapterArgs {
     int tiles;         // of 16 or 64 tokens
     int slices, steps; // slices of in_features, and steps of 32 in each
     int blocks;        // up: blocks of out_features
-    int slots;         // down, 16 tokens: adapters of a tile, a workgroup each
+    int slots;         // down: workgroups that share the adapters of a tile
     int chunk;         // tiles of an XCD (0: too few to keep together)
 };
 
@@ -46,8 +47,7 @@ struct AdapterArgs {
 // XCDs, eight in turn, so XCD x takes the x-th eighth of the tiles: tiles of
 // one prompt share its adapter in that XCD's L2, and a tile's partials are
 // read from the L2 they were written to.
-__device__ __forceinline__ void place_of(const AdapterArgs &g, int parts, int *tile, int *part) {
-    const int b = blockIdx.x;
+__device__ __forceinline__ void place_of(const AdapterArgs &g, int b, int parts, int *tile, int *part) {
     if (g.chunk > 0) {
         const int x = b & 7, q = b >> 3, at = q / parts;
         *tile = at < g.chunk ? x * g.chunk + at : g.tiles;
@@ -110,28 +110,25 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
 
 // ------------------------------------------------------------------------ down
 
-// The workgroup's sum of a product: 16 RB ranks by 16 CB tokens of each wave,
-// joined in LDS ([waves][16 RB][16 CB + 1]); those of the tokens in `own` are
-// written as this slice's partial.
-template <int RB, int CB>
-__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&acc)[CB][RB], int64_t m0, uint64_t own,
-                                          int rank0, int slice, float *lds) {
-    constexpr int kRow = 16 * CB + 1;
+// The workgroup's sum of a product of each wave, 16 RB ranks by 16 tokens,
+// joined in LDS ([waves][16 RB][17]); the tokens in `own` are written as this
+// slice's partial.
+template <int RB>
+__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&acc)[RB], int64_t m0, uint32_t own, int rank0,
+                                          int slice, float *lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     __syncthreads();  // the last use of lds is over
 #pragma unroll
-    for (int c = 0; c < CB; c++)
+    for (int r = 0; r < RB; r++)
 #pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) lds[(wave * 16 * RB + 16 * r + 4 * lg + i) * kRow + 16 * c + col] = acc[c][r][i];
+        for (int i = 0; i < 4; i++) lds[(wave * 16 * RB + 16 * r + 4 * lg + i) * 17 + col] = acc[r][i];
     __syncthreads();
-    for (int x = threadIdx.x; x < 256 * RB * CB; x += 64 * kDown) {
+    for (int x = threadIdx.x; x < 256 * RB; x += 64 * kDown) {
         const int j = x % (16 * RB), t = x / (16 * RB);
         if (!(own >> t & 1) || rank0 + j >= g.a.rank) continue;
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kDown; w++) sum += lds[(w * 16 * RB + j) * kRow + t];
+        for (int w = 0; w < kDown; w++) sum += lds[(w * 16 * RB + j) * 17 + t];
         g.low[((int64_t)slice * g.a.tokens + m0 + t) * g.a.rank + rank0 + j] = sum;
     }
 }
@@ -161,9 +158,9 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int i
         const int j = rank0 + 16 * r + col;
         ap[r] = (const uint16_t *)g.a.a + ((int64_t)id * g.a.rank + (j < g.a.rank ? j : g.a.rank - 1)) * K + 8 * lg;
     }
-    f32x4 acc[1][RB];
+    f32x4 acc[RB];
 #pragma unroll
-    for (int r = 0; r < RB; r++) acc[0][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < RB; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     int s, end;
     const bool tail = down_steps(g, slice, &s, &end);
     const u32x4 zero = {0u, 0u, 0u, 0u};
@@ -180,142 +177,193 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int i
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int r = 0; r < RB; r++)
-                acc[0][r] = mfma<BF>(s + u < end ? a[u][r] : zero, s + u < end ? x[u] : zero, acc[0][r]);
+                acc[r] = mfma<BF>(s + u < end ? a[u][r] : zero, s + u < end ? x[u] : zero, acc[r]);
     }
     if (tail) {
         const int64_t k = K / 32 * 32, left = K - k - 8 * lg;
         const u32x4 x = load8<W>(xp + k, left, xp - 8 * lg);
 #pragma unroll
-        for (int r = 0; r < RB; r++) acc[0][r] = mfma<BF>(load8<W>(ap[r] + k, left, ap[r] - 8 * lg), x, acc[0][r]);
+        for (int r = 0; r < RB; r++) acc[r] = mfma<BF>(load8<W>(ap[r] + k, left, ap[r] - 8 * lg), x, acc[r]);
     }
-    down_join<RB, 1>(g, acc, m0, own, rank0, slice, lds);
+    down_join<RB>(g, acc, m0, own, rank0, slice, lds);
 }
 
-// A slice for 64 tokens and every adapter among them; the loads of the next
-// step's tokens and first adapter go ahead of this one's products.
+// A slice for 64 tokens of many adapters: each step's tokens with every
+// adapter in turn, the products kept in their own tokens' columns.
 template <int RB, bool BF, int W>
 __device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int rank0, int slice, float *lds) {
+    constexpr int IDS = RB == 1 ? 4 : 2;  // adapters whose loads are in flight together
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t K = g.a.in_features;
     const int mine = adapter_of(g, m0 + lane);
     const uint64_t own = __ballot(mine >= 0);
     if (!own) return;
-    auto take = [&](uint64_t &todo, int &id) -> uint64_t {  // the next adapter and its tokens
-        id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
-        const uint64_t same = __ballot(mine == id);
-        todo &= ~same;
-        return same;
-    };
     const uint16_t *xp[4];
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const int64_t m = m0 + 16 * c + col;
-        xp[c] = (const uint16_t *)g.a.x + (m < g.a.tokens ? m : g.a.tokens - 1) * g.a.x_stride + 8 * lg;
+        xp[c] = (const uint16_t *)g.a.x + (m < g.a.tokens ? m : g.a.tokens - 1) * g.a.x_stride;
     }
     int64_t row[RB];
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         const int j = rank0 + 16 * r + col;
-        row[r] = (j < g.a.rank ? j : g.a.rank - 1) * K + 8 * lg;
+        row[r] = (j < g.a.rank ? j : g.a.rank - 1) * K;
     }
     f32x4 acc[4][RB];
 #pragma unroll
     for (int c = 0; c < 4; c++)
 #pragma unroll
         for (int r = 0; r < RB; r++) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int s, end, id0;
-    const bool tail = down_steps(g, slice, &s, &end);
-    auto stack = [&](int id) { return (const uint16_t *)g.a.a + (int64_t)id * g.a.rank * K; };
-    auto load_x = [&](int at, u32x4 x[4]) {
+    int s, end;
+    if (down_steps(g, slice, &s, &end)) end++;  // (the step that in_features ends inside among them: all loads are checked)
+    for (; s < end; s++) {
+        const int64_t k = (int64_t)s * 32 + 8 * lg;
+        u32x4 x[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) x[c] = load8<W>(xp[c] + (int64_t)at * 32);
-    };
-    auto load_a = [&](int at, const uint16_t *p, u32x4 a[RB]) {
-#pragma unroll
-        for (int r = 0; r < RB; r++) a[r] = load8<W>(p + row[r] + (int64_t)at * 32);
-    };
-    auto product = [&](const u32x4 a[RB], const u32x4 x[4]) {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int r = 0; r < RB; r++) acc[c][r] = mfma<BF>(a[r], x[c], acc[c][r]);
-    };
-    auto product_of = [&](const u32x4 a[RB], const u32x4 x[4], uint64_t same) {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const f32x4 t = mfma<BF>(a[r], x[c], acc[c][r]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[c][r][i] = same >> (16 * c + col) & 1 ? t[i] : acc[c][r][i];
-            }
-    };
-    uint64_t rest = own;
-    const uint64_t same0 = take(rest, id0);
-    const uint16_t *a0 = stack(id0);
-    u32x4 x[2][4], a[2][RB];
-    if (s < end) {
-        load_x(s, x[0]);
-        load_a(s, a0, a[0]);
-    }
-    if (!rest) {  // (one adapter: the other columns are not written)
-        while (s < end) {
-            const int n1 = s + 1 < end ? s + 1 : s;
-            load_x(n1, x[1]);
-            load_a(n1, a0, a[1]);
-            product(a[0], x[0]);
-            if (++s == end) break;
-            const int n0 = s + 1 < end ? s + 1 : s;
-            load_x(n0, x[0]);
-            load_a(n0, a0, a[0]);
-            product(a[1], x[1]);
-            s++;
-        }
-    } else {
-        for (; s < end; s++) {
-            const int n = s + 1 < end ? s + 1 : s;
-            load_x(n, x[1]);
-            load_a(n, a0, a[1]);
-            product_of(a[0], x[0], same0);
-            for (uint64_t todo = rest; todo;) {
-                int id;
-                u32x4 b[RB];
-                const uint64_t same = take(todo, id);
-                load_a(s, stack(id), b);
-                product_of(b, x[0], same);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[0][c] = x[1][c];
-#pragma unroll
-            for (int r = 0; r < RB; r++) a[0][r] = a[1][r];
-        }
-    }
-    if (tail) {
-        const int64_t k = K / 32 * 32, left = K - k - 8 * lg;
-#pragma unroll
-        for (int c = 0; c < 4; c++) x[0][c] = load8<W>(xp[c] + k, left, xp[c] - 8 * lg);
+        for (int c = 0; c < 4; c++) x[c] = load8<W>(xp[c] + k, K - k, xp[c]);
         for (uint64_t todo = own; todo;) {
-            int id;
-            const uint64_t same = take(todo, id);
-            const uint16_t *p = stack(id);
+            int id[IDS];
+            u32x4 a[IDS][RB];
+            uint64_t same[IDS];
 #pragma unroll
-            for (int r = 0; r < RB; r++) a[0][r] = load8<W>(p + row[r] + k, left, p);
-            product_of(a[0], x[0], same);
+            for (int i = 0; i < IDS; i++) {
+                same[i] = 0;
+                id[i] = i > 0 ? id[0] : 0;  // (none left: the first's loads again)
+                if (todo) {
+                    id[i] = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
+                    same[i] = __ballot(mine == id[i]);
+                    todo &= ~same[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < IDS; i++) {
+                const uint16_t *p = (const uint16_t *)g.a.a + (int64_t)id[i] * g.a.rank * K;
+#pragma unroll
+                for (int r = 0; r < RB; r++) a[i][r] = load8<W>(p + row[r] + k, K - k, p);
+            }
+#pragma unroll
+            for (int i = 0; i < IDS; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < RB; r++) {
+                        const f32x4 t = mfma<BF>(a[i][r], x[c], acc[c][r]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[c][r][e] = same[i] >> (16 * c + col) & 1 ? t[e] : acc[c][r][e];
+                    }
         }
     }
-    down_join<RB, 4>(g, acc, m0, own, rank0, slice, lds);
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t o = (uint32_t)(own >> (16 * c)) & 0xffffu;
+        if (o) down_join<RB>(g, acc[c], m0 + 16 * c, o, rank0, slice, lds);
+    }
+}
+
+// A slice for 64 tokens and one adapter, through LDS: stages of 64 columns of
+// the tokens' rows and of A, read in whole 128-byte lines (16 bytes a lane
+// straight into the operands touch each line twice, and the L1 does not hold
+// it that long), kAhead stages of them in flight in registers, written to LDS
+// with the 16-byte chunks of a row permuted by the row (no bank is hit twice).
+// The waves split the product, so there is no sum over them.
+constexpr int kAhead = 6;
+template <int RB, bool BF>
+__device__ __forceinline__ void down_staged(const AdapterArgs &g, int64_t m0, int id, uint64_t own, int rank0, int slice,
+                                            u32x4 *lds) {
+    constexpr int kRows = 64 + 16 * RB, kLoads = (kRows * 8 + 64 * kDown - 1) / (64 * kDown);  // rows of a stage, chunks a thread
+    constexpr int kCols = RB == 4 ? 2 : 1;  // token groups of a wave
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, lg = lane >> 4;
+    const int64_t K = g.a.in_features;
+    const int k0 = slice * g.steps * 32;
+    const int64_t stop = (int64_t)k0 + g.steps * 32 < K ? (int64_t)k0 + g.steps * 32 : K;
+    const int stages = (int)((stop - k0 + 63) / 64);
+    const uint16_t *src[kLoads];
+    int at[kLoads], chunk[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+        int row = (tid + i * 64 * kDown) >> 3;
+        chunk[i] = tid & 7;
+        if (row >= kRows) row = kRows - 1;  // (a copy, written to the same place)
+        at[i] = row * 8 + (chunk[i] ^ (row & 7));
+        if (row < 64) {
+            const int64_t m = m0 + row < g.a.tokens ? m0 + row : g.a.tokens - 1;
+            src[i] = (const uint16_t *)g.a.x + m * g.a.x_stride;
+        } else {
+            const int j = rank0 + row - 64;
+            src[i] = (const uint16_t *)g.a.a + ((int64_t)id * g.a.rank + (j < g.a.rank ? j : g.a.rank - 1)) * K;
+        }
+    }
+    u32x4 held[kAhead][kLoads];
+    auto load = [&](int stage, u32x4 v[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int64_t k = (int64_t)k0 + 64 * stage + 8 * chunk[i];
+            v[i] = load8<8>(src[i] + k, stop - k, src[i]);
+        }
+    };
+    f32x4 acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; c++) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int rb = wave % RB, cg = RB == 4 ? wave / 4 * 2 : wave / RB;  // its ranks and first token group (from four on: none)
+    const bool works = cg < 4;
+#pragma unroll
+    for (int d = 0; d < kAhead; d++) load(d, held[d]);
+    for (int s0 = 0; s0 < stages; s0 += kAhead) {
+#pragma unroll
+        for (int d = 0; d < kAhead; d++) {
+            if (s0 + d >= stages) break;
+            u32x4 *buf = lds + (d & 1) * kRows * 8;  // (kAhead is even)
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) buf[at[i]] = held[d][i];
+            // every wave has written this stage, and is done with the last
+            // one's buffer, which the next stage goes to; loads stay in flight
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            load(s0 + d + kAhead, held[d]);
+            if (works) {
+                const int ar = 64 + 16 * rb + col;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const u32x4 a = buf[ar * 8 + ((4 * u + lg) ^ (ar & 7))];
+#pragma unroll
+                    for (int c = 0; c < kCols; c++) {
+                        const int xr = 16 * (cg + c) + col;
+                        acc[c] = mfma<BF>(a, buf[xr * 8 + ((4 * u + lg) ^ (xr & 7))], acc[c]);
+                    }
+                }
+            }
+        }
+    }
+    if (works) {
+#pragma unroll
+        for (int c = 0; c < kCols; c++) {
+            const int t = 16 * (cg + c) + col, j = rank0 + 16 * rb + 4 * lg;
+            if (!(own >> t & 1)) continue;
+            float *dst = g.low + ((int64_t)slice * g.a.tokens + m0 + t) * g.a.rank + j;
+            if (g.a.rank % 4 == 0) {
+                if (j < g.a.rank) *reinterpret_cast<f32x4 *>(dst) = acc[c];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (j + i < g.a.rank) dst[i] = acc[c][i];
+            }
+        }
+    }
+    __syncthreads();  // the buffers are free for the next pass
 }
 
 template <int RB, int CB, bool BF, int W>
-__global__ __launch_bounds__(64 * kDown) void adapter_down_kernel(AdapterArgs g) {
+__global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs g) {
     extern __shared__ float down_lds[];
-    int tile, part;
-    place_of(g, CB == 1 ? g.slices * g.slots : g.slices, &tile, &part);
+    // (all first slots in front: most others end at once)
+    const int per_slot = gridDim.x / g.slots, slot = blockIdx.x / per_slot;
+    int tile, slice;
+    place_of(g, blockIdx.x - slot * per_slot, g.slices, &tile, &slice);
     if (tile >= g.tiles) return;
     const int64_t m0 = (int64_t)tile * 16 * CB;
     if constexpr (CB == 1) {
         // the slot's adapter: the slot-th token that is its adapter's first
-        const int slice = part / g.slots, slot = part - slice * g.slots, col = threadIdx.x & 15;
+        const int col = threadIdx.x & 15;
         const int mine = adapter_of(g, m0 + col);
         bool first = mine >= 0;
 #pragma unroll
@@ -330,7 +378,28 @@ __global__ __launch_bounds__(64 * kDown) void adapter_down_kernel(AdapterArgs g)
         const uint32_t own = (uint32_t)__ballot(mine == id) & 0xffffu;
         for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m0, id, own, r, slice, down_lds);
     } else {
-        for (int r = 0; r < g.a.rank; r += 16 * RB) down_all<RB, BF, W>(g, m0, r, part, down_lds);
+        // up to kShared adapters: the slots take them in turn; more: the
+        // first slot takes all at once
+        constexpr int kAll = RB < 2 ? RB : 2;
+        const int mine = adapter_of(g, m0 + (threadIdx.x & 63));
+        const uint64_t own = __ballot(mine >= 0);
+        int distinct = 0;
+        for (uint64_t todo = own; todo && distinct <= kShared; distinct++)
+            todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1));
+        if (W != 8 || distinct > kShared) {
+            if (slot == 0)
+                for (int r = 0; r < g.a.rank; r += kAll * 16) down_all<kAll, BF, W>(g, m0, r, slice, down_lds);
+            return;
+        }
+        int k = 0;
+        for (uint64_t todo = own; todo; k++) {
+            const int id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
+            const uint64_t same = __ballot(mine == id);
+            todo &= ~same;
+            if (k % g.slots != slot) continue;
+            for (int r = 0; r < g.a.rank; r += 16 * RB)
+                down_staged<RB, BF>(g, m0, id, same, r, slice, reinterpret_cast<u32x4 *>(down_lds));
+        }
     }
 }
 
@@ -424,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
     extern __shared__ u32x4 parts[];           // [4][kks][2][64]
     __shared__ int shifts[kTokens];
     int tile, block;
-    place_of(g, g.blocks, &tile, &block);
+    place_of(g, blockIdx.x, g.blocks, &tile, &block);
     if (tile >= g.tiles) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     const int kks = (g.a.rank + 31) / 32, each = kks * 128;
@@ -612,12 +681,13 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     const bool few = a.tokens <= kFew;
     int64_t most = a.tokens < 16 ? a.tokens : 16;
     if (a.count < most) most = a.count < 1 ? 1 : a.count;
-    g.slots = few ? (int)most : 1;
-    int64_t slices = (int64_t)cus / (g.tiles * (int64_t)g.slots);
+    g.slots = few ? (int)most : 2;  // (many tokens: a tile mostly has one adapter, or two where a run ends)
+    int64_t slices = (int64_t)cus / (g.tiles * (int64_t)(few ? g.slots : 1));
     if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;
     if (slices > 8) slices = 8;
     if (slices < 1) slices = 1;
     g.steps = (int)((steps + slices - 1) / slices);
+    if (!few) g.steps += g.steps & 1;  // whole 128-byte lines
     g.slices = (int)((steps + g.steps - 1) / g.steps);
     const int64_t span = few ? kUp : 4 * kUp;
     g.blocks = (int)((a.out_features + span - 1) / span);
@@ -642,7 +712,8 @@ hipError_t launch_lds(Kernel kernel, unsigned groups, int threads, size_t lds, h
 template <int RB, bool BF>
 hipError_t down_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
     const bool few = g.a.tokens <= kFew, wide = multiple(g.a.x, g.a.x_stride, 8) && multiple(g.a.a, g.a.in_features, 8);
-    const size_t lds = (size_t)kDown * 16 * RB * ((few ? 16 : kTokens) + 1) * sizeof(float);
+    const size_t join = (size_t)kDown * 16 * RB * 17 * sizeof(float), staged = (size_t)2 * (64 + 16 * RB) * 128;
+    const size_t lds = few || join > staged ? join : staged;
     auto go = [&](auto kernel) { return launch_lds(kernel, groups, 64 * kDown, lds, stream, g); };
     if (few) return wide ? go(adapter_down_kernel<RB, 1, BF, 8>) : go(adapter_down_kernel<RB, 1, BF, 1>);
     return wide ? go(adapter_down_kernel<RB, 4, BF, 8>) : go(adapter_down_kernel<RB, 4, BF, 1>);

@@ -54,7 +54,9 @@ def check(y, x, a, b, ids, scales=None, out=None):
 @pytest.mark.parametrize("M,K,N,r,n", [
     (1, 4096, 4096, 16, 1), (3, 512, 700, 8, 2), (16, 256, 256, 32, 5), (33, 1024, 1000, 64, 3), (64, 512, 1536, 16, 64),
     (65, 512, 512, 128, 1), (130, 264, 333, 20, 7), (257, 1000, 999, 4, 4), (70, 96, 64, 256, 3), (40, 128, 130, 1, 3),
-    (9, 33, 17, 5, 2), (12, 1, 1, 3, 2), (300, 2048, 512, 24, 2), (5, 11008, 4096, 40, 9)])
+    (9, 33, 17, 5, 2), (12, 1, 1, 3, 2), (300, 2048, 512, 24, 2), (5, 11008, 4096, 40, 9), (600, 1000, 200, 64, 1),
+    (577, 512, 264, 16, 3), (700, 264, 128, 32, 4), (513, 320, 130, 20, 5), (1000, 128, 136, 8, 64), (530, 200, 72, 200, 2),
+    (640, 96, 80, 100, 20), (520, 77, 40, 12, 3), (515, 40, 33, 7, 9)])
 def test_adapters(gpu, M, K, N, r, n, dtype):
     check(*case(M, K, N, r, n, DT[dtype]))
 
@@ -63,6 +65,10 @@ def test_no_scales_in_place_and_runs(gpu):
     y, x, a, b, ids, _ = case(200, 512, 640, 16, 3, torch.float16)
     ids = torch.sort(ids).values.contiguous()
     want = check(y, x, a, b, ids)
+    # runs that end inside tiles of many tokens
+    wide = case(900, 512, 640, 32, 5, torch.bfloat16)
+    runs = torch.sort(wide[4]).values.contiguous()
+    check(*wide[:4], runs, wide[5])
     y2 = y.clone()
     got = _C_ops.adapter_add(y2, x, a, b, ids, out=y2)
     assert got.data_ptr() == y2.data_ptr() and torch.equal(y2, want)
@@ -107,16 +113,31 @@ def test_large_and_small_values(gpu):
     check(y, x, a, b, ids, s)
 
 
-def test_infinities_and_nan_stay_in_their_tokens(gpu):
-    y, x, a, b, ids, s = case(40, 512, 256, 16, 3, torch.float16)
+@pytest.mark.parametrize("M", [40, 600])
+def test_infinities_and_nan_stay_in_their_tokens(gpu, M):
+    y, x, a, b, ids, s = case(M, 512, 256, 16, 3, torch.float16)
     ids.fill_(1)
     want = _C_ops.adapter_add(y, x, a, b, ids, s)
     x[7, 3] = float("inf")
     x[9, 5] = float("nan")
     got = _C_ops.adapter_add(y, x, a, b, ids, s)
-    keep = [m for m in range(40) if m not in (7, 9)]
+    keep = [m for m in range(M) if m not in (7, 9)]
     assert torch.equal(got[keep], want[keep])
     assert not bool(got[7].isfinite().any()) and bool(got[9].isnan().all())
+
+
+@pytest.mark.parametrize("M,n", [(30, 3), (600, 3), (600, 9)])
+def test_an_adapter_of_infinities_reaches_its_own_tokens_only(gpu, M, n):
+    y, x, a, b, ids, s = case(M, 256, 264, 16, n, torch.float16)
+    want = _C_ops.adapter_add(y, x, a, b, ids, s)
+    a[1, 3, 5] = float("inf")
+    b[2 % n, 7] = float("nan")
+    got = _C_ops.adapter_add(y, x, a, b, ids, s)
+    rest = (ids != 1) & (ids != 2)
+    assert torch.equal(got[rest], want[rest])
+    two = got[ids == 2]
+    assert bool(two[:, 7].isnan().all()) and bool(two[:, :7].isfinite().all())
+    assert not bool(got[ids == 1].isfinite().any())
 
 
 def test_same_bits_every_time_other_streams_and_replays(gpu):
