@@ -21,6 +21,8 @@
 // Bound by reading the adapters (few tokens: workgroups of 16 tokens, whose
 // waves split in_features, then the adapters) or x, y and out (many: 64
 // tokens a workgroup share each adapter's loads).
+#include <type_traits>
+
 #include "orth_serve.h"
 
 namespace orth {
@@ -41,6 +43,7 @@ struct AdapterArgs {
     int blocks;        // up: blocks of out_features
     int slots;         // down: workgroups that share the adapters of a tile
     int chunk;         // tiles of an XCD (0: too few to keep together)
+    int sorted;        // 16-token tiles take tokens by adapter (few_token)
 };
 
 // Workgroup -> (tile, part of it).  Neighbours in blockIdx go to different
@@ -63,6 +66,36 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs &g, int64_t m) {
     if (m >= g.a.tokens) return -1;
     const int i = g.a.adapters[m];
     return i >= 0 && i < g.a.count ? i : -1;
+}
+
+// The token of column lane & 15 of a 16-token tile, where tokens are few, and
+// its adapter (-1: none, or no token).  Where the stack has fewer adapters
+// than there are tokens, the four tiles of a window of 64 take its tokens in
+// the order of their adapters, so that the tokens of one adapter fall into
+// one tile, or two, and it is read so often.  False: the column has no token
+// (`m` then is some token's).
+__device__ __forceinline__ bool few_token(const AdapterArgs &g, int tile, int *m, int *mine) {
+    const int lane = threadIdx.x & 63, col = lane & 15, tokens = (int)g.a.tokens;
+    if (!g.sorted) {
+        const int at = tile * 16 + col;
+        *m = at < tokens ? at : tokens - 1;
+        *mine = adapter_of(g, at);
+        return at < tokens;
+    }
+    const int base = (tile >> 2) * 64, n = tokens - base < 64 ? tokens - base : 64;
+    const int id = adapter_of(g, base + lane);
+    // adapter, then token: tokens without an adapter after all others, places
+    // without a token last (`sorted` says that the numbers fit)
+    const uint32_t key = lane < n ? (uint32_t)(id >= 0 ? id : 1 << 25) * 64 + lane : 0xffffffc0u + lane;
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j++) at += (uint32_t)__builtin_amdgcn_readlane((int)key, j) < key;
+    const int order = __builtin_amdgcn_ds_permute(at * 4, lane);  // lane p: the p-th token of the window
+    const int p = (tile & 3) * 16 + col, t = __shfl(order, p, 64);
+    const int of = __shfl(id, t, 64);
+    *m = p < n ? base + t : tokens - 1;
+    *mine = p < n ? of : -1;
+    return p < n;
 }
 
 // Eight 16-bit elements from p; those from `left` on are zero, and nothing
@@ -111,10 +144,10 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
 // ------------------------------------------------------------------------ down
 
 // The workgroup's sum of a product of each wave, 16 RB ranks by 16 tokens,
-// joined in LDS ([waves][16 RB][17]); the tokens in `own` are written as this
-// slice's partial.
+// joined in LDS ([waves][16 RB][17]); the columns in `own` (column lane & 15 is
+// token m) are written as this slice's partial.
 template <int RB>
-__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&acc)[RB], int64_t m0, uint32_t own, int rank0,
+__device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&acc)[RB], int m, uint32_t own, int rank0,
                                           int slice, float *lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     __syncthreads();  // the last use of lds is over
@@ -124,12 +157,12 @@ __device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&ac
         for (int i = 0; i < 4; i++) lds[(wave * 16 * RB + 16 * r + 4 * lg + i) * 17 + col] = acc[r][i];
     __syncthreads();
     for (int x = threadIdx.x; x < 256 * RB; x += 64 * kDown) {
-        const int j = x % (16 * RB), t = x / (16 * RB);
+        const int j = x % (16 * RB), t = x / (16 * RB), token = __shfl(m, t, 64);
         if (!(own >> t & 1) || rank0 + j >= g.a.rank) continue;
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kDown; w++) sum += lds[(w * 16 * RB + j) * 17 + t];
-        g.low[((int64_t)slice * g.a.tokens + m0 + t) * g.a.rank + rank0 + j] = sum;
+        g.low[((int64_t)slice * g.a.tokens + token) * g.a.rank + rank0 + j] = sum;
     }
 }
 
@@ -148,10 +181,10 @@ __device__ __forceinline__ bool down_steps(const AdapterArgs &g, int slice, int 
 // A slice for one of a 16-token tile's adapters: a workgroup reads its part
 // of one A, all of a wave's loads in flight.
 template <int RB, bool BF, int W>
-__device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int id, uint32_t own, int rank0, int slice, float *lds) {
+__device__ __forceinline__ void down_one(const AdapterArgs &g, int m, int id, uint32_t own, int rank0, int slice, float *lds) {
     constexpr int U = RB == 1 ? 8 : 4;
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
-    const int64_t K = g.a.in_features, m = m0 + col < g.a.tokens ? m0 + col : g.a.tokens - 1;
+    const int64_t K = g.a.in_features;
     const uint16_t *xp = (const uint16_t *)g.a.x + m * g.a.x_stride + 8 * lg, *ap[RB];
 #pragma unroll
     for (int r = 0; r < RB; r++) {
@@ -185,7 +218,7 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int64_t m0, int i
 #pragma unroll
         for (int r = 0; r < RB; r++) acc[r] = mfma<BF>(load8<W>(ap[r] + k, left, ap[r] - 8 * lg), x, acc[r]);
     }
-    down_join<RB>(g, acc, m0, own, rank0, slice, lds);
+    down_join<RB>(g, acc, m, own, rank0, slice, lds);
 }
 
 // A slice for 64 tokens of many adapters: each step's tokens with every
@@ -257,7 +290,7 @@ __device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int r
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const uint32_t o = (uint32_t)(own >> (16 * c)) & 0xffffu;
-        if (o) down_join<RB>(g, acc[c], m0 + 16 * c, o, rank0, slice, lds);
+        if (o) down_join<RB>(g, acc[c], (int)m0 + 16 * c + col, o, rank0, slice, lds);
     }
 }
 
@@ -362,21 +395,37 @@ __global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs
     if (tile >= g.tiles) return;
     const int64_t m0 = (int64_t)tile * 16 * CB;
     if constexpr (CB == 1) {
-        // the slot's adapter: the slot-th token that is its adapter's first
+        // the slot's adapter: that of the slot-th column that is its
+        // adapter's first
         const int col = threadIdx.x & 15;
-        const int mine = adapter_of(g, m0 + col);
+        int m, mine;
+        few_token(g, tile, &m, &mine);
         bool first = mine >= 0;
-#pragma unroll
-        for (int d = 1; d < 16; d++) {
-            const int other = __shfl_up(mine, d, 16);  // (all lanes take part)
-            first &= !(col >= d && other == mine);
-        }
+        auto unlike = [&](auto d) {  // the adapter d columns before, within the row of 16 lanes
+            const int other = __builtin_amdgcn_update_dpp(-1, mine, 0x110 + decltype(d)::value, 0xf, 0xf, false);
+            first &= other != mine;
+        };
+        unlike(std::integral_constant<int, 1>{});
+        unlike(std::integral_constant<int, 2>{});
+        unlike(std::integral_constant<int, 3>{});
+        unlike(std::integral_constant<int, 4>{});
+        unlike(std::integral_constant<int, 5>{});
+        unlike(std::integral_constant<int, 6>{});
+        unlike(std::integral_constant<int, 7>{});
+        unlike(std::integral_constant<int, 8>{});
+        unlike(std::integral_constant<int, 9>{});
+        unlike(std::integral_constant<int, 10>{});
+        unlike(std::integral_constant<int, 11>{});
+        unlike(std::integral_constant<int, 12>{});
+        unlike(std::integral_constant<int, 13>{});
+        unlike(std::integral_constant<int, 14>{});
+        unlike(std::integral_constant<int, 15>{});
         uint32_t firsts = (uint32_t)__ballot(first) & 0xffffu;
         for (int i = 0; i < slot; i++) firsts &= firsts - 1;
         if (!firsts) return;
         const int id = __builtin_amdgcn_readlane(mine, __ffs(firsts) - 1);
         const uint32_t own = (uint32_t)__ballot(mine == id) & 0xffffu;
-        for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m0, id, own, r, slice, down_lds);
+        for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m, id, own, r, slice, down_lds);
     } else {
         // up to kShared adapters: the slots take them in turn; more: the
         // first slot takes all at once
@@ -498,10 +547,22 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
     const int kks = (g.a.rank + 31) / 32, each = kks * 128;
     const int64_t m0 = (int64_t)tile * 16 * CB, N = g.a.out_features;
-    const int mine = adapter_of(g, m0 + (CB == 1 ? col : lane));
-    const uint64_t own = __ballot(mine >= 0) & (CB == 1 ? 0xffffull : ~0ull);
-    const int64_t left = g.a.tokens - m0;
-    const uint64_t here = left >= 16 * CB ? (CB == 1 ? 0xffffull : ~0ull) : ((uint64_t)1 << left) - 1;
+    // the tokens: CB 1, of column col; CB 4, of lane
+    int mine, m1 = 0;
+    bool present;
+    if constexpr (CB == 1) {
+        present = few_token(g, tile, &m1, &mine);
+    } else {
+        mine = adapter_of(g, m0 + lane);
+        present = m0 + lane < g.a.tokens;
+    }
+    const uint64_t whole = CB == 1 ? 0xffffull : ~0ull;
+    const uint64_t own = __ballot(mine >= 0) & whole, here = __ballot(present) & whole;
+    auto token = [&](int c) -> int64_t {  // of column col of group c
+        if constexpr (CB == 1) return m1;
+        const int64_t m = m0 + 16 * c + col;
+        return m < g.a.tokens ? m : g.a.tokens - 1;
+    };
     auto take = [&](uint64_t &todo, int &id) -> uint64_t {  // the next adapter and its tokens
         id = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)todo) - 1);
         const uint64_t same = __ballot(mine == id) & own;
@@ -526,9 +587,9 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
 #pragma unroll
     for (int c = 0; c < CB; c++) {
         const bool on = held >> (16 * c + col) & 1;
-        const uint16_t *y = (const uint16_t *)g.a.y + (on ? m0 + 16 * c + col : m0) * g.a.y_stride + n;
+        const uint16_t *y = (const uint16_t *)g.a.y + token(c) * g.a.y_stride + n;
         if constexpr (YV) {
-            // (a token that is not this wave's: the first's, not used)
+            // (also of tokens that are not this wave's)
             yv[c][0] = load8<8>(y, N - n, (const uint16_t *)g.a.y);
             yv[c][1] = load8<8>(y + 8, N - n - 8, (const uint16_t *)g.a.y);
         } else {
@@ -549,13 +610,14 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
 #pragma unroll
         for (int i = 0; i < IDS; i++) {
             same[i] = 0;
-            ids[i] = i > 0 ? ids[0] : 0;  // (none left: the first's loads again)
+            ids[i] = 0;
             if (todo) same[i] = take(todo, ids[i]);
         }
     };
     auto load_b = [&](int kk0) {
 #pragma unroll
         for (int i = 0; i < IDS; i++) {
+            if (!same[i]) break;
             const uint16_t *b = (const uint16_t *)g.a.b + (int64_t)ids[i] * N * g.a.rank;
 #pragma unroll
             for (int k = 0; k < KB; k++)
@@ -565,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
         }
     };
     next();
-    if (same[0]) load_b(0);
+    load_b(0);
 
     // the low-rank values
     const int tl = CB == 1 ? mine : __shfl(mine, 16 * wave + col, 64);
@@ -573,7 +635,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
     if (__any(tl >= 0)) {
         for (int kk = 0; kk < kks; kk++) {
             f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            if (tl >= 0) low_sum<CB == 1 ? 2 : 4>(g, m0 + (CB == 1 ? 0 : 16 * wave) + col, 32 * kk + 8 * lg, CB == 1 ? wave : 0, CB == 1 ? 4 : 1, v);
+            if (tl >= 0) low_sum<CB == 1 ? 2 : 4>(g, token(wave), 32 * kk + 8 * lg, CB == 1 ? wave : 0, CB == 1 ? 4 : 1, v);
             if (CB > 1) {
                 v[0] *= scale;
                 v[1] *= scale;
@@ -634,13 +696,13 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
                 }
         }
         next();
-        if (same[0]) load_b(0);
+        load_b(0);
     }
 #pragma unroll
     for (int c = 0; c < CB; c++) {
         if (!(held >> (16 * c + col) & 1)) continue;
         const bool add = own >> (16 * c + col) & 1;
-        uint16_t *out = (uint16_t *)g.a.out + (m0 + 16 * c + col) * g.a.out_stride + n;
+        uint16_t *out = (uint16_t *)g.a.out + token(c) * g.a.out_stride + n;
         const int sh = !BF && add ? shifts[16 * c + col] : 0;
         uint16_t r[16];
 #pragma unroll
@@ -681,6 +743,7 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     const bool few = a.tokens <= kFew;
     int64_t most = a.tokens < 16 ? a.tokens : 16;
     if (a.count < most) most = a.count < 1 ? 1 : a.count;
+    g.sorted = few && a.tokens > 16 && a.count < a.tokens && a.count < (1 << 25);
     g.slots = few ? (int)most : 2;  // (many tokens: a tile mostly has one adapter, or two where a run ends)
     int64_t slices = (int64_t)cus / (g.tiles * (int64_t)(few ? g.slots : 1));
     if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;
