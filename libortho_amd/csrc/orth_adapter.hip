@@ -169,7 +169,7 @@ __device__ __forceinline__ void down_join(const AdapterArgs &g, const f32x4 (&ac
 // The whole steps of this wave in a slice: [s, end); true where the step that
 // in_features ends inside follows them.
 __device__ __forceinline__ bool down_steps(const AdapterArgs &g, int slice, int *s, int *end) {
-    const int wave = threadIdx.x >> 6, share = (g.steps + kDown - 1) / kDown, last = (slice + 1) * g.steps;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = (g.steps + kDown - 1) / kDown, last = (slice + 1) * g.steps;
     const int whole = (int)(g.a.in_features / 32);
     *s = slice * g.steps + wave * share;
     int e = *s + share;
@@ -182,7 +182,7 @@ __device__ __forceinline__ bool down_steps(const AdapterArgs &g, int slice, int 
 // of one A, all of a wave's loads in flight.
 template <int RB, bool BF, int W>
 __device__ __forceinline__ void down_one(const AdapterArgs &g, int m, int id, uint32_t own, int rank0, int slice, float *lds) {
-    constexpr int U = RB == 1 ? 8 : 4;
+    constexpr int U = 8 / RB;  // steps whose loads are in flight together
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t K = g.a.in_features;
     const uint16_t *xp = (const uint16_t *)g.a.x + m * g.a.x_stride + 8 * lg, *ap[RB];
@@ -196,21 +196,22 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int m, int id, ui
     for (int r = 0; r < RB; r++) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     int s, end;
     const bool tail = down_steps(g, slice, &s, &end);
-    const u32x4 zero = {0u, 0u, 0u, 0u};
     for (; s < end; s += U) {
         u32x4 x[U], a[U][RB];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t k = (int64_t)(s + u < end ? s + u : end - 1) * 32;
+            if (s + u >= end) break;
+            const int64_t k = (int64_t)(s + u) * 32;
             x[u] = load8<W>(xp + k);
 #pragma unroll
             for (int r = 0; r < RB; r++) a[u][r] = load8<W>(ap[r] + k);
         }
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++) {
+            if (s + u >= end) break;
 #pragma unroll
-            for (int r = 0; r < RB; r++)
-                acc[r] = mfma<BF>(s + u < end ? a[u][r] : zero, s + u < end ? x[u] : zero, acc[r]);
+            for (int r = 0; r < RB; r++) acc[r] = mfma<BF>(a[u][r], x[u], acc[r]);
+        }
     }
     if (tail) {
         const int64_t k = K / 32 * 32, left = K - k - 8 * lg;

@@ -30,8 +30,6 @@
 // share (of some 100 tokens in one load and one scan).  A share that ends
 // inside a (token, key head) leaves a piece (m, l, o) for a second launch to
 // join; whole ones are written at once.
-#include <type_traits>
-
 #include "orth_serve.h"
 
 namespace orth {
@@ -76,20 +74,6 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     k.tiles = (int)(((int64_t)k.end + kTile - 1) / kTile) - k.tile0;
     k.units = k.tiles > g.nsub ? (uint32_t)(k.tiles + g.nsub - 1) / g.nsub : 1;  // (one that sees nothing is written too)
     return k;
-}
-
-// Inclusive sums over the wave.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    auto add = [&](auto ctrl, auto rows) {
-        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
-    };
-    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
-    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
-    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
-    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
-    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15, 31
-    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
-    return v;
 }
 
 // Inclusive sums of the units of tokens t0 + 2 lane, + 1, in u[2].  (32 bits
@@ -191,7 +175,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         }
         before += all;
     }
-    Keys k = keys_of(g, t);
+    Keys k = keys_of(g, t);  // (from the L1: the scan has read them)
     const uint64_t inside = cur - before * items;
     int item = (int)(inside / k.units);
     uint32_t unit = (uint32_t)(inside - (uint64_t)item * k.units);

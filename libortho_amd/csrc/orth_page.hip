@@ -19,29 +19,32 @@ namespace {
 //
 // Bound by latency: one launch, in which every workgroup repeats the scan of
 // all requests (8 bytes each from the L2) instead of waiting for one that
-// does it, and then writes kStepThreads tokens.
-constexpr int kStepThreads = 1024;
-constexpr int kStepWaves = kStepThreads / 64;
+// does it, and then writes a token a thread.  The sums of a scan are 32 bits
+// wide where `tokens` allows it (64-bit ones took 2 us more for 16 requests:
+// a wave's scan is then a dozen LDS permutes instead of six adds).
+constexpr int kStepMost = 1024;  // threads of a workgroup (256 for up to 256 requests)
 
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
+__device__ __forceinline__ uint32_t scan_in_wave(uint32_t v) { return wave_scan(v); }
+__device__ __forceinline__ uint64_t scan_in_wave(uint64_t v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up(v, d, 64);
+        const uint64_t o = __shfl_up(v, d, 64);
         if (lane >= d) v += o;
     }
     return v;
 }
 
 // Inclusive prefix sums over the workgroup; `sums` holds a wave's total each.
-__device__ __forceinline__ int64_t group_scan(int64_t v, int64_t *sums, int64_t *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_scan(v, lane);
+template <class Sum>
+__device__ __forceinline__ Sum group_scan(Sum v, Sum *sums, Sum *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    v = scan_in_wave(v);
     __syncthreads();  // the last use of sums is over
     if (lane == 63) sums[wave] = v;
     __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kStepWaves; w++) {
+    Sum before = 0, all = 0;
+    for (int w = 0; w < waves; w++) {
         before += w < wave ? sums[w] : 0;
         all += sums[w];
     }
@@ -49,10 +52,11 @@ __device__ __forceinline__ int64_t group_scan(int64_t v, int64_t *sums, int64_t 
     return v + before;
 }
 
-__global__ __launch_bounds__(kStepThreads) void page_step_kernel(orth_hip_step_t s, FastDiv page) {
+template <class Sum>
+__global__ __launch_bounds__(kStepMost) void page_step_kernel(orth_hip_step_t s, FastDiv page) {
     extern __shared__ int32_t lds[];
-    int32_t *start = lds, *first = lds + s.requests;  // first page (-1: refused) and first place of each request
-    __shared__ int64_t sums[kStepWaves];
+    int32_t *start = lds, *first = lds + s.requests;  // first place and first page (-1: refused) of each request
+    __shared__ Sum sums[kStepMost / 64];
     __shared__ int32_t used, status;
     const int tid = threadIdx.x;
     int64_t head = s.pool[0];
@@ -62,14 +66,16 @@ __global__ __launch_bounds__(kStepThreads) void page_step_kernel(orth_hip_step_t
         status = 0;
     }
     int64_t places = 0, pages = head;
-    for (int64_t r0 = 0; r0 < s.requests; r0 += kStepThreads) {
+    for (int64_t r0 = 0; r0 < s.requests; r0 += blockDim.x) {
         const int64_t r = r0 + tid;
         const bool here = r < s.requests;
         const int64_t L = here ? s.lengths[r] : 0, n = here ? s.new_tokens[r] : 0, all = L + n;
-        int64_t total;
-        const int64_t end = places + group_scan(n > 0 ? n : 0, sums, &total);
-        const int64_t at = end - (n > 0 ? n : 0);
-        places += total;
+        // (a request of more than `tokens` fits nowhere, nor does any after it)
+        const int64_t wants = n <= 0 ? 0 : (n <= s.tokens ? n : s.tokens + 1);
+        Sum total;
+        const int64_t end = places + (int64_t)group_scan<Sum>((Sum)wants, sums, &total);
+        const int64_t at = end - wants;
+        places += (int64_t)total;
         bool ok = L >= 0 && n >= 0 && all <= INT32_MAX && end <= s.tokens;
         int64_t need = 0;
         if (ok) {
@@ -79,8 +85,8 @@ __global__ __launch_bounds__(kStepThreads) void page_step_kernel(orth_hip_step_t
             need = ok ? last - old : 0;
         }
         const bool room = ok;
-        const int64_t pend = pages + group_scan(need, sums, &total);
-        pages += total;
+        const int64_t pend = pages + (int64_t)group_scan<Sum>((Sum)need, sums, &total);
+        pages += (int64_t)total;
         ok = ok && (need == 0 || pend <= s.free_count);
         if (here) {
             start[r] = (int32_t)(at < s.tokens ? at : s.tokens);
@@ -100,7 +106,7 @@ __global__ __launch_bounds__(kStepThreads) void page_step_kernel(orth_hip_step_t
         s.pool_out[0] = used;
         s.pool_out[1] = status;
     }
-    const int64_t t = (int64_t)blockIdx.x * kStepThreads + tid;
+    const int64_t t = (int64_t)blockIdx.x * blockDim.x + tid;
     if (t >= s.tokens) return;
     int32_t row = -1, pos = -1;
     int64_t slot = -1;
@@ -294,15 +300,21 @@ void append_launch(const AppendArgs &g, dim3 grid, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_page_step(const orth_hip_step_t &s, hipStream_t stream) {
-    const int64_t groups = s.tokens > 0 ? (s.tokens + kStepThreads - 1) / kStepThreads : 1;
+    const int threads = s.requests <= 256 ? 256 : kStepMost;
+    const int64_t groups = s.tokens > 0 ? (s.tokens + threads - 1) / threads : 1;
     const size_t lds = (size_t)s.requests * 8;
-    if (lds > 48 * 1024) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(page_step_kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return e;
-    }
-    page_step_kernel<<<dim3((unsigned)groups), kStepThreads, lds, stream>>>(s, fast_div((uint32_t)s.page_size));
-    return hipGetLastError();
+    const FastDiv page = fast_div((uint32_t)s.page_size);
+    auto go = [&](auto kernel) -> hipError_t {
+        if (lds > 48 * 1024) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<dim3((unsigned)groups), threads, lds, stream>>>(s, page);
+        return hipGetLastError();
+    };
+    // (1024 requests' places, tokens + 1 at most each, and pages, one more)
+    return s.tokens <= (1 << 20) ? go(page_step_kernel<uint32_t>) : go(page_step_kernel<uint64_t>);
 }
 
 hipError_t launch_cache_append(const orth_hip_cache_t &c, const orth_hip_append_t &a, int cus, hipStream_t stream) {

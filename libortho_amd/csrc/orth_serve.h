@@ -33,6 +33,18 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, const FastDiv &f) {
     return (uint32_t)(((uint64_t)n * f.m) >> f.shift);
 }
 
+// Inclusive sums over the wave: DPP adds within rows of 16 lanes, then each
+// row's last sum to the rows behind it.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // 16-bit elements as float, and back (round to nearest even), by type.
 template <bool BF>
 __device__ __forceinline__ float load16(uint16_t b) {

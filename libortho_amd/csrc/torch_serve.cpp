@@ -75,6 +75,17 @@ void strides2(const at::Tensor &t, int64_t *s) {
     s[1] = stride_of(t, 1);
 }
 
+// n elements of an int32 tensor's storage from *at on, as a tensor of `type`.
+at::Tensor part_of(const at::Tensor &all, int64_t *at, int64_t n, at::ScalarType type) {
+    const int64_t words = type == at::kLong ? 2 : 1;
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                            c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_storage_offset(*at / words);
+    *at += n * words;
+    return t;
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 page_step(const at::Tensor &lengths, const at::Tensor &new_tokens, const at::Tensor &table, const at::Tensor &free_pages,
           const at::Tensor &pool, int64_t page_size, int64_t tokens) {
@@ -91,10 +102,12 @@ page_step(const at::Tensor &lengths, const at::Tensor &new_tokens, const at::Ten
     req(page_size >= 1 && page_size <= INT32_MAX, "page_size must be positive");
     req(tokens >= 0 && tokens <= INT32_MAX, "tokens must not be negative, at most 2^31 - 1");
     c10::DeviceGuard guard(dev);
-    const auto i32 = lengths.options();
-    at::Tensor lengths_out = at::empty({R}, i32), pool_out = at::empty({2}, i32), start = at::empty({R + 1}, i32),
-               rows = at::empty({tokens}, i32), positions = at::empty({tokens}, i32),
-               slots = at::empty({tokens}, i32.dtype(at::kLong));
+    // one allocation, six views of it (each of its own takes longer than the launch)
+    const at::Tensor all = at::empty({4 * tokens + 2 * R + 3}, lengths.options());
+    int64_t at = 0;
+    const at::Tensor slots = part_of(all, &at, tokens, at::kLong), rows = part_of(all, &at, tokens, at::kInt),
+                     positions = part_of(all, &at, tokens, at::kInt), lengths_out = part_of(all, &at, R, at::kInt),
+                     start = part_of(all, &at, R + 1, at::kInt), pool_out = part_of(all, &at, 2, at::kInt);
     orth_hip_step_t s{};
     s.lengths = static_cast<const int32_t *>(ptr(lengths));
     s.new_tokens = static_cast<const int32_t *>(ptr(new_tokens));
