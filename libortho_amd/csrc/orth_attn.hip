@@ -28,8 +28,9 @@
 // workgroups by the keys the tokens really see, which only the device knows:
 // every wave sums up the tokens' 128-key units and finds its workgroup's
 // share (of some 100 tokens in one load and one scan).  A share that ends
-// inside a (token, key head) leaves a piece (m, l, o) for a second launch to
-// join; whole ones are written at once.
+// inside a (token, key head) leaves a piece (m, l, o); the workgroup that
+// writes an item's last piece joins them, or a second launch where they are
+// many.  Whole items are written at once.
 #include "orth_serve.h"
 
 namespace orth {
@@ -52,6 +53,7 @@ struct AttendArgs {
     float *part;         // pieces [workgroups * 2][nh][gt][head_dim]
     float2 *stat;        // (m, l) [workgroups * 2][nh][16]
     int4 *split;         // [workgroups]: (token, item, slot, last workgroup) of the split item that starts there
+    uint32_t *arrived;   // [workgroups], zeros: the pieces of that item written so far; null: a second launch joins
 };
 
 struct Keys {
@@ -59,6 +61,23 @@ struct Keys {
     int tile0, tiles;
     uint32_t units;
 };
+
+// a / b, in 32 bits where both fit (a 64-bit division takes a quarter of a
+// microsecond, and a short call is a chain of such latencies).
+__device__ __forceinline__ uint64_t div64(uint64_t a, uint64_t b) {
+    if ((a | b) >> 32) return a / b;
+    return (uint32_t)a / (uint32_t)b;
+}
+
+// Memory of all XCDs: written through and read past the L2 of this one.
+__device__ __forceinline__ void store_shared(float *p, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared(const float *p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
 
 __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     const int64_t row = g.a.rows ? (int64_t)g.a.rows[t] : t;
@@ -76,17 +95,18 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     return k;
 }
 
-// Inclusive sums of the units of tokens t0 + 2 lane, + 1, in u[2].  (32 bits
+// Inclusive sums of the units of tokens t0 + 2 lane, + 1, whose keys are in k[2].  (32 bits
 // hold them: a token has at most 2^24 units of four tiles, or of one tile
 // where the launch has seen that its table holds no more than 2^28 keys.)
 constexpr int kScan = 128;
-__device__ __forceinline__ uint32_t block_units(const AttendArgs &g, int64_t t0, int lane, uint32_t u[2]) {
+__device__ __forceinline__ uint32_t block_units(const AttendArgs &g, int64_t t0, int lane, Keys k[2]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int64_t t = t0 + 2 * lane + i;
-        u[i] = t < g.a.tokens ? keys_of(g, t).units : 0;
+        k[i] = Keys{0, 0, 0, 0, 0};
+        if (t < g.a.tokens) k[i] = keys_of(g, t);
     }
-    return wave_scan(u[0] + u[1]);
+    return wave_scan(k[0].units + k[1].units);
 }
 
 // The maximum over the four lanes that hold one column.
@@ -135,6 +155,12 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     constexpr int VW = EL / 2;                          // words of them
     constexpr bool VTAIL = TAIL || 16 * EL != 32 * KS;
     constexpr float kShift = BF ? 0.f : 14.f;
+    // the arguments' lines into the scalar cache at once: read where they are
+    // first used, each would be waited for in turn
+    typedef const __attribute__((address_space(4))) uint32_t *Words;
+    const Words words = (Words)__builtin_amdgcn_kernarg_segment_ptr();
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(AttendArgs); i += 64) asm volatile("" ::"s"(words[i / 4]));
     extern __shared__ float lds[];  // o [waves][gt][16 EL + 4], then (m, l) [waves][16]
     const int D = g.c.head_dim, row_floats = 16 * EL + 4;
     float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
@@ -144,21 +170,23 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     const int hw = wave / g.nsub, sub = wave - hw * g.nsub;
 
     // ------------------------------------------------ this workgroup's share
-    uint32_t mine[2], incl = 0;
+    Keys mine[2];
+    uint32_t incl = 0;
     uint64_t run = 0;
     for (int64_t t0 = 0; t0 < g.a.tokens; t0 += kScan) {
         incl = block_units(g, t0, lane, mine);
         run += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
     const uint64_t total = run * items;
-    uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+    uint64_t per = div64(total + gridDim.x - 1, gridDim.x);
     per = per < g.min_units ? g.min_units : per;
     uint64_t cur = blockIdx.x * per;
     const uint64_t first = cur, stop = cur + per < total ? cur + per : total;
-    if (threadIdx.x == 0) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
+    if (threadIdx.x == 0 && !g.arrived) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
     if (cur >= total) return;
-    const uint64_t want = cur / items;  // the unit, were a token one item
+    const uint64_t want = div64(cur, items);  // the unit, were a token one item
     int64_t t = 0;
+    Keys k;
     uint64_t before = 0;  // units of the tokens in front of t
     for (int64_t t0 = 0;; t0 += kScan) {
         if (g.a.tokens > kScan) incl = block_units(g, t0, lane, mine);
@@ -167,17 +195,22 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             const uint32_t at = (uint32_t)(want - before);
             const int l = __ffsll((unsigned long long)__ballot(incl > at)) - 1;
             const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)incl, l);
-            const uint32_t u1 = (uint32_t)__builtin_amdgcn_readlane((int)mine[1], l), u0 = (uint32_t)__builtin_amdgcn_readlane((int)mine[0], l);
+            const uint32_t u1 = (uint32_t)__builtin_amdgcn_readlane((int)mine[1].units, l);
             const bool second = end - u1 <= at;
             t = t0 + 2 * l + (second ? 1 : 0);
-            before += second ? end - u1 : end - u1 - u0;
+            const Keys &x = second ? mine[1] : mine[0];
+            k.begin = __builtin_amdgcn_readlane(x.begin, l);
+            k.end = __builtin_amdgcn_readlane(x.end, l);
+            k.tile0 = __builtin_amdgcn_readlane(x.tile0, l);
+            k.tiles = __builtin_amdgcn_readlane(x.tiles, l);
+            k.units = (uint32_t)__builtin_amdgcn_readlane((int)x.units, l);
+            before += second ? end - u1 : end - u1 - k.units;
             break;
         }
         before += all;
     }
-    Keys k = keys_of(g, t);  // (from the L1: the scan has read them)
     const uint64_t inside = cur - before * items;
-    int item = (int)(inside / k.units);
+    int item = (int)div64(inside, k.units);
     uint32_t unit = (uint32_t)(inside - (uint64_t)item * k.units);
 
     const int64_t k_slot = g.c.k_strides[1], v_slot = g.c.v_strides[1];
@@ -187,7 +220,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     while (cur < stop) {
         const uint64_t left = stop - cur;
         const uint32_t n = k.units - unit < left ? k.units - unit : (uint32_t)left;
-        const int ht = item * g.nh + hw, kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;  // first query head of the tile
+        const int ht = item * g.nh + hw, kvh = g.gtiles == 1 ? ht : ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;  // first query head of the tile
         const int cols = g.group - gt0 < 16 ? g.group - gt0 : 16;
         const int64_t q_head = (int64_t)kvh * g.group + gt0;
 
@@ -420,7 +453,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         const int chunks = D / 8;  // eight elements of one query head a thread
         for (int x = threadIdx.x; x < g.nh * g.gt * chunks; x += 256) {
             const int hx = x / chunks, d = (x - hx * chunks) * 8, hh = hx / g.gt, h = hx - hh * g.gt;
-            const int tile_x = item * g.nh + hh, kv = tile_x / g.gtiles, head0 = (tile_x - kv * g.gtiles) * 16;
+            const int tile_x = item * g.nh + hh, kv = g.gtiles == 1 ? tile_x : tile_x / g.gtiles, head0 = (tile_x - kv * g.gtiles) * 16;
             if (head0 + h >= g.group) continue;
             float top = -__builtin_inff(), sum = 0.f;
             float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -452,13 +485,83 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             } else {
                 const int64_t piece = (int64_t)slot * g.nh + hh;
                 float *dst = g.part + (piece * g.gt + h) * D + d;
-                *reinterpret_cast<f32x4 *>(dst) = f32x4{r[0], r[1], r[2], r[3]};
-                *reinterpret_cast<f32x4 *>(dst + 4) = f32x4{r[4], r[5], r[6], r[7]};
-                if (d == 0) g.stat[piece * 16 + h] = float2{top, sum};
+                if (g.arrived) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) store_shared(dst + i, r[i], r[i + 1]);
+                    if (d == 0) store_shared(&g.stat[piece * 16 + h].x, top, sum);
+                } else {
+                    *reinterpret_cast<f32x4 *>(dst) = f32x4{r[0], r[1], r[2], r[3]};
+                    *reinterpret_cast<f32x4 *>(dst + 4) = f32x4{r[4], r[5], r[6], r[7]};
+                    if (d == 0) g.stat[piece * 16 + h] = float2{top, sum};
+                }
             }
         }
-        if (!whole && unit == 0 && threadIdx.x == 0)
-            g.split[blockIdx.x] = int4{(int)t, item, slot, (int)((cur + k.units - 1) / per)};
+        if (!whole) {
+            const uint64_t u0 = cur - unit;
+            const int from = (int)div64(u0, per), to = (int)div64(u0 + k.units - 1, per);  // the item's workgroups
+            const int slot0 = from * 2 + (u0 == from * per ? 0 : 1);
+            if (!g.arrived) {
+                if (unit == 0 && threadIdx.x == 0) g.split[blockIdx.x] = int4{(int)t, item, slot0, to};
+            } else {
+                // The last of the item's workgroups to arrive joins its
+                // pieces.  No fence: the pieces are written through to memory
+                // (store_shared), every wave waits for its own to be there,
+                // the barrier collects the waves, then one lane counts the
+                // workgroup in; the last one reads past its L2.  No workgroup
+                // waits for another, and the count is left at zero.
+                __shared__ int last_one;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    const uint32_t there = __hip_atomic_fetch_add(g.arrived + from, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    last_one = there == (uint32_t)(to - from);
+                    if (last_one) __hip_atomic_store(g.arrived + from, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (last_one) {
+                    const int quads = D / 4;
+                    for (int x = threadIdx.x; x < g.nh * g.gt * quads; x += 256) {
+                        const int hx = x / quads, e4 = (x - hx * quads) * 4, hh = hx / g.gt, h = hx - hh * g.gt;
+                        const int ht = item * g.nh + hh, kv = g.gtiles == 1 ? ht : ht / g.gtiles, head0 = (ht - kv * g.gtiles) * 16;
+                        if (head0 + h >= g.group) continue;
+                        float top = -__builtin_inff(), sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+                        for (int i0 = from; i0 <= to; i0 += 4) {
+                            float2 st[4], v[4][2];
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                const int i = i0 + u < to ? i0 + u : to;
+                                const int64_t piece = (int64_t)(i == from ? slot0 : 2 * i) * g.nh + hh;
+                                const float *src = g.part + (piece * g.gt + h) * D + e4;
+                                st[u] = load_shared(&g.stat[piece * 16 + h].x);
+                                v[u][0] = load_shared(src);
+                                v[u][1] = load_shared(src + 2);
+                            }
+                            float most = top;
+#pragma unroll
+                            for (int u = 0; u < 4; u++) most = fmaxf(most, st[u].x);  // (the last one again where there are fewer)
+                            const float base = most == -__builtin_inff() ? 0.f : most, keep = __builtin_amdgcn_exp2f(top - base);
+                            sum *= keep;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) r[e] *= keep;
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                if (i0 + u > to) continue;
+                                const float w = __builtin_amdgcn_exp2f(st[u].x - base);
+                                sum += w * st[u].y;
+                                r[0] += w * v[u][0].x;
+                                r[1] += w * v[u][0].y;
+                                r[2] += w * v[u][1].x;
+                                r[3] += w * v[u][1].y;
+                            }
+                            top = most;
+                        }
+                        uint16_t *out = (uint16_t *)g.a.out + t * g.a.out_strides[0] + ((int64_t)kv * g.group + head0 + h) * g.a.out_strides[1] + e4;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / sum);
+                    }
+                }
+            }
+        }
         __syncthreads();
         cur += n;
         unit = 0;
@@ -470,64 +573,22 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     }
 }
 
-// Joins the pieces of the split item that starts in workgroup blockIdx.x.  Up
-// to kFewPieces: a thread takes four elements of all pieces.  More (few
-// tokens, long): a workgroup a query head, a thread four elements of every
-// 256 / (head_dim / 4)-th piece, eight in flight.
-constexpr int kFewPieces = 16;
+// Joins the pieces of the split item that starts in workgroup blockIdx.x,
+// where they are many (few tokens, long ones): a workgroup a query head, a
+// thread four elements of every 256 / (head_dim / 4)-th piece, eight in
+// flight.
 template <bool BF>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
     const int4 s = g.split[blockIdx.x];
     if (s.x < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = g.c.head_dim, quads = D / 4, at_once = 256 / quads;
     const int n = s.w - (int)blockIdx.x + 1, p0 = tid / quads, q = tid - p0 * quads;
-    if (n <= kFewPieces) {
-        for (int x = blockIdx.y * 256 + tid; x < g.nh * g.gt * quads; x += gridDim.y * 256) {
-            const int hx = x / quads, e4 = (x - hx * quads) * 4, hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
-            const int kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;
-            if (gt0 + h >= g.group) continue;
-            auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)blockIdx.x + i) * 2) * g.nh + hh; };
-            f32x4 r = {0.f, 0.f, 0.f, 0.f};
-            float top = -__builtin_inff(), sum = 0.f;
-            for (int i0 = 0; i0 < n; i0 += 4) {
-                f32x4 v[4];
-                float2 st[4];
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int64_t p = piece(i0 + u < n ? i0 + u : n - 1);
-                    st[u] = g.stat[p * 16 + h];
-                    v[u] = *reinterpret_cast<const f32x4 *>(g.part + (p * g.gt + h) * D + e4);
-                }
-                float most = top;
-#pragma unroll
-                for (int u = 0; u < 4; u++) most = fmaxf(most, st[u].x);  // (the last one again where there are fewer)
-                const float base = most == -__builtin_inff() ? 0.f : most, keep = __builtin_amdgcn_exp2f(top - base);
-                sum *= keep;
-#pragma unroll
-                for (int e = 0; e < 4; e++) r[e] *= keep;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    if (i0 + u >= n) continue;
-                    const float w = __builtin_amdgcn_exp2f(st[u].x - base);
-                    sum += w * st[u].y;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) r[e] += w * v[u][e];
-                }
-                top = most;
-            }
-            const int64_t head = (int64_t)kvh * g.group + gt0 + h;
-            uint16_t *out = (uint16_t *)g.a.out + s.x * g.a.out_strides[0] + head * g.a.out_strides[1] + e4;
-#pragma unroll
-            for (int e = 0; e < 4; e++) out[e] = store16<BF>(top == -__builtin_inff() ? 0.f : r[e] / sum);
-        }
-        return;
-    }
     __shared__ f32x4 acc[256];
     __shared__ float weight[256], red[8];
-    for (int hx = blockIdx.y; hx < g.nh * g.gt; hx += gridDim.y) {
-        const int hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
+    {
+        const int hx = blockIdx.y, hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
         const int kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;
-        if (gt0 + h >= g.group) continue;
+        if (gt0 + h >= g.group) return;
         auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)blockIdx.x + i) * 2) * g.nh + hh; };
         float top = -__builtin_inff();
         for (int i = tid; i < n; i += 256) top = fmaxf(top, g.stat[piece(i) * 16 + h].x);
@@ -559,9 +620,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
                     }
 #pragma unroll
                     for (int u = 0; u < 8; u++) {
-                        const float w = i + u * at_once < m ? weight[i + u * at_once] : 0.f;
+                        const bool in = i + u * at_once < m;
+                        const float w = in ? weight[i + u * at_once] : 0.f;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) r[e] += i + u * at_once < m ? w * v[u][e] : 0.f;
+                        for (int e = 0; e < 4; e++) r[e] += in ? w * v[u][e] : 0.f;
                     }
                 }
         }
@@ -583,6 +645,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
         __syncthreads();
     }
 }
+
+// Pieces of an item up to which the workgroup that writes its last one joins
+// them.
+constexpr int64_t kFewPieces = 16;
 
 // The resident workgroups, and no more than there can be units.
 int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, const AttendArgs &g) {
@@ -641,15 +707,19 @@ hipError_t attend_by_width(const AttendArgs &g, int64_t groups, hipStream_t stre
                  : D <= 128 ? attend_launch<4, BF>(g, groups, lds, stream)
                             : attend_launch<8, BF>(g, groups, lds, stream);
     if (e != hipSuccess) return e;
-    // many items have few pieces each: the workgroups that 256 threads a
-    // four elements make; few items have many: one a head
-    const int64_t items = g.a.tokens * (g.c.kv_heads * (int64_t)g.gtiles / g.nh), heads = g.nh * g.gt;
-    const int64_t y = items * kFewPieces >= groups ? (heads * (D / 4) + 255) / 256 : heads;
-    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)y), 256, 0, stream>>>(g);
+    if (g.arrived) return hipSuccess;
+    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)(g.nh * g.gt)), 256, 0, stream>>>(g);
     return hipGetLastError();
 }
 
 }  // namespace
+
+// Pieces joined by the workgroup that writes the last one need `groups`
+// zeroed counters; a second launch is as fast where an item has many of them.
+bool attention_counts(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups) {
+    const AttendArgs g = attend_args(c, a, cus, groups);
+    return a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh) * kFewPieces >= *groups;
+}
 
 int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus) {
     int64_t groups = 0;
@@ -657,13 +727,14 @@ int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_atte
     return groups * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2)) + (int64_t)sizeof(int4));
 }
 
-hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work,
+hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work, uint32_t *counters,
                                   hipStream_t stream) {
     int64_t groups = 0;
     AttendArgs g = attend_args(c, a, cus, &groups);
     g.split = static_cast<int4 *>(work);
     g.stat = reinterpret_cast<float2 *>(g.split + groups);
     g.part = reinterpret_cast<float *>(g.stat + groups * 2 * g.nh * 16);
+    g.arrived = counters;
     return c.dtype == ORTH_DT_BF16 ? attend_by_width<true>(g, groups, stream) : attend_by_width<false>(g, groups, stream);
 }
 

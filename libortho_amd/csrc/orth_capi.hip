@@ -202,6 +202,11 @@ int resolve(const orth_hip_layer_t *L, const void *input, void *output, int64_t 
 // is used.
 static __device__ __align__(256) unsigned char scratch[ORTH_NOALLOC_SCRATCH_BYTES];
 
+// Counters of captured calls (host_counters), zero from the start; by their
+// device address, as above.
+constexpr int64_t kCounters = 4096;
+static __device__ uint32_t counters[kCounters];
+
 // Per-device check that the current device is a gfx950 (the only code object
 // this library carries), one-time kernel attribute set-up, and the device
 // address of the scratch array.
@@ -210,6 +215,7 @@ struct DeviceState {
     int cus = 256;
     char arch[64] = {0};
     void *scratch = nullptr;      // device address of this device's scratch array
+    void *counters = nullptr;     // the same of its counters
     // the last no-allocation call's completion on this device (recorded on
     // its stream), so that a call on another stream waits for it before it
     // touches the scratch array
@@ -245,6 +251,9 @@ int current_device_ok(int *dev_out) {
                 e = hipGetSymbolAddress(&ptr, HIP_SYMBOL(scratch));
                 if (e != hipSuccess) return fail_hip(e, "hipGetSymbolAddress (scratch)");
                 st.scratch = ptr;
+                e = hipGetSymbolAddress(&ptr, HIP_SYMBOL(counters));
+                if (e != hipSuccess) return fail_hip(e, "hipGetSymbolAddress (counters)");
+                st.counters = ptr;
                 e = hipEventCreateWithFlags(&st.noalloc_done, hipEventDisableTiming);
                 if (e != hipSuccess) return fail_hip(e, "hipEventCreateWithFlags (no-allocation ordering)");
             }
@@ -276,6 +285,7 @@ struct Workspace {
     int64_t part_bytes = 0;
     void *cap = nullptr;  // capture buffer
     int64_t cap_bytes = 0;
+    uint32_t *counters = nullptr;  // kCounters, zero between calls
 };
 std::mutex g_ws_mu;
 std::map<std::pair<int, void *>, Workspace> g_ws;
@@ -707,6 +717,32 @@ int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p) {
     int rc = workspace_for(dev, stream, bytes, &f);
     *p = f;
     return rc;
+}
+int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p) {
+    *p = nullptr;
+    if (count > kCounters) return ORTH_OK;
+    bool cap = false;
+    int rc = capturing(stream, &cap);
+    if (rc != ORTH_OK) return rc;
+    if (cap) {
+        *p = static_cast<uint32_t *>(g_dev[dev].counters);
+        return ORTH_OK;
+    }
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    Workspace &w = g_ws[{dev, static_cast<void *>(stream)}];
+    if (!w.counters) {
+        void *mem = nullptr;
+        hipError_t e = hipMalloc(&mem, kCounters * sizeof(uint32_t));
+        if (e != hipSuccess) return fail_hip(e, "hipMalloc (counters)");
+        e = hipMemsetAsync(mem, 0, kCounters * sizeof(uint32_t), stream);  // (in front of all that counts there)
+        if (e != hipSuccess) {
+            (void)hipFree(mem);
+            return fail_hip(e, "hipMemsetAsync (counters)");
+        }
+        w.counters = static_cast<uint32_t *>(mem);
+    }
+    *p = w.counters;
+    return ORTH_OK;
 }
 }  // namespace orth
 
