@@ -155,12 +155,6 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     constexpr int VW = EL / 2;                          // words of them
     constexpr bool VTAIL = TAIL || 16 * EL != 32 * KS;
     constexpr float kShift = BF ? 0.f : 14.f;
-    // the arguments' lines into the scalar cache at once: read where they are
-    // first used, each would be waited for in turn
-    typedef const __attribute__((address_space(4))) uint32_t *Words;
-    const Words words = (Words)__builtin_amdgcn_kernarg_segment_ptr();
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(AttendArgs); i += 64) asm volatile("" ::"s"(words[i / 4]));
     extern __shared__ float lds[];  // o [waves][gt][16 EL + 4], then (m, l) [waves][16]
     const int D = g.c.head_dim, row_floats = 16 * EL + 4;
     float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
