@@ -33,6 +33,7 @@ constexpr int kTokens = 64;    // tokens of a tile, where they are many
 constexpr int kFew = 512;      // up to here, tiles of 16: decode batches, whose adapters differ by token
 constexpr int kUp = 64;        // outputs a wave takes at a time
 constexpr int kShared = 4;     // adapters of a 64-token tile up to which each has a pass of its own
+constexpr int kUpWaves = 8;    // waves of an up workgroup of 64 tokens
 constexpr int kDown = 8;       // waves of a down workgroup: steps in flight without more partials to add
 
 struct AdapterArgs {
@@ -530,15 +531,16 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
     return sh;
 }
 
-// CB 1: 16 tokens a workgroup and one unit of kUp outputs; the waves split
-// the slices to add, and then the adapters.  CB 4: 64 tokens; each wave adds
-// 16 of them up and then takes a unit of its own for all.  Product t's row
+// CB 1: 16 tokens a workgroup of four waves and one unit of kUp outputs; the
+// waves split the slices to add, and then the adapters.  CB 4: 64 tokens and
+// eight waves; two of them add 16 tokens up, and then each takes a unit of
+// its own for all (eight: the sums are read half as often).  Product t's row
 // 4 a + i is output 16 a + 4 t + i of the unit, so a lane (rows 4 lg + i of
 // all four) holds outputs 16 lg .. 16 lg + 15 of its token.  The loads of y
 // and of the first adapters' B go ahead of the low-rank sums.  KB: steps of
 // 32 ranks whose loads are in flight together.
 template <int CB, bool BF, int W, bool YV, int KB>
-__global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
+__global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(AdapterArgs g) {
     constexpr int IDS = CB == 1 ? 4 / KB : 1;  // adapters whose loads are in flight together
     extern __shared__ u32x4 parts[];           // [4][kks][2][64]
     __shared__ int shifts[kTokens];
@@ -580,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
             if (k % 4 == wave) held |= same;
         }
     }
-    const int64_t n0 = CB == 1 ? (int64_t)block * kUp : ((int64_t)block * 4 + wave) * kUp, n = n0 + 16 * lg;
+    const int64_t n0 = CB == 1 ? (int64_t)block * kUp : ((int64_t)block * kUpWaves + wave) * kUp, n = n0 + 16 * lg;
     if (n0 >= N) held = 0;
 
     u32x4 yv[CB][2];
@@ -631,34 +633,34 @@ __global__ __launch_bounds__(256, 2) void adapter_up_kernel(AdapterArgs g) {
     load_b(0);
 
     // the low-rank values
-    const int tl = CB == 1 ? mine : __shfl(mine, 16 * wave + col, 64);
+    const int group = wave & 3, tl = CB == 1 ? mine : __shfl(mine, 16 * group + col, 64);
     const float scale = tl >= 0 ? (g.a.scales ? g.a.scales[tl] : 1.f) : 0.f;
-    if (__any(tl >= 0)) {
-        for (int kk = 0; kk < kks; kk++) {
+    const bool any = __any(tl >= 0);
+    if (any)
+        for (int kk = CB == 1 ? 0 : wave >> 2; kk < kks; kk += CB == 1 ? 1 : 2) {
             f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            if (tl >= 0) low_sum<CB == 1 ? 2 : 4>(g, token(wave), 32 * kk + 8 * lg, CB == 1 ? wave : 0, CB == 1 ? 4 : 1, v);
+            if (tl >= 0) low_sum<CB == 1 ? 2 : 4>(g, token(group), 32 * kk + 8 * lg, CB == 1 ? wave : 0, CB == 1 ? 4 : 1, v);
             if (CB > 1) {
                 v[0] *= scale;
                 v[1] *= scale;
             }
-            parts[wave * each + (2 * kk) * 64 + lane] = __builtin_bit_cast(u32x4, v[0]);
-            parts[wave * each + (2 * kk + 1) * 64 + lane] = __builtin_bit_cast(u32x4, v[1]);
+            parts[group * each + (2 * kk) * 64 + lane] = __builtin_bit_cast(u32x4, v[0]);
+            parts[group * each + (2 * kk + 1) * 64 + lane] = __builtin_bit_cast(u32x4, v[1]);
         }
-        if constexpr (CB == 1) {
-            __syncthreads();
-            // (x, the rank words, dealt over the waves)
-            for (int x = wave; x < 2 * kks; x += 4) {
-                f32x4 v = __builtin_bit_cast(f32x4, parts[x * 64 + lane]);
+    __syncthreads();
+    if constexpr (CB == 1) {
+        // (x, the rank words, dealt over the waves)
+        for (int x = wave; any && x < 2 * kks; x += 4) {
+            f32x4 v = __builtin_bit_cast(f32x4, parts[x * 64 + lane]);
 #pragma unroll
-                for (int w = 1; w < 4; w++) v += __builtin_bit_cast(f32x4, parts[w * each + x * 64 + lane]);
-                parts[x * 64 + lane] = __builtin_bit_cast(u32x4, v * scale);
-            }
-            __syncthreads();
+            for (int w = 1; w < 4; w++) v += __builtin_bit_cast(f32x4, parts[w * each + x * 64 + lane]);
+            parts[x * 64 + lane] = __builtin_bit_cast(u32x4, v * scale);
         }
-        if (CB > 1 || wave == 0) {
-            const int sh = low_parts<BF>(kks, parts + (CB == 1 ? 0 : wave * each));
-            if (lane < 16) shifts[(CB == 1 ? 0 : 16 * wave) + lane] = sh;
-        }
+        __syncthreads();
+    }
+    if (any && wave < CB) {
+        const int sh = low_parts<BF>(kks, parts + wave * each);
+        if (lane < 16) shifts[16 * wave + lane] = sh;
     }
     __syncthreads();
     if (!held) return;
@@ -753,7 +755,7 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     g.steps = (int)((steps + slices - 1) / slices);
     if (!few) g.steps += g.steps & 1;  // whole 128-byte lines
     g.slices = (int)((steps + g.steps - 1) / g.steps);
-    const int64_t span = few ? kUp : 4 * kUp;
+    const int64_t span = few ? kUp : kUpWaves * kUp;
     g.blocks = (int)((a.out_features + span - 1) / span);
     g.chunk = g.tiles >= 8 ? (g.tiles + 7) / 8 : 0;
     return g;
@@ -788,7 +790,7 @@ hipError_t up_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) 
     const size_t lds = (size_t)4 * ((g.a.rank + 31) / 32) * 128 * sizeof(u32x4);
     const bool yv = g.a.out_features % 8 == 0 && multiple(g.a.y, g.a.y_stride, 8) && multiple(g.a.out, g.a.out_stride, 8);
     const bool one = g.a.rank <= 32;  // one step of ranks: more adapters' loads at a time
-    auto go = [&](auto kernel) { return launch_lds(kernel, groups, 256, lds, stream, g); };
+    auto go = [&](auto kernel) { return launch_lds(kernel, groups, CB == 1 ? 256 : 64 * kUpWaves, lds, stream, g); };
     if (multiple(g.a.b, g.a.rank, 8)) {
         if (yv) return one ? go(adapter_up_kernel<CB, BF, 8, true, 1>) : go(adapter_up_kernel<CB, BF, 8, true, 2>);
         return one ? go(adapter_up_kernel<CB, BF, 8, false, 1>) : go(adapter_up_kernel<CB, BF, 8, false, 2>);
