@@ -26,7 +26,7 @@
 //
 // Bound by reading the cache once.  The work is cut evenly over the resident
 // workgroups by the keys the tokens really see, which only the device knows:
-// every wave sums up the tokens' 128-key units and finds its workgroup's
+// every wave sums up the tokens' units of 256 keys and finds its workgroup's
 // share (of some 100 tokens in one load and one scan).  A share that ends
 // inside a (token, key head) leaves a piece (m, l, o); the workgroup that
 // writes an item's last piece joins them, or a second launch where they are
@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                // keys a wave takes at a time
+constexpr int kPair = 2;                 // tiles a wave takes in a unit, the least share of a workgroup
 constexpr float kLeast = -3.0e38f;       // the maximum of a token that has seen keys, at the least
 
 struct AttendArgs {
@@ -49,7 +50,6 @@ struct AttendArgs {
     int group, gtiles;   // query heads of a key head, and their tiles of 16
     int gt;              // query heads of a tile: min(group, 16)
     int nh, nsub;        // head tiles a workgroup takes at once, and the waves of each: nh * nsub = 4
-    uint32_t min_units;  // the least share of a workgroup
     float *part;         // pieces [workgroups * 2][nh][gt][head_dim]
     float2 *stat;        // (m, l) [workgroups * 2][nh][16]
     int4 *split;         // [workgroups]: (token, item, slot, last workgroup) of the split item that starts there
@@ -91,7 +91,8 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     k.end = (int)(end > INT32_MAX ? INT32_MAX : end);
     k.tile0 = k.begin / kTile;
     k.tiles = (int)(((int64_t)k.end + kTile - 1) / kTile) - k.tile0;
-    k.units = k.tiles > g.nsub ? (uint32_t)(k.tiles + g.nsub - 1) / g.nsub : 1;  // (one that sees nothing is written too)
+    const int unit = kPair * g.nsub;
+    k.units = k.tiles > unit ? (uint32_t)(k.tiles + unit - 1) / unit : 1;  // (one that sees nothing is written too)
     return k;
 }
 
@@ -173,7 +174,6 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     }
     const uint64_t total = run * items;
     uint64_t per = div64(total + gridDim.x - 1, gridDim.x);
-    per = per < g.min_units ? g.min_units : per;
     uint64_t cur = blockIdx.x * per;
     const uint64_t first = cur, stop = cur + per < total ? cur + per : total;
     if (threadIdx.x == 0 && !g.arrived) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
         const uint16_t *kbase = (const uint16_t *)g.c.k_cache + kvh * g.c.k_strides[2];
         const uint16_t *vbase = (const uint16_t *)g.c.v_cache + kvh * g.c.v_strides[2];
         const int last = k.end - 1;
-        const uint64_t upto = (uint64_t)(unit + n) * g.nsub;
+        const uint64_t upto = (uint64_t)(unit + n) * (kPair * g.nsub);
         const int step = g.nsub, tile_end = k.tile0 + (int)(upto < (uint64_t)k.tiles ? upto : (uint64_t)k.tiles);
-        int tile = k.tile0 + (int)unit * g.nsub + sub;
+        int tile = k.tile0 + (int)unit * (kPair * g.nsub) + sub;
 
         f32x4 o[EL];
         float m = -__builtin_inff(), l = 0.f;
@@ -649,7 +649,7 @@ int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int
     const int64_t groups = (int64_t)cus * (c.head_dim > 128 ? 1 : c.head_dim > 64 ? 2 : 3);
     const int64_t held = a.table_width > INT32_MAX / c.page_size ? INT32_MAX : a.table_width * c.page_size;
     const int64_t keys = a.window > 0 && (int64_t)a.window + kTile < held ? (int64_t)a.window + kTile : held;
-    const int64_t units = keys / (kTile * g.nsub) + 1, items = a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh);
+    const int64_t units = keys / (kPair * kTile * g.nsub) + 1, items = a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh);
     return items > groups / units ? groups : items * units;
 }
 
@@ -671,7 +671,6 @@ AttendArgs attend_args(const orth_hip_cache_t &c, const orth_hip_attend_t &a, in
     const bool few_keys = a.table_width <= ((int64_t)1 << 28) / c.page_size;  // (block_units)
     while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && a.tokens * (tiles / (2 * g.nh)) >= cus / 4) g.nh *= 2;
     g.nsub = kWaves / g.nh;
-    g.min_units = 2;
     *groups = attend_groups(c, a, cus, g);
     return g;
 }
