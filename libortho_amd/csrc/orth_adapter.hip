@@ -44,7 +44,9 @@ struct AdapterArgs {
     int blocks;        // up: blocks of out_features
     int slots;         // down: workgroups that share the adapters of a tile
     int chunk;         // tiles of an XCD (0: too few to keep together)
-    int sorted;        // 16-token tiles take tokens by adapter (few_token)
+    int order_by;      // of 16-token tiles: an Order
+    int few;           // 16-token tiles
+    int *order;        // [tokens], by the down launch for the up launch (ORDER_GROUP)
 };
 
 // Workgroup -> (tile, part of it).  Neighbours in blockIdx go to different
@@ -69,34 +71,65 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs &g, int64_t m) {
     return i >= 0 && i < g.a.count ? i : -1;
 }
 
-// The token of column lane & 15 of a 16-token tile, where tokens are few, and
-// its adapter (-1: none, or no token).  Where the stack has fewer adapters
-// than there are tokens, the four tiles of a window of 64 take its tokens in
-// the order of their adapters, so that the tokens of one adapter fall into
-// one tile, or two, and it is read so often.  False: the column has no token
-// (`m` then is some token's).
-__device__ __forceinline__ bool few_token(const AdapterArgs &g, int tile, int *m, int *mine) {
-    const int lane = threadIdx.x & 63, col = lane & 15, tokens = (int)g.a.tokens;
-    if (!g.sorted) {
-        const int at = tile * 16 + col;
-        *m = at < tokens ? at : tokens - 1;
-        *mine = adapter_of(g, at);
-        return at < tokens;
+// The tokens of 16-token tiles.  Where the stack has fewer adapters than
+// there are tokens, the tiles take the tokens in the order of their adapters
+// (those without one last, a stable order), so that the tokens of one adapter
+// fall into few tiles and it is read so often: up to 64 tokens each wave
+// orders them, more the down launch's workgroups, which leave the order for
+// the up launch.
+enum Order { ORDER_NONE = 0, ORDER_WAVE = 1, ORDER_GROUP = 2 };
+constexpr int kOrdered = 512;  // tokens up to which they are ordered
+
+// The token of column lane & 15 of a tile, and its adapter (-1: none, or no
+// token); `order`: the tokens in their order (ORDER_GROUP).  False: the column
+// has no token (`m` then is some token's).
+__device__ __forceinline__ bool few_token(const AdapterArgs &g, int tile, const int *order, int *m, int *mine) {
+    const int lane = threadIdx.x & 63, tokens = (int)g.a.tokens, at = tile * 16 + (lane & 15);
+    const bool present = at < tokens;
+    if (g.order_by != ORDER_WAVE) {
+        *m = present ? (g.order_by == ORDER_GROUP ? order[at] : at) : tokens - 1;
+        *mine = present ? adapter_of(g, *m) : -1;
+        return present;
     }
-    const int base = (tile >> 2) * 64, n = tokens - base < 64 ? tokens - base : 64;
-    const int id = adapter_of(g, base + lane);
-    // adapter, then token: tokens without an adapter after all others, places
-    // without a token last (`sorted` says that the numbers fit)
-    const uint32_t key = lane < n ? (uint32_t)(id >= 0 ? id : 1 << 25) * 64 + lane : 0xffffffc0u + lane;
-    int at = 0;
+    // adapter, then token (adapter_args has seen that the numbers fit)
+    const int id = adapter_of(g, lane);
+    const uint32_t key = lane < tokens ? (uint32_t)(id >= 0 ? id : 1 << 25) * 64 + lane : 0xffffffc0u + lane;
+    int rank = 0;
 #pragma unroll
-    for (int j = 0; j < 64; j++) at += (uint32_t)__builtin_amdgcn_readlane((int)key, j) < key;
-    const int order = __builtin_amdgcn_ds_permute(at * 4, lane);  // lane p: the p-th token of the window
-    const int p = (tile & 3) * 16 + col, t = __shfl(order, p, 64);
-    const int of = __shfl(id, t, 64);
-    *m = p < n ? base + t : tokens - 1;
-    *mine = p < n ? of : -1;
-    return p < n;
+    for (int j = 0; j < 64; j++) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, j) < key;
+    const int by = __builtin_amdgcn_ds_permute(rank * 4, lane);  // lane p: the p-th token
+    const int t = __shfl(by, at & 63, 64), of = __shfl(id, t, 64);
+    *m = present ? t : tokens - 1;
+    *mine = present ? of : -1;
+    return present;
+}
+
+// Orders up to kOrdered tokens: `order` in LDS, room for 2 * kOrdered words.
+__device__ __forceinline__ void order_tokens(const AdapterArgs &g, int *order) {
+    const int n = (int)g.a.tokens, tid = threadIdx.x, threads = blockDim.x;
+    uint32_t *keys = reinterpret_cast<uint32_t *>(order + kOrdered);
+    for (int t = tid; t < kOrdered; t += threads) {
+        const int id = t < n ? adapter_of(g, t) : -1;
+        keys[t] = t < n ? (uint32_t)(id >= 0 ? id : 1 << 22) * kOrdered + t : 0xffffffffu;
+        order[t] = 0;
+    }
+    __syncthreads();
+    // `parts` threads a token, each counting the smaller keys of its part
+    const int parts = threads / ((n + 63) / 64 * 64), wide = threads / parts, part = tid / wide, t = tid - part * wide;
+    const int span = ((n + parts - 1) / parts + 3) / 4 * 4;
+    const uint32_t key = t < n ? keys[t] : 0u;
+    int rank = 0;
+    for (int j = part * span; j < (part + 1) * span && j < kOrdered; j += 4) {
+        const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + j);
+#pragma unroll
+        for (int e = 0; e < 4; e++) rank += k[e] < key;
+    }
+    if (t < n) atomicAdd(order + t, rank);
+    __syncthreads();
+    const int place = tid < n ? order[tid] : 0;
+    __syncthreads();
+    if (tid < n) order[place] = tid;
+    __syncthreads();
 }
 
 // Eight 16-bit elements from p; those from `left` on are zero, and nothing
@@ -397,11 +430,16 @@ __global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs
     if (tile >= g.tiles) return;
     const int64_t m0 = (int64_t)tile * 16 * CB;
     if constexpr (CB == 1) {
-        // the slot's adapter: that of the slot-th column that is its
+        // the slot's adapters: those of every slots-th column that is its
         // adapter's first
-        const int col = threadIdx.x & 15;
+        __shared__ int order[CB == 1 ? 2 * kOrdered : 1];
+        if (g.order_by == ORDER_GROUP) {
+            order_tokens(g, order);
+            if (slice == 0 && slot == 0 && threadIdx.x < 16 && tile * 16 + (int)threadIdx.x < g.a.tokens)
+                g.order[tile * 16 + threadIdx.x] = order[tile * 16 + threadIdx.x];
+        }
         int m, mine;
-        few_token(g, tile, &m, &mine);
+        few_token(g, tile, order, &m, &mine);
         bool first = mine >= 0;
         auto unlike = [&](auto d) {  // the adapter d columns before, within the row of 16 lanes
             const int other = __builtin_amdgcn_update_dpp(-1, mine, 0x110 + decltype(d)::value, 0xf, 0xf, false);
@@ -423,11 +461,12 @@ __global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs
         unlike(std::integral_constant<int, 14>{});
         unlike(std::integral_constant<int, 15>{});
         uint32_t firsts = (uint32_t)__ballot(first) & 0xffffu;
-        for (int i = 0; i < slot; i++) firsts &= firsts - 1;
-        if (!firsts) return;
-        const int id = __builtin_amdgcn_readlane(mine, __ffs(firsts) - 1);
-        const uint32_t own = (uint32_t)__ballot(mine == id) & 0xffffu;
-        for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m, id, own, r, slice, down_lds);
+        for (int i = 0; firsts; i++, firsts &= firsts - 1) {
+            if (i % g.slots != slot) continue;
+            const int id = __builtin_amdgcn_readlane(mine, __ffs(firsts) - 1);
+            const uint32_t own = (uint32_t)__ballot(mine == id) & 0xffffu;
+            for (int r = 0; r < g.a.rank; r += 16 * RB) down_one<RB, BF, W>(g, m, id, own, r, slice, down_lds);
+        }
     } else {
         // up to kShared adapters: the slots take them in turn; more: the
         // first slot takes all at once
@@ -554,7 +593,7 @@ __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(Adap
     int mine, m1 = 0;
     bool present;
     if constexpr (CB == 1) {
-        present = few_token(g, tile, &m1, &mine);
+        present = few_token(g, tile, g.order, &m1, &mine);
     } else {
         mine = adapter_of(g, m0 + lane);
         present = m0 + lane < g.a.tokens;
@@ -737,17 +776,28 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     AdapterArgs g;
     g.a = a;
     g.low = nullptr;
-    const int wide = a.tokens <= kFew ? 16 : kTokens;
-    g.tiles = (int)((a.tokens + wide - 1) / wide);
+    g.order = nullptr;
+    // 16 tokens a tile, also where wider tiles would leave the up launch too
+    // few workgroups (911 tokens, 1000 -> 999: 34 us so, 20 with 16; 1,024
+    // tokens, 4096 -> 4096: 17 and 36)
+    const int64_t wide_tiles = (a.tokens + kTokens - 1) / kTokens, wide_blocks = (a.out_features + kUpWaves * kUp - 1) / (kUpWaves * kUp);
+    g.few = a.tokens <= kFew || wide_tiles * wide_blocks < cus / 4;
+    const bool few = g.few;
+    g.tiles = (int)(few ? (a.tokens + 15) / 16 : wide_tiles);
     const int64_t steps = (a.in_features + 31) / 32;
+    g.order_by = !few || a.tokens <= 16 || a.count >= a.tokens ? ORDER_NONE
+               : a.tokens <= 64 && a.count < (1 << 25) ? ORDER_WAVE
+               : a.tokens <= kOrdered && a.count < (1 << 22) ? ORDER_GROUP : ORDER_NONE;
+    // slots: as many as a 16-token tile can have adapters; in their order, as
+    // a tile has on average and one (the tiles' adapters are then taken in turn)
+    int64_t most = a.tokens < 16 ? a.tokens : 16;
+    if (a.count < most) most = a.count < 1 ? 1 : a.count;
+    const int64_t average = a.count / g.tiles + 1;
+    if (g.order_by != ORDER_NONE && average < most) most = average;
+    g.slots = few ? (int)most : 2;  // (many tokens: a tile mostly has one adapter, or two where a run ends)
     // down: slices for a workgroup of eight waves a CU, of four steps at
     // least; every slice is a partial more that each workgroup of the second
     // launch adds
-    const bool few = a.tokens <= kFew;
-    int64_t most = a.tokens < 16 ? a.tokens : 16;
-    if (a.count < most) most = a.count < 1 ? 1 : a.count;
-    g.sorted = few && a.tokens > 16 && a.count < a.tokens && a.count < (1 << 25);
-    g.slots = few ? (int)most : 2;  // (many tokens: a tile mostly has one adapter, or two where a run ends)
     int64_t slices = (int64_t)cus / (g.tiles * (int64_t)(few ? g.slots : 1));
     if (slices > (steps + 3) / 4) slices = (steps + 3) / 4;
     if (slices > 8) slices = 8;
@@ -777,7 +827,7 @@ hipError_t launch_lds(Kernel kernel, unsigned groups, int threads, size_t lds, h
 
 template <int RB, bool BF>
 hipError_t down_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
-    const bool few = g.a.tokens <= kFew, wide = multiple(g.a.x, g.a.x_stride, 8) && multiple(g.a.a, g.a.in_features, 8);
+    const bool few = g.few, wide = multiple(g.a.x, g.a.x_stride, 8) && multiple(g.a.a, g.a.in_features, 8);
     const size_t join = (size_t)kDown * 16 * RB * 17 * sizeof(float), staged = (size_t)2 * (64 + 16 * RB) * 128;
     const size_t lds = few || join > staged ? join : staged;
     auto go = [&](auto kernel) { return launch_lds(kernel, groups, 64 * kDown, lds, stream, g); };
@@ -813,18 +863,21 @@ hipError_t adapter_launch(const AdapterArgs &g, hipStream_t stream) {
                                       : down_launch<4, BF>(g, down, stream);
         if (e != hipSuccess) return e;
     }
-    return g.a.tokens <= kFew ? up_launch<1, BF>(g, up, stream) : up_launch<4, BF>(g, up, stream);
+    return g.few ? up_launch<1, BF>(g, up, stream) : up_launch<4, BF>(g, up, stream);
 }
 
 }  // namespace
 
 int64_t adapter_workspace_bytes(const orth_hip_adapter_t &a, int cus) {
-    return a.count > 0 ? (int64_t)adapter_args(a, cus).slices * a.tokens * a.rank * 4 : 0;
+    if (a.count == 0) return 0;
+    const AdapterArgs g = adapter_args(a, cus);
+    return (int64_t)g.slices * a.tokens * a.rank * 4 + (g.order_by == ORDER_GROUP ? a.tokens * 4 : 0);
 }
 
 hipError_t launch_adapter_add(const orth_hip_adapter_t &a, int cus, void *work, hipStream_t stream) {
     AdapterArgs g = adapter_args(a, cus);
     g.low = static_cast<float *>(work);
+    g.order = reinterpret_cast<int *>(g.low + (int64_t)g.slices * a.tokens * a.rank);
     return a.dtype == ORTH_DT_BF16 ? adapter_launch<true>(g, stream) : adapter_launch<false>(g, stream);
 }
 

@@ -56,7 +56,8 @@ def check(y, x, a, b, ids, scales=None, out=None):
     (65, 512, 512, 128, 1), (130, 264, 333, 20, 7), (257, 1000, 999, 4, 4), (70, 96, 64, 256, 3), (40, 128, 130, 1, 3),
     (9, 33, 17, 5, 2), (12, 1, 1, 3, 2), (300, 2048, 512, 24, 2), (5, 11008, 4096, 40, 9), (600, 1000, 200, 64, 1),
     (577, 512, 264, 16, 3), (700, 264, 128, 32, 4), (513, 320, 130, 20, 5), (1000, 128, 136, 8, 64), (530, 200, 72, 200, 2),
-    (640, 96, 80, 100, 20), (520, 77, 40, 12, 3), (515, 40, 33, 7, 9)])
+    (640, 96, 80, 100, 20), (520, 77, 40, 12, 3), (515, 40, 33, 7, 9),
+    (400, 128, 96, 16, 120), (512, 64, 72, 8, 511), (65, 64, 64, 8, 30), (48, 160, 64, 32, 24), (900, 64, 50, 8, 30)])
 def test_adapters(gpu, M, K, N, r, n, dtype):
     check(*case(M, K, N, r, n, DT[dtype]))
 
@@ -72,6 +73,19 @@ def test_no_scales_in_place_and_runs(gpu):
     y2 = y.clone()
     got = _C_ops.adapter_add(y2, x, a, b, ids, out=y2)
     assert got.data_ptr() == y2.data_ptr() and torch.equal(y2, want)
+
+
+def test_uneven_use_of_the_stack(gpu):
+    # most tokens on one adapter, the others' tokens on one each: more
+    # adapters in a tile than on average; and one token between others
+    for M, n in ((300, 90), (60, 40), (200, 3)):
+        y, x, a, b, ids, s = case(M, 128, 136, 16, n, torch.float16)
+        ids.fill_(n - 1)
+        ids[:min(n, M // 2)] = torch.arange(min(n, M // 2), device="cuda", dtype=torch.int32)
+        check(y, x, a, b, ids, s)
+        ids.fill_(-1)
+        ids[M // 2] = 1
+        check(y, x, a, b, ids, s)
 
 
 def test_adapters_outside_the_stack_add_nothing(gpu):
