@@ -18,9 +18,18 @@
 // output's own rounding), FP16 ones scaled by a power of two per token, so
 // that none overflows or loses its low bits.
 //
-// Bound by reading the adapters (few tokens: workgroups of 16 tokens, whose
-// waves split in_features, then the adapters) or x, y and out (many: 64
-// tokens a workgroup share each adapter's loads).
+// Bound by reading the adapters (few tokens: workgroups of 16 tokens, a slot
+// for each adapter among them, then waves that split the adapters) or x, y
+// and out (many: 64 tokens a workgroup share each adapter's loads).
+//
+// Measured (one MI355X, a call among others): one token, 4096 -> 4096, rank
+// 16, FP16: 8.9 us, two chains of latencies (number, weights, join; number,
+// partials, store); 48 tokens of 24 adapters, 4096 -> 11008, rank 32, BF16:
+// 16.4 us (23.7 MB, 1.5 TB/s; down 6, up 10.5); 2,048 tokens in five runs,
+// 11008 -> 4096, rank 64, FP16: 37.3 us (86 MB, 2.3 TB/s; down 19, up 19: the
+// partials' round trip and the launches' starts and ends, with one round of
+// workgroups each).  A wave per low-rank value and a thread per output took
+// 12, 57 and 2,500 us.
 #include <type_traits>
 
 #include "orth_serve.h"

@@ -21,7 +21,9 @@ namespace {
 // all requests (8 bytes each from the L2) instead of waiting for one that
 // does it, and then writes a token a thread.  The sums of a scan are 32 bits
 // wide where `tokens` allows it (64-bit ones took 2 us more for 16 requests:
-// a wave's scan is then a dozen LDS permutes instead of six adds).
+// a wave's scan is then a dozen LDS permutes instead of six adds).  Measured:
+// 3.3 us in the kernel for 16 requests of one token, 6.3 for 512 with 64
+// prompts (13,321 places); 5.6 and 5.8 us a call among others.
 constexpr int kStepMost = 1024;  // threads of a workgroup (256 for up to 256 requests)
 
 __device__ __forceinline__ uint32_t scan_in_wave(uint32_t v) { return wave_scan(v); }
@@ -148,7 +150,9 @@ __global__ __launch_bounds__(kStepMost) void page_step_kernel(orth_hip_step_t s,
 // each half, or 2 V neighbours when interleaved), the rest are copied.  A
 // thread keeps one item and steps through the heads, so its cosines and sines
 // (as many bytes as the item's elements read and written) are loaded once for
-// all of a token's heads.
+// all of a token's heads.  Measured: 2,048 tokens of 32 + 8 heads of 128 in
+// 9.7 us, 5.3 TB/s; 4 tokens 3.6 us in the kernel (launch and three dependent
+// reads: slot, position, cosines).
 struct AppendArgs {
     orth_hip_cache_t c;
     orth_hip_append_t a;
