@@ -794,7 +794,7 @@ AdapterArgs adapter_args(const orth_hip_adapter_t &a, int cus) {
     const bool few = g.few;
     g.tiles = (int)(few ? (a.tokens + 15) / 16 : wide_tiles);
     const int64_t steps = (a.in_features + 31) / 32;
-    g.order_by = !few || a.tokens <= 16 || a.count >= a.tokens ? ORDER_NONE
+    g.order_by = !few || a.tokens <= 16 || a.count < 1 || a.count >= a.tokens ? ORDER_NONE
                : a.tokens <= 64 && a.count < (1 << 25) ? ORDER_WAVE
                : a.tokens <= kOrdered && a.count < (1 << 22) ? ORDER_GROUP : ORDER_NONE;
     // slots: as many as a 16-token tile can have adapters; in their order, as
@@ -886,7 +886,7 @@ int64_t adapter_workspace_bytes(const orth_hip_adapter_t &a, int cus) {
 hipError_t launch_adapter_add(const orth_hip_adapter_t &a, int cus, void *work, hipStream_t stream) {
     AdapterArgs g = adapter_args(a, cus);
     g.low = static_cast<float *>(work);
-    g.order = reinterpret_cast<int *>(g.low + (int64_t)g.slices * a.tokens * a.rank);
+    if (g.order_by == ORDER_GROUP) g.order = reinterpret_cast<int *>(g.low + (int64_t)g.slices * a.tokens * a.rank);
     return a.dtype == ORTH_DT_BF16 ? adapter_launch<true>(g, stream) : adapter_launch<false>(g, stream);
 }
 

@@ -93,8 +93,10 @@ def test_adapters_outside_the_stack_add_nothing(gpu):
     for bad in (-1, 3, 2 ** 31 - 1, -2 ** 31):
         ids.fill_(bad)
         assert torch.equal(_C_ops.adapter_add(y, x, a, b, ids, s), y)
-    assert torch.equal(_C_ops.adapter_add(y, x, a[:0], b[:0], ids, s[:0]), y)
-    assert _C_ops.adapter_add(y[:0], x[:0], a, b, ids[:0], s).shape == (0, 256)
+    for M in (20, 100, 300, 600):  # an empty stack
+        y, x, _, _, ids, _ = case(M, 256, 256, 16, 3, torch.bfloat16)
+        assert torch.equal(_C_ops.adapter_add(y, x, a[:0], b[:0], ids, s[:0]), y)
+    assert _C_ops.adapter_add(y[:0], x[:0], a, b, ids[:0], s).shape == (0, 256)  # and no token
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
