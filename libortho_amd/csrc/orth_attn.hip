@@ -29,14 +29,14 @@
 // every wave sums up the tokens' units of 256 keys and finds its workgroup's
 // share (of some 100 tokens in one load and one scan).  A share that ends
 // inside a (token, key head) leaves a piece (m, l, o); the workgroup that
-// writes an item's last piece joins them, or a second launch where they are
-// many.  Whole items are written at once.
+// writes an item's last piece joins them, or a second launch where an item
+// has many.  Whole items are written at once.
 //
 // Measured (one MI355X, a call among others, inputs from HBM): 128 requests
 // of 2,048 to 16,384 keys, 8 of 64 heads of 128, BF16: 590 us, 5.7 TB/s of
-// keys and values; 32 ragged requests up to 4,096 keys, 32 heads, FP16: 72.6
-// us, 4.7 TB/s; one of 32,768 keys, 8 of 32 heads: 39.9 us (32 the keys, 7.5
-// the join of 64 pieces a key head), 3.4 TB/s; one of 190 keys, 32 heads: 9.2 us,
+// keys and values; 32 ragged requests up to 4,096 keys, 32 heads, FP16: 73.6
+// us, 4.6 TB/s; one of 32,768 keys, 8 of 32 heads: 37.1 us (32 the keys, 5
+// the join of 64 pieces a key head), 3.6 TB/s; one of 190 keys, 32 heads: 9.2 us,
 // a chain of latencies (position 1.2, share 0.7, table 1.6, keys 2, join 1).
 // A wave per query head on the vector unit (no matrix products, no split)
 // took 35,500, 7,900, 57,500 and 164 us.
@@ -49,6 +49,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                // keys a wave takes at a time
 constexpr int kPair = 2;                 // tiles a wave takes in a unit, the least share of a workgroup
+constexpr int kPieces = 16;              // pieces of an item (and one for its ends) that a workgroup joins
 constexpr float kLeast = -3.0e38f;       // the maximum of a token that has seen keys, at the least
 
 struct AttendArgs {
@@ -61,8 +62,9 @@ struct AttendArgs {
     int nh, nsub;        // head tiles a workgroup takes at once, and the waves of each: nh * nsub = 4
     float *part;         // pieces [workgroups * 2][nh][gt][head_dim]
     float2 *stat;        // (m, l) [workgroups * 2][nh][16]
-    int4 *split;         // [workgroups]: (token, item, slot, last workgroup) of the split item that starts there
-    uint32_t *arrived;   // [workgroups], zeros: the pieces of that item written so far; null: a second launch joins
+    uint32_t *arrived;   // [workgroups], zeros: the pieces written so far of the split item that starts there
+    int4 *many;          // [workgroups / kPieces, up]: (token, item, first piece's slot, last workgroup) of an item
+                         // of more than kPieces + 1 pieces, or a token of -1: joined by a second launch
 };
 
 struct Keys {
@@ -185,8 +187,11 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     uint64_t per = div64(total + gridDim.x - 1, gridDim.x);
     uint64_t cur = blockIdx.x * per;
     const uint64_t first = cur, stop = cur + per < total ? cur + per : total;
-    if (threadIdx.x == 0 && !g.arrived) g.split[blockIdx.x] = int4{-1, 0, 0, 0};
-    if (cur >= total) return;
+    const bool marks = blockIdx.x % kPieces == 0 && threadIdx.x == 0;
+    if (cur >= total) {
+        if (marks) g.many[blockIdx.x / kPieces] = int4{-1, 0, 0, 0};
+        return;
+    }
     const uint64_t want = div64(cur, items);  // the unit, were a token one item
     int64_t t = 0;
     Keys k;
@@ -215,6 +220,16 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     const uint64_t inside = cur - before * items;
     int item = (int)div64(inside, k.units);
     uint32_t unit = (uint32_t)(inside - (uint64_t)item * k.units);
+
+    if (marks) {
+        // an item of more than kPieces + 1 pieces has a workgroup of these
+        // behind its first one, and only one within kPieces of it, at whose
+        // start no other item lies: it names the item to the second launch
+        const uint64_t u0 = cur - unit;
+        const int from = (int)div64(u0, per), to = (int)div64(u0 + k.units - 1, per);
+        const bool big = to - from > kPieces && from < (int)blockIdx.x && (int)blockIdx.x - from <= kPieces;
+        g.many[blockIdx.x / kPieces] = big ? int4{(int)t, item, from * 2 + (u0 == from * per ? 0 : 1), to} : int4{-1, 0, 0, 0};
+    }
 
     const int64_t k_slot = g.c.k_strides[1], v_slot = g.c.v_strides[1];
     const bool q16 = ((reinterpret_cast<uintptr_t>(g.a.q) | (uintptr_t)(g.a.q_strides[0] * 2) | (uintptr_t)(g.a.q_strides[1] * 2)) & 15) == 0;
@@ -488,24 +503,16 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             } else {
                 const int64_t piece = (int64_t)slot * g.nh + hh;
                 float *dst = g.part + (piece * g.gt + h) * D + d;
-                if (g.arrived) {
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) store_shared(dst + i, r[i], r[i + 1]);
-                    if (d == 0) store_shared(&g.stat[piece * 16 + h].x, top, sum);
-                } else {
-                    *reinterpret_cast<f32x4 *>(dst) = f32x4{r[0], r[1], r[2], r[3]};
-                    *reinterpret_cast<f32x4 *>(dst + 4) = f32x4{r[4], r[5], r[6], r[7]};
-                    if (d == 0) g.stat[piece * 16 + h] = float2{top, sum};
-                }
+                for (int i = 0; i < 8; i += 2) store_shared(dst + i, r[i], r[i + 1]);
+                if (d == 0) store_shared(&g.stat[piece * 16 + h].x, top, sum);
             }
         }
         if (!whole) {
             const uint64_t u0 = cur - unit;
             const int from = (int)div64(u0, per), to = (int)div64(u0 + k.units - 1, per);  // the item's workgroups
             const int slot0 = from * 2 + (u0 == from * per ? 0 : 1);
-            if (!g.arrived) {
-                if (unit == 0 && threadIdx.x == 0) g.split[blockIdx.x] = int4{(int)t, item, slot0, to};
-            } else {
+            if (to - from <= kPieces) {
                 // The last of the item's workgroups to arrive joins its
                 // pieces.  No fence: the pieces are written through to memory
                 // (store_shared), every wave waits for its own to be there,
@@ -576,23 +583,22 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     }
 }
 
-// Joins the pieces of the split item that starts in workgroup blockIdx.x,
-// where they are many (few tokens, long ones): a workgroup a query head, a
-// thread four elements of every 256 / (head_dim / 4)-th piece, eight in
-// flight.
+// Joins the pieces of an item that has many (a long request): a workgroup a
+// query head, a thread four elements of every 256 / (head_dim / 4)-th piece,
+// eight in flight.
 template <bool BF>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
-    const int4 s = g.split[blockIdx.x];
+    const int4 s = g.many[blockIdx.x];
     if (s.x < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = g.c.head_dim, quads = D / 4, at_once = 256 / quads;
-    const int n = s.w - (int)blockIdx.x + 1, p0 = tid / quads, q = tid - p0 * quads;
+    const int from = s.z >> 1, n = s.w - from + 1, p0 = tid / quads, q = tid - p0 * quads;
     __shared__ f32x4 acc[256];
     __shared__ float weight[256], red[8];
     {
         const int hx = blockIdx.y, hh = hx / g.gt, h = hx - hh * g.gt, ht = s.y * g.nh + hh;
         const int kvh = ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;
         if (gt0 + h >= g.group) return;
-        auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)blockIdx.x + i) * 2) * g.nh + hh; };
+        auto piece = [&](int i) -> int64_t { return (i == 0 ? (int64_t)s.z : ((int64_t)from + i) * 2) * g.nh + hh; };
         float top = -__builtin_inff();
         for (int i = tid; i < n; i += 256) top = fmaxf(top, g.stat[piece(i) * 16 + h].x);
 #pragma unroll
@@ -649,18 +655,17 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
     }
 }
 
-// Pieces of an item up to which the workgroup that writes its last one joins
-// them: 40 requests with windows 17.5 -> 16.1 us, one short request 10.6 ->
-// 9.5.  Past it one workgroup would read them all (64 pieces of four heads:
-// 128 KB), where the second launch has one for each head.
-constexpr int64_t kFewPieces = 16;
+// The most units a token can have.
+int64_t attend_units(const AttendArgs &g) {
+    const int64_t held = g.a.table_width > INT32_MAX / g.c.page_size ? INT32_MAX : g.a.table_width * g.c.page_size;
+    const int64_t keys = g.a.window > 0 && (int64_t)g.a.window + kTile < held ? (int64_t)g.a.window + kTile : held;
+    return keys / (kPair * kTile * g.nsub) + 1;
+}
 
 // The resident workgroups, and no more than there can be units.
-int64_t attend_groups(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, const AttendArgs &g) {
-    const int64_t groups = (int64_t)cus * (c.head_dim > 128 ? 1 : c.head_dim > 64 ? 2 : 3);
-    const int64_t held = a.table_width > INT32_MAX / c.page_size ? INT32_MAX : a.table_width * c.page_size;
-    const int64_t keys = a.window > 0 && (int64_t)a.window + kTile < held ? (int64_t)a.window + kTile : held;
-    const int64_t units = keys / (kPair * kTile * g.nsub) + 1, items = a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh);
+int64_t attend_groups(const AttendArgs &g, int cus) {
+    const int64_t groups = (int64_t)cus * (g.c.head_dim > 128 ? 1 : g.c.head_dim > 64 ? 2 : 3);
+    const int64_t units = attend_units(g), items = g.a.tokens * (g.c.kv_heads * (int64_t)g.gtiles / g.nh);
     return items > groups / units ? groups : items * units;
 }
 
@@ -684,7 +689,7 @@ AttendArgs attend_args(const orth_hip_cache_t &c, const orth_hip_attend_t &a, in
     const bool few_keys = a.table_width <= ((int64_t)1 << 28) / c.page_size;  // (block_units)
     while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && a.tokens * (tiles / (2 * g.nh)) >= cus / 4) g.nh *= 2;
     g.nsub = kWaves / g.nh;
-    *groups = attend_groups(c, a, cus, g);
+    *groups = attend_groups(g, cus);
     return g;
 }
 
@@ -713,32 +718,32 @@ hipError_t attend_by_width(const AttendArgs &g, int64_t groups, hipStream_t stre
                  : D <= 128 ? attend_launch<4, BF>(g, groups, lds, stream)
                             : attend_launch<8, BF>(g, groups, lds, stream);
     if (e != hipSuccess) return e;
-    if (g.arrived) return hipSuccess;
-    join_kernel<BF><<<dim3((unsigned)groups, (unsigned)(g.nh * g.gt)), 256, 0, stream>>>(g);
+    // No item has many pieces where none has many units, and of one token's
+    // items, which are all of one length, none where they are many.  Requests
+    // of several lengths may have: one long among short ones.  (40 requests
+    // with windows: 15.3 us without the second launch, 16.8 with it, 17.5
+    // where it joined all.  A workgroup alone would take tens of microseconds
+    // to join the hundreds of pieces of a long request.)
+    const int64_t items = g.a.tokens * (g.c.kv_heads * (int64_t)g.gtiles / g.nh);
+    if (attend_units(g) <= kPieces + 1 || (g.a.tokens == 1 && items * kPieces >= groups)) return hipSuccess;
+    join_kernel<BF><<<dim3((unsigned)((groups + kPieces - 1) / kPieces), (unsigned)(g.nh * g.gt)), 256, 0, stream>>>(g);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Pieces joined by the workgroup that writes the last one need `groups`
-// zeroed counters; a second launch is as fast where an item has many of them.
-bool attention_counts(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups) {
+int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups) {
     const AttendArgs g = attend_args(c, a, cus, groups);
-    return a.tokens * (c.kv_heads * (int64_t)g.gtiles / g.nh) * kFewPieces >= *groups;
-}
-
-int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus) {
-    int64_t groups = 0;
-    const AttendArgs g = attend_args(c, a, cus, &groups);
-    return groups * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2)) + (int64_t)sizeof(int4));
+    return *groups * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2))) +
+           (*groups + kPieces - 1) / kPieces * (int64_t)sizeof(int4);
 }
 
 hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work, uint32_t *counters,
                                   hipStream_t stream) {
     int64_t groups = 0;
     AttendArgs g = attend_args(c, a, cus, &groups);
-    g.split = static_cast<int4 *>(work);
-    g.stat = reinterpret_cast<float2 *>(g.split + groups);
+    g.many = static_cast<int4 *>(work);
+    g.stat = reinterpret_cast<float2 *>(g.many + (groups + kPieces - 1) / kPieces);
     g.part = reinterpret_cast<float *>(g.stat + groups * 2 * g.nh * 16);
     g.arrived = counters;
     return c.dtype == ORTH_DT_BF16 ? attend_by_width<true>(g, groups, stream) : attend_by_width<false>(g, groups, stream);

@@ -720,7 +720,8 @@ int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p) {
 }
 int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p) {
     *p = nullptr;
-    if (count > kCounters) return ORTH_OK;
+    if (count > kCounters)
+        return fail(ORTH_ERR_UNSUPPORTED, "a call needs %lld counters, more than %lld", (long long)count, (long long)kCounters);
     bool cap = false;
     int rc = capturing(stream, &cap);
     if (rc != ORTH_OK) return rc;

@@ -15,7 +15,6 @@ int host_device(int *dev, int *cus);
 int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p);
 // Counters that are zero between calls (each kernel that counts in them leaves
 // zeros): the stream's own, or, under capture, those of all captured calls.
-// Null where there are not as many.
 int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p);
 
 }  // namespace orth

@@ -10,8 +10,8 @@ hipError_t launch_page_step(const orth_hip_step_t &s, hipStream_t stream);
 
 hipError_t launch_cache_append(const orth_hip_cache_t &c, const orth_hip_append_t &a, int cus, hipStream_t stream);
 
-int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus);
-bool attention_counts(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups);
+// (`groups`: the counters that a call takes)
+int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups);
 hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work, uint32_t *counters,
                                   hipStream_t stream);
 

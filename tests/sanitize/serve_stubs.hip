@@ -6,8 +6,10 @@
 namespace orth {
 hipError_t launch_page_step(const orth_hip_step_t &, hipStream_t) { return hipErrorInvalidValue; }
 hipError_t launch_cache_append(const orth_hip_cache_t &, const orth_hip_append_t &, int, hipStream_t) { return hipErrorInvalidValue; }
-int64_t attention_workspace_bytes(const orth_hip_cache_t &, const orth_hip_attend_t &, int) { return 64; }
-bool attention_counts(const orth_hip_cache_t &, const orth_hip_attend_t &, int, int64_t *groups) { *groups = 1; return true; }
+int64_t attention_workspace_bytes(const orth_hip_cache_t &, const orth_hip_attend_t &, int, int64_t *groups) {
+    *groups = 1;
+    return 64;
+}
 hipError_t launch_paged_attention(const orth_hip_cache_t &, const orth_hip_attend_t &, int, void *, uint32_t *, hipStream_t) {
     return hipErrorInvalidValue;
 }

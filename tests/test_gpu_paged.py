@@ -286,7 +286,7 @@ LENS = [0, 1, 2, 31, 32, 33, 64, 127, 129, 300, 513]
 @pytest.mark.parametrize("H,G,D,P", [
     (4, 4, 128, 16), (8, 2, 128, 32), (8, 1, 64, 8), (6, 2, 80, 16), (7, 1, 96, 64), (4, 2, 256, 16), (16, 1, 128, 16),
     (17, 1, 64, 16), (40, 2, 128, 128), (3, 3, 8, 16), (4, 2, 72, 24), (2, 1, 112, 8), (4, 4, 128, 1), (8, 2, 64, 7),
-    (5, 5, 248, 20)])
+    (5, 5, 248, 20), (16, 1, 256, 16), (32, 2, 200, 8)])
 def test_attention_heads_and_pages(gpu, H, G, D, P, dtype):
     attend_check(*attend_case(LENS, H, G, D, P, DT[dtype]))
 
@@ -299,7 +299,8 @@ def test_attention_window(gpu, window, P):
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("lens,H,G,D,P", [
-    ([20000], 8, 2, 128, 64), ([5000, 1, 0, 9001], 4, 4, 64, 16), ([3000] * 3, 32, 4, 80, 16), ([4097], 2, 1, 256, 128)])
+    ([20000], 8, 2, 128, 64), ([5000, 1, 0, 9001], 4, 4, 64, 16),
+    ([1, 7, 30000, 300, 2], 4, 1, 128, 32), ([40] * 70 + [25000] + [3] * 20, 8, 4, 64, 16), ([18000, 20000], 5, 1, 64, 8), ([3000] * 3, 32, 4, 80, 16), ([4097], 2, 1, 256, 128)])
 def test_attention_long(gpu, lens, H, G, D, P, dtype):
     attend_check(*attend_case(lens, H, G, D, P, DT[dtype]))
 
