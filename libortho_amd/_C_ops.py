@@ -746,9 +746,10 @@ def paged_attention(q, k_cache, v_cache, block_table, positions, rows=None, scal
     ``scale`` defaults to head_dim ** -0.5.
 
     A token at position -1 (or whose row lies outside the table) gets zeros;
-    pages outside the cache and keys past the table are not seen.  Several
-    new tokens of one request may be passed at once, each with its own
-    position, once all their keys are in the cache."""
+    pages outside the cache and keys past the table (of 2**31 - 512 keys at
+    the most) are not seen.  Several new tokens of one request may be passed
+    at once, each with its own position, once all their keys are in the
+    cache."""
     T = _lib.torch_ops()
     if T is not None:
         return T.paged_attention(q, k_cache, v_cache, block_table, positions, rows, scale, window, out)

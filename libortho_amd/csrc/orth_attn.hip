@@ -52,6 +52,10 @@ constexpr int kPair = 2;                 // tiles a wave takes in a unit, the le
 constexpr int kPieces = 16;              // pieces of an item (and one for its ends) that a workgroup joins
 constexpr float kLeast = -3.0e38f;       // the maximum of a token that has seen keys, at the least
 
+// Loads run up to two steps of kWaves tiles ahead of the last key: their key
+// numbers stay within an int.
+static_assert(kMostKeys + (2 * kWaves + 1) * kTile <= INT32_MAX, "a table's keys");
+
 struct AttendArgs {
     orth_hip_cache_t c;
     orth_hip_attend_t a;
@@ -99,7 +103,7 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
     if (row < 0 || row >= g.a.table_rows || end <= begin) begin = end = 0;
     Keys k;
     k.begin = (int)begin;
-    k.end = (int)(end > INT32_MAX ? INT32_MAX : end);
+    k.end = (int)end;
     k.tile0 = k.begin / kTile;
     k.tiles = (int)(((int64_t)k.end + kTile - 1) / kTile) - k.tile0;
     const int unit = kPair * g.nsub;
@@ -657,7 +661,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs g) {
 
 // The most units a token can have.
 int64_t attend_units(const AttendArgs &g) {
-    const int64_t held = g.a.table_width > INT32_MAX / g.c.page_size ? INT32_MAX : g.a.table_width * g.c.page_size;
+    const int64_t held = g.a.table_width * g.c.page_size;
     const int64_t keys = g.a.window > 0 && (int64_t)g.a.window + kTile < held ? (int64_t)g.a.window + kTile : held;
     return keys / (kPair * kTile * g.nsub) + 1;
 }

@@ -6,6 +6,10 @@
 
 namespace orth {
 
+// The most keys a block table may hold: the attention's key numbers, and
+// those its loads run ahead to, are 32-bit.
+constexpr int64_t kMostKeys = ((int64_t)1 << 31) - 512;
+
 hipError_t launch_page_step(const orth_hip_step_t &s, hipStream_t stream);
 
 hipError_t launch_cache_append(const orth_hip_cache_t &c, const orth_hip_append_t &a, int cus, hipStream_t stream);

@@ -153,6 +153,8 @@ int orth_paged_attention_hip(const orth_hip_cache_t *c, const orth_hip_attend_t 
             return invalid("table_rows and table_width must not be negative, at most 2^31 - 1");
         if (a->table_stride < a->table_width || (a->table_rows > 0 && a->table_stride > kMaxSpan / a->table_rows))
             return invalid("table_stride is smaller than table_width, or too large");
+        if (a->table_width * c->page_size > kMostKeys)
+            return host_fail(ORTH_ERR_UNSUPPORTED, "table_width * page_size passes 2^31 - 512");
         if (a->tokens > 0) {
             if (!a->q || !a->out || !a->positions) return invalid("q, out or positions is NULL");
             if (a->table_rows > 0 && a->table_width > 0 && !a->block_table) return invalid("block_table is NULL");

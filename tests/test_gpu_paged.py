@@ -401,6 +401,23 @@ def test_attention_past_32_bit_offsets(gpu):
     assert torch.equal(cache[-1, P - 3], k[0])
 
 
+@pytest.mark.parametrize("P", [32, 28])
+def test_attention_last_key_numbers(gpu, P):
+    # windows at the end of the widest table there is (one page in every place)
+    W = ((1 << 31) - 512) // P
+    table = torch.zeros(1, W, dtype=torch.int32, device="cuda")
+    kc, vc = (torch.randn(1, P, 1, 8, device="cuda").half() for _ in range(2))
+    q = torch.randn(1, 2, 8, device="cuda").half()
+    for back, window in ((1, 1), (1, 300), (40, 1000), (0, 70)):
+        last = W * P - back  # (back 0: one key past the table, not seen)
+        got = _C_ops.paged_attention(q, kc, vc, table, i32([last]), window=window)
+        j = np.arange(max(0, last + 1 - window), min(last + 1, W * P)) % P
+        s = (q[0].double() @ kc[0, :, 0].double().T.contiguous())[:, torch.tensor(j).cuda()] * 8 ** -0.5
+        want = torch.softmax(s, -1) @ vc[0, :, 0].double()[torch.tensor(j).cuda()].contiguous()
+        # FP16's rounding of values up to |v| <= 4, and FP32 sums behind it
+        assert float((got[0].double() - want).abs().max()) <= 2 ** -9
+
+
 def test_attention_is_the_same_every_time_and_on_other_streams(gpu):
     q, kc, vc, table, pos = attend_case([9000, 17, 4000], 8, 2, 128, 16, torch.bfloat16)
     want = attend_check(q, kc, vc, table, pos)

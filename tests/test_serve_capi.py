@@ -126,6 +126,18 @@ def test_attention_refusals(L, kw, status, needle):
     refused(L, L.orth_paged_attention_hip(ctypes.byref(cache()), ctypes.byref(attend(**kw)), None), status, needle)
 
 
+def test_attention_refuses_tables_of_more_keys_than_its_numbers_hold(L):
+    def call(width, page):
+        return L.orth_paged_attention_hip(ctypes.byref(cache(page_size=page)),
+                                          ctypes.byref(attend(table_width=width, table_stride=width)), None)
+    refused(L, call(2, 1 << 30), UNSUPPORTED, "2^31 - 512")
+    refused(L, call((1 << 31) - 1, (1 << 31) - 1), UNSUPPORTED, "2^31 - 512")
+    refused(L, call((1 << 26) - 15, 32), UNSUPPORTED, "2^31 - 512")
+    # the most it takes: no complaint about the table (a null query ends the call)
+    a = attend(table_width=(1 << 26) - 16, table_stride=(1 << 26) - 16, q=None)
+    refused(L, L.orth_paged_attention_hip(ctypes.byref(cache(page_size=32)), ctypes.byref(a), None), INVALID, "NULL")
+
+
 @pytest.mark.parametrize("kw,status,needle", [
     ({"dtype": _lib.DT_F32}, UNSUPPORTED, "F16 or BF16"), ({"rank": 0}, UNSUPPORTED, "rank"),
     ({"rank": 257}, UNSUPPORTED, "rank"), ({"in_features": 0}, INVALID, "in_features"), ({"tokens": -1}, INVALID, "tokens"),
