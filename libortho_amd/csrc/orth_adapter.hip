@@ -269,7 +269,10 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int m, int id, ui
 // adapter in turn, the products kept in their own tokens' columns.
 template <int RB, bool BF, int W>
 __device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int rank0, int slice, float *lds) {
-    constexpr int IDS = RB == 1 ? 4 : 2;  // adapters whose loads are in flight together
+    // adapters whose loads are in flight together (with eight, and two in the
+    // up launch, 538 tokens of 24 adapters in turn, 4000 -> 11008, rank 16,
+    // take 82 us; with four and one 91)
+    constexpr int IDS = RB == 1 ? 8 : 2;
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t K = g.a.in_features;
     const int mine = adapter_of(g, m0 + lane);
@@ -589,8 +592,8 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
 // 32 ranks whose loads are in flight together.
 template <int CB, bool BF, int W, bool YV, int KB>
 __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(AdapterArgs g) {
-    constexpr int IDS = CB == 1 ? 4 / KB : 1;  // adapters whose loads are in flight together
-    extern __shared__ u32x4 parts[];           // [4][kks][2][64]
+    constexpr int IDS = (CB == 1 ? 4 : 2) / KB;  // adapters whose loads are in flight together (as many as registers hold)
+    extern __shared__ u32x4 parts[];             // [4][kks][2][64]
     __shared__ int shifts[kTokens];
     int tile, block;
     place_of(g, blockIdx.x, g.blocks, &tile, &block);
