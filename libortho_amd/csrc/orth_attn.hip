@@ -20,9 +20,10 @@
 //           elements (a key's vector lies across 16 lanes) and transposes
 //           them in registers, one v_perm_b32 per two values.
 //
-// The weights enter the second product as two 16-bit parts, so that rounding
-// them costs 2^-16 and not as much as the output's own rounding; FP16 ones
-// are held 2^14 times larger, which keeps small weights normal numbers.
+// The weights enter the second product as FP32 values do: as 16-bit parts,
+// three in BF16 and two in FP16 (split_pair), whose products with the values
+// are exact and add up in FP32.  FP16 ones are held 2^14 times larger, which
+// keeps the parts of small weights normal numbers.
 //
 // Bound by reading the cache once.  The work is cut evenly over the resident
 // workgroups by the keys the tokens really see, which only the device knows:
@@ -146,19 +147,32 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, const f32x
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Two floats as a pair of 16-bit values plus the pair of what they leave.
+// Two weights as pairs of 16-bit parts, part[0] the largest.  BF16: three
+// parts of eight bits each, cut off, whose sum is the FP32 weight exactly.
+// FP16: two parts of eleven bits, rounded to nearest (the second one's sign is
+// a bit more): 2^-24 of the weight, as an FP32 operation's rounding, or 2^-39
+// of the largest weight where that is more.
 template <bool BF>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t *hi, uint32_t *lo) {
+constexpr int kParts = BF ? 3 : 2;
+template <bool BF>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t part[kParts<BF>]) {
     if constexpr (BF) {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        const bf16x2 h = {(__bf16)x, (__bf16)y};
-        *hi = __builtin_bit_cast(uint32_t, h);
-        const bf16x2 r = {(__bf16)(x - __uint_as_float(*hi << 16)), (__bf16)(y - __uint_as_float(*hi & 0xffff0000u))};
-        *lo = __builtin_bit_cast(uint32_t, r);
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            part[k] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            x -= __uint_as_float(a & 0xffff0000u);
+            y -= __uint_as_float(b & 0xffff0000u);
+        }
     } else {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        *hi = __builtin_bit_cast(uint32_t, h);
-        *lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+            const f16x2 h = {(f16)x, (f16)y};
+            part[k] = __builtin_bit_cast(uint32_t, h);
+            x -= (float)h[0];
+            y -= (float)h[1];
+        }
     }
 }
 
@@ -428,15 +442,15 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                     m = top;
                 }
                 const float base = m - kShift;
-                u32x4 ph, pl;
+                u32x4 p[kParts<BF>];
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(x[i] - base), p1 = __builtin_amdgcn_exp2f(x[i + 1] - base);
                     l += p0 + p1;
-                    uint32_t h, r;
-                    split_pair<BF>(p0, p1, &h, &r);
-                    ph[i >> 1] = h;
-                    pl[i >> 1] = r;
+                    uint32_t part[kParts<BF>];
+                    split_pair<BF>(p0, p1, part);
+#pragma unroll
+                    for (int k = 0; k < kParts<BF>; k++) p[k][i >> 1] = part[k];
                 }
 #pragma unroll
                 for (int c = 0; c < VW; c++) {
@@ -446,10 +460,11 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                         a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][c], vf[2 * i][c], 0x05040100u);
                         b[i] = __builtin_amdgcn_perm(vf[2 * i + 1][c], vf[2 * i][c], 0x07060302u);
                     }
-                    o[2 * c] = mfma<BF>(a, ph, o[2 * c]);
-                    o[2 * c + 1] = mfma<BF>(b, ph, o[2 * c + 1]);
-                    o[2 * c] = mfma<BF>(a, pl, o[2 * c]);
-                    o[2 * c + 1] = mfma<BF>(b, pl, o[2 * c + 1]);
+#pragma unroll
+                    for (int k = 0; k < kParts<BF>; k++) {
+                        o[2 * c] = mfma<BF>(a, p[k], o[2 * c]);
+                        o[2 * c + 1] = mfma<BF>(b, p[k], o[2 * c + 1]);
+                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);

@@ -1,0 +1,56 @@
+"""What the serving operators keep of their intermediate values, and what they
+make of infinite ones, against the formulas in 64 bits.
+
+Tolerances, derived: the output's own rounding, 2^-11 (FP16) or 2^-8 (BF16) of
+its value plus half the least subnormal; what precedes it in FP32 is stated at
+each test."""
+import pytest
+import torch
+
+from libortho_amd import _C_ops
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D,n", [(64, 3), (128, 3), (80, 600), (256, 34), (128, 9000)])
+def test_attention_weights_keep_their_bits(gpu, D, n, dtype):
+    # Key 0 has the largest score, keys 1 and 2 weights of about a half that
+    # nearly agree and opposite values, all others the value zero: the output
+    # is the difference of two weights, far below both.  The scores (one
+    # product each) are exact; what is made of keys 1 and 2 (magnitude below 1)
+    # errs by 2^-24 in the scaling, the subtraction and 2^-23 in the
+    # exponential of a weight, below 2^-21 in the difference of the two over a
+    # sum of at least 2.
+    dt = DT[dtype]
+    rng = torch.Generator().manual_seed(D + n)
+    H = 16
+    k = torch.zeros(n, D)
+    k[:, 0] = -30.0
+    k[0, 0], k[1, 0], k[2, 0] = 1.0, 0.125, 0.125 - 2.0 ** -10
+    v = torch.zeros(n, D)
+    v[1], v[2] = 1.0, -1.0
+    q = torch.zeros(1, H, D)
+    q[0, :, 0] = torch.randint(128, 256, (H,), generator=rng) / 256.0
+    q, k, v = q.to(dt).cuda(), k.to(dt).cuda(), v.to(dt).cuda()
+    P = 16
+    pages = -(-n // P)
+    kc, vc = (torch.zeros(pages * P, 1, D, dtype=dt, device="cuda") for _ in range(2))
+    kc[:n, 0], vc[:n, 0] = k, v
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    for scale in (1.0, 0.75, 0.5):
+        got = _C_ops.paged_attention(q, kc.view(pages, P, 1, D), vc.view(pages, P, 1, D), table, i32([n - 1]),
+                                     scale=scale)[0].double().cpu()
+        s = q[0].double().cpu() @ k.double().cpu().T.contiguous() * scale
+        want = torch.softmax(s, -1) @ v.double().cpu()
+        bound = U[dt] * 1.01 * want.abs() + TINY[dt] + 2.0 ** -21
+        err = (got - want).abs()
+        assert bool((err <= bound).all()), (scale, float(err.max()), float(want.abs().max()))
