@@ -440,8 +440,9 @@ int orth_paged_attention_hip(const orth_hip_cache_t *cache, const orth_hip_atten
  *   out[m] = y[m] + scales[i] * (x[m] a[i]^T) b[i]^T,  i = adapters[m]
  * (out[m] = y[m] where i lies outside [0, count)); a[i] is [rank,
  * in_features], b[i] [out_features, rank], both contiguous.  Products are
- * exact, sums FP32, one rounding at the end.  out may be y (the same
- * stride); other overlaps give unspecified values. */
+ * exact, sums and the low-rank values FP32 (FP16: those below 2^-15 of their
+ * token's largest keep 2^-39 of it), one rounding at the end.  out may be y
+ * (the same stride); other overlaps give unspecified values. */
 #define ORTH_ADAPTER_RANK 256
 typedef struct {
     const void *x;               /* [tokens, in_features], row stride x_stride */

@@ -13,10 +13,10 @@
 // product is formed for all columns and kept in those of its own tokens: a
 // run of one prompt's tokens is one product, a decode batch of 16 requests
 // reads each of their adapters once, and what one adapter holds cannot reach
-// another's tokens.  The low-rank values enter the second product as two
-// 16-bit parts (16 bits of them or more; one part would cost as much as the
-// output's own rounding), FP16 ones scaled by a power of two per token, so
-// that none overflows or loses its low bits.
+// another's tokens.  The low-rank values enter the second product as FP32
+// values do: as 16-bit parts (three in BF16, two in FP16), whose products with
+// B are exact and add up in FP32; FP16 ones are scaled by a power of two per
+// token, so that none overflows or loses its low bits.
 //
 // Bound by reading the adapters (few tokens: workgroups of 16 tokens, a slot
 // for each adapter among them, then waves that split the adapters) or x, y
@@ -538,15 +538,21 @@ __device__ __forceinline__ void low_sum(const AdapterArgs &g, int64_t m, int j0,
 }
 
 // Sixteen tokens' low-rank values (of token col, ranks 32 kk + 8 lg .. + 7 in
-// a lane), FP32 in `dst`, become their two parts there; returns the power of
-// two that the lane's token was scaled by.
+// a lane), FP32 in the first two of the kLowParts<BF> words of each kk in
+// `dst`, become their 16-bit parts there; returns the power of two that the
+// lane's token was scaled by.  BF16: three parts of eight bits, cut off, whose
+// sum is the value exactly.  FP16: two of eleven bits, rounded to nearest (the
+// second one's sign is a bit more): 2^-24 of the value, as an FP32 operation's
+// rounding, or 2^-39 of the token's largest where that is more.
+template <bool BF>
+constexpr int kLowParts = BF ? 3 : 2;
 template <bool BF>
 __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
     const int lane = threadIdx.x & 63;
     int sh = 0;
     if constexpr (!BF) {
         float top = 0.f;
-        for (int x = 0; x < 2 * kks; x++) {
+        for (int x = 0; x < 2 * kks; x++) {  // (two parts: no word between)
             const f32x4 v = __builtin_bit_cast(f32x4, dst[x * 64 + lane]);
             top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
         }
@@ -557,27 +563,26 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
         if (top > 0.f && top < __builtin_inff()) sh = 15 - __builtin_amdgcn_frexp_expf(top);
     }
     for (int kk = 0; kk < kks; kk++) {
-        const f32x4 v[2] = {__builtin_bit_cast(f32x4, dst[(2 * kk) * 64 + lane]),
-                            __builtin_bit_cast(f32x4, dst[(2 * kk + 1) * 64 + lane])};
-        u32x4 h, l;
+        u32x4 *word = dst + kk * kLowParts<BF> * 64 + lane;
+        const f32x4 v[2] = {__builtin_bit_cast(f32x4, word[0]), __builtin_bit_cast(f32x4, word[64])};
+        u32x4 part[kLowParts<BF>];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            uint32_t hw = 0, lw = 0;
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float x0 = v[i >> 1][(2 * i + e) & 3], x = BF ? x0 : __builtin_amdgcn_ldexpf(x0, sh);
-                const uint16_t hb = store16<BF>(x);
-                const float hv = load16<BF>(hb);
-                // (an infinity has no rest)
-                const uint16_t lb = fabsf(hv) < __builtin_inff() ? store16<BF>(x - hv) : 0;
-                hw |= (uint32_t)hb << (16 * e);
-                lw |= (uint32_t)lb << (16 * e);
+                const float x0 = v[i >> 1][(2 * i + e) & 3];
+                float x = BF ? x0 : __builtin_amdgcn_ldexpf(x0, sh);
+                const bool finite = fabsf(x) < __builtin_inff();
+#pragma unroll
+                for (int k = 0; k < kLowParts<BF>; k++) {
+                    const uint16_t b = !BF ? store16<BF>(x) : x == x ? (uint16_t)(__float_as_uint(x) >> 16) : (uint16_t)0x7fc0;
+                    part[k][i] = e == 0 ? b : part[k][i] | (uint32_t)b << 16;
+                    x = finite ? x - load16<BF>(b) : 0.f;  // (an infinity or a NaN has no rest)
+                }
             }
-            h[i] = hw;
-            l[i] = lw;
         }
-        dst[(2 * kk) * 64 + lane] = h;
-        dst[(2 * kk + 1) * 64 + lane] = l;
+#pragma unroll
+        for (int k = 0; k < kLowParts<BF>; k++) word[64 * k] = part[k];
     }
     return sh;
 }
@@ -593,13 +598,14 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
 template <int CB, bool BF, int W, bool YV, int KB>
 __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(AdapterArgs g) {
     constexpr int IDS = (CB == 1 ? 4 : 2) / KB;  // adapters whose loads are in flight together (as many as registers hold)
-    extern __shared__ u32x4 parts[];             // [4][kks][2][64]
+    constexpr int PT = kLowParts<BF>;
+    extern __shared__ u32x4 parts[];             // [4][kks][PT][64]
     __shared__ int shifts[kTokens];
     int tile, block;
     place_of(g, blockIdx.x, g.blocks, &tile, &block);
     if (tile >= g.tiles) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, lg = lane >> 4;
-    const int kks = (g.a.rank + 31) / 32, each = kks * 128;
+    const int kks = (g.a.rank + 31) / 32, each = kks * PT * 64;
     const int64_t m0 = (int64_t)tile * 16 * CB, N = g.a.out_features;
     // the tokens: CB 1, of column col; CB 4, of lane
     int mine, m1 = 0;
@@ -695,17 +701,18 @@ __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(Adap
                 v[0] *= scale;
                 v[1] *= scale;
             }
-            parts[group * each + (2 * kk) * 64 + lane] = __builtin_bit_cast(u32x4, v[0]);
-            parts[group * each + (2 * kk + 1) * 64 + lane] = __builtin_bit_cast(u32x4, v[1]);
+            parts[group * each + (PT * kk) * 64 + lane] = __builtin_bit_cast(u32x4, v[0]);
+            parts[group * each + (PT * kk + 1) * 64 + lane] = __builtin_bit_cast(u32x4, v[1]);
         }
     __syncthreads();
     if constexpr (CB == 1) {
         // (x, the rank words, dealt over the waves)
         for (int x = wave; any && x < 2 * kks; x += 4) {
-            f32x4 v = __builtin_bit_cast(f32x4, parts[x * 64 + lane]);
+            u32x4 *word = parts + (x / 2 * PT + x % 2) * 64 + lane;
+            f32x4 v = __builtin_bit_cast(f32x4, *word);
 #pragma unroll
-            for (int w = 1; w < 4; w++) v += __builtin_bit_cast(f32x4, parts[w * each + x * 64 + lane]);
-            parts[x * 64 + lane] = __builtin_bit_cast(u32x4, v * scale);
+            for (int w = 1; w < 4; w++) v += __builtin_bit_cast(f32x4, word[w * each]);
+            *word = __builtin_bit_cast(u32x4, v * scale);
         }
         __syncthreads();
     }
@@ -736,12 +743,15 @@ __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(Adap
 #pragma unroll
                     for (int k = 0; k < KB; k++)
                         if (kk0 + k < kks) {
-                            const u32x4 *p = parts + c * each + (kk0 + k) * 128 + lane;
-                            const u32x4 h = p[0], l = p[64];
+                            const u32x4 *word = parts + c * each + (kk0 + k) * PT * 64 + lane;
 #pragma unroll
-                            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], h, d[t]);
+                            for (int j = 0; j < PT; j++) {
+                                const u32x4 p = word[64 * j];
 #pragma unroll
-                            for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], l, d[t]);
+                                for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], p, d[t]);
+                                // (a part at a time: three together take registers for a third wave a SIMD)
+                                if constexpr (CB == 1 && BF) __builtin_amdgcn_sched_barrier(0);
+                            }
                         }
                     if (tokens >> col & 1) {
 #pragma unroll
@@ -849,7 +859,7 @@ hipError_t down_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream
 
 template <int CB, bool BF>
 hipError_t up_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) {
-    const size_t lds = (size_t)4 * ((g.a.rank + 31) / 32) * 128 * sizeof(u32x4);
+    const size_t lds = (size_t)4 * ((g.a.rank + 31) / 32) * kLowParts<BF> * 64 * sizeof(u32x4);
     const bool yv = g.a.out_features % 8 == 0 && multiple(g.a.y, g.a.y_stride, 8) && multiple(g.a.out, g.a.out_stride, 8);
     const bool one = g.a.rank <= 32;  // one step of ranks: more adapters' loads at a time
     auto go = [&](auto kernel) { return launch_lds(kernel, groups, CB == 1 ? 256 : 64 * kUpWaves, lds, stream, g); };

@@ -54,3 +54,39 @@ def test_attention_weights_keep_their_bits(gpu, D, n, dtype):
         bound = U[dt] * 1.01 * want.abs() + TINY[dt] + 2.0 ** -21
         err = (got - want).abs()
         assert bool((err <= bound).all()), (scale, float(err.max()), float(want.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,r", [(3, 16), (40, 40), (600, 64), (70, 256), (900, 200), (520, 20)])
+def test_adapter_keeps_the_bits_of_its_low_rank_values(gpu, M, r, dtype):
+    # Ranks in pairs: A's rows differ in one element's last bit, B's are 1 and
+    # -1, so an output is the difference of low-rank values near 1, far below
+    # them.  They are single products times a scale of 8 bits: exact in FP32,
+    # as is their difference; the output has only its own rounding (and the
+    # sums of a pair's parts in FP32, 2^-22 of 2 a pair at most).
+    dt = DT[dtype]
+    rng = torch.Generator().manual_seed(M + r)
+    K, N, n = 64, 72, 3
+    x = torch.zeros(M, K)
+    x[:, 5] = 1.0 + torch.randint(0, 128, (M,), generator=rng) / 128.0
+    a = torch.zeros(n, r, K)
+    a[:, 0::2, 5] = 1.0
+    a[:, 1::2, 5] = 1.0 - 2.0 ** -8
+    b = torch.zeros(n, N, r)
+    pair = torch.arange(N) % (r // 2)
+    for i in range(n):
+        b[i, torch.arange(N), 2 * pair] = 1.0
+        b[i, torch.arange(N), 2 * pair + 1] = -1.0
+    scales = 1.0 + torch.randint(0, 2 ** 7, (n,), generator=rng) / 128.0
+    ids = torch.randint(-1, n, (M,), generator=rng).int()
+    y = torch.zeros(M, N, dtype=dt, device="cuda")
+    x, a, b = x.to(dt).cuda(), a.to(dt).cuda(), b.to(dt).cuda()
+    got = _C_ops.adapter_add(y, x, a, b, ids.cuda(), scales.cuda()).double().cpu()
+    want = torch.zeros(M, N, dtype=torch.float64)
+    for m, i in enumerate(ids.tolist()):
+        if i >= 0:
+            want[m] = float(scales[i]) * (b[i].double().cpu() @ (a[i].double().cpu() @ x[m].double().cpu()))
+    bound = U[dt] * 1.01 * want.abs() + TINY[dt] + 2.0 ** -21
+    assert float(want.abs().max()) > 2.0 ** -8
+    err = (got - want).abs()
+    assert bool((err <= bound).all()), (float((err - bound).max()), float(err.max()))
