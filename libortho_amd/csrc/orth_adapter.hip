@@ -434,7 +434,7 @@ __device__ __forceinline__ void down_staged(const AdapterArgs &g, int64_t m0, in
 
 template <int RB, int CB, bool BF, int W>
 __global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs g) {
-    extern __shared__ float down_lds[];
+    extern __shared__ __align__(16) float down_lds[];
     // (all first slots in front: most others end at once)
     const int per_slot = gridDim.x / g.slots, slot = blockIdx.x / per_slot;
     int tile, slice;
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(64 * kDown, 4) void adapter_down_kernel(AdapterArgs
     if constexpr (CB == 1) {
         // the slot's adapters: those of every slots-th column that is its
         // adapter's first
-        __shared__ int order[CB == 1 ? 2 * kOrdered : 1];
+        __shared__ __align__(16) int order[CB == 1 ? 2 * kOrdered : 1];  // (its second half is read as vectors)
         if (g.order_by == ORDER_GROUP) {
             order_tokens(g, order);
             if (slice == 0 && slot == 0 && threadIdx.x < 16 && tile * 16 + (int)threadIdx.x < g.a.tokens)

@@ -185,7 +185,9 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     constexpr int VW = EL / 2;                          // words of them
     constexpr bool VTAIL = TAIL || 16 * EL != 32 * KS;
     constexpr float kShift = BF ? 0.f : 14.f;
-    extern __shared__ float lds[];  // o [waves][gt][16 EL + 4], then (m, l) [waves][16]
+    // o [waves][gt][16 EL + 4], then (m, l) [waves][16]; both start at 16 bytes, and so does each row of o
+    extern __shared__ __align__(16) float lds[];
+    static_assert((16 * EL + 4) % 4 == 0, "rows of o");
     const int D = g.c.head_dim, row_floats = 16 * EL + 4;
     float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
