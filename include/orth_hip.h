@@ -309,7 +309,8 @@ int orth_sieve_hdiag_hip(const void *x, int32_t x_dtype, int64_t rows, int64_t i
  * GEMM, /root/reference/torch_bind/bindings.cpp:9-48); they serve the block
  * whose projections orth_layers_forward_hip computes.  All pointers are
  * device memory, strides count elements, and the calls are asynchronous on
- * `stream`.  Contents of index arrays are checked on the device: an index
+ * `stream`; several host threads may call on one stream (a call's launches
+ * stay together).  Contents of index arrays are checked on the device: an index
  * outside its range is skipped as each entry says, never followed.
  *
  * A paged key-value cache: `pages` pages of `page_size` token slots, each

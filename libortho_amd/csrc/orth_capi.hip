@@ -269,7 +269,10 @@ int current_device_ok(int *dev_out) {
 // Split-K workspace of the mid-batch kernels, one per (device, stream): the
 // FP32 partials their reduction kernel sums.  Calls on one stream are
 // ordered; calls on different streams use different workspaces.  Allocation
-// happens on first use (and on growth), outside graph capture only.
+// happens on first use (and on growth), outside graph capture only.  Several
+// host threads may call on one stream: a call holds its stream's workspace
+// (`mu`) from the lookup to its last launch, so that no other call's launches
+// come between those that write the memory and those that read it.
 //
 // A captured call records no allocation: its partials (or the temporary
 // plan of an unplanned prefill call) go to the device's scratch array when
@@ -281,6 +284,7 @@ int current_device_ok(int *dev_out) {
 // no-allocation calls, on the same GPU share that memory and must be
 // ordered by the caller.
 struct Workspace {
+    std::mutex mu;  // held by a call (Held); in front of g_ws_mu where both are
     void *buf = nullptr;
     int64_t part_bytes = 0;
     void *cap = nullptr;  // capture buffer
@@ -290,6 +294,24 @@ struct Workspace {
 std::mutex g_ws_mu;
 std::map<std::pair<int, void *>, Workspace> g_ws;
 std::vector<void *> g_ws_retired;
+using Held = std::unique_lock<std::mutex>;
+
+// The stream's workspace, held by `held` from here on.
+Workspace &stream_workspace(int dev, hipStream_t stream, Held *held) {
+    Workspace *w;
+    {
+        std::lock_guard<std::mutex> lk(g_ws_mu);
+        w = &g_ws[{dev, static_cast<void *>(stream)}];
+    }
+    if (!held->owns_lock()) *held = Held(w->mu);
+    return *w;
+}
+
+// A buffer that in-flight work may still use: kept, not freed.
+void retire(void *p) {
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    g_ws_retired.push_back(p);
+}
 
 int capturing(hipStream_t stream, bool *cap) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -299,16 +321,14 @@ int capturing(hipStream_t stream, bool *cap) {
     return ORTH_OK;
 }
 
-// Memory for a captured call (see above): *out, or ORTH_ERR_UNSUPPORTED.
-int capture_memory(int dev, hipStream_t stream, int64_t bytes, const char *what, void **out) {
+// Memory for a captured call (see above) on the stream of `w`: *out, or ORTH_ERR_UNSUPPORTED.
+int capture_memory(int dev, const Workspace &w, int64_t bytes, const char *what, void **out) {
     if (bytes <= (int64_t)ORTH_NOALLOC_SCRATCH_BYTES) {
         *out = g_dev[dev].scratch;
         return ORTH_OK;
     }
-    std::lock_guard<std::mutex> lk(g_ws_mu);
-    auto it = g_ws.find({dev, static_cast<void *>(stream)});
-    if (it != g_ws.end() && it->second.cap && it->second.cap_bytes >= bytes) {
-        *out = it->second.cap;
+    if (w.cap && w.cap_bytes >= bytes) {
+        *out = w.cap;
         return ORTH_OK;
     }
     return fail(ORTH_ERR_UNSUPPORTED,
@@ -317,23 +337,23 @@ int capture_memory(int dev, hipStream_t stream, int64_t bytes, const char *what,
                 (long long)bytes, what, (long long)ORTH_NOALLOC_SCRATCH_BYTES);
 }
 
-int workspace_for(int dev, hipStream_t stream, int64_t part_bytes, float **part) {
+// (the caller keeps `held` until its last launch)
+int workspace_for(int dev, hipStream_t stream, int64_t part_bytes, float **part, Held *held) {
     bool cap = false;
     int rc = capturing(stream, &cap);
     if (rc != ORTH_OK) return rc;
+    Workspace &w = stream_workspace(dev, stream, held);
     if (cap) {
         void *p = nullptr;
-        rc = capture_memory(dev, stream, part_bytes, "split-K workspace", &p);
+        rc = capture_memory(dev, w, part_bytes, "split-K workspace", &p);
         *part = static_cast<float *>(p);
         return rc;
     }
-    std::lock_guard<std::mutex> lk(g_ws_mu);
-    Workspace &w = g_ws[{dev, static_cast<void *>(stream)}];
     hipError_t e = hipSuccess;
     if (part_bytes > (int64_t)ORTH_NOALLOC_SCRATCH_BYTES && w.cap_bytes < part_bytes) {
         // a capture of this call on this stream will find a buffer (an older,
         // smaller one is retired: graphs captured earlier may still use it)
-        if (w.cap) g_ws_retired.push_back(w.cap);
+        if (w.cap) retire(w.cap);
         w.cap = nullptr;
         w.cap_bytes = 0;
         e = hipMalloc(&w.cap, (size_t)part_bytes);
@@ -346,7 +366,7 @@ int workspace_for(int dev, hipStream_t stream, int64_t part_bytes, float **part)
     }
     if (w.buf) {
         // a smaller buffer is retired, not freed: in-flight work may still use it
-        g_ws_retired.push_back(w.buf);
+        retire(w.buf);
         w.buf = nullptr;
         w.part_bytes = 0;
     }
@@ -517,6 +537,8 @@ int forward_impl(const orth_hip_layer_t *layer, const void *plan, int64_t plan_b
 int launch_kernel(const ForwardArgs &a, const void *plan, int kernel, int dev, hipStream_t stream, bool noalloc) {
     int rc = ORTH_OK;
     hipError_t e = hipSuccess;
+    Held held;  // the stream's workspace, where the call's launches share memory
+    if (noalloc) stream_workspace(dev, stream, &held);
     if (kernel == KERNEL_DECODE) {
         e = launch_decode(a, plan, g_dev[dev].cus, stream);
     } else if (kernel == KERNEL_MID) {
@@ -534,7 +556,7 @@ int launch_kernel(const ForwardArgs &a, const void *plan, int kernel, int dev, h
                             (long long)ORTH_NOALLOC_SCRATCH_BYTES);
             part = static_cast<float *>(g_dev[dev].scratch);
         } else if (pbytes > 0) {
-            rc = workspace_for(dev, stream, pbytes, &part);
+            rc = workspace_for(dev, stream, pbytes, &part, &held);
             if (rc != ORTH_OK) return rc;
         }
         // without a plan the split-K kernel filters each row's CSR by column
@@ -552,7 +574,7 @@ int launch_kernel(const ForwardArgs &a, const void *plan, int kernel, int dev, h
                 return fail(ORTH_ERR_UNSUPPORTED, "prefill K split needs %lld bytes of scratch", (long long)pbytes);
             part = static_cast<float *>(g_dev[dev].scratch);
         } else {
-            rc = workspace_for(dev, stream, pbytes, &part);
+            rc = workspace_for(dev, stream, pbytes, &part, &held);
             if (rc != ORTH_OK) return rc;
         }
         e = launch_prefill(a, a.has_ortho ? plan : nullptr, stream, part, S);
@@ -582,7 +604,7 @@ int launch_kernel(const ForwardArgs &a, const void *plan, int kernel, int dev, h
             if (rc != ORTH_OK) return rc;
             if (cap) {
                 void *p = nullptr;
-                rc = capture_memory(dev, stream, pb, "temporary ortho plan (pass a plan to capture this call)", &p);
+                rc = capture_memory(dev, stream_workspace(dev, stream, &held), pb, "temporary ortho plan (pass a plan to capture this call)", &p);
                 if (rc != ORTH_OK) return rc;
                 e = launch_plan_build_prefill(a, p, stream);
                 if (e == hipSuccess) e = pf(p);
@@ -680,8 +702,9 @@ int group_forward_impl(const orth_hip_layer_t *const *layers, const void *const 
             hipStream_t stream = static_cast<hipStream_t>(stream_v);
             const int64_t pbytes = split_group_workspace_bytes(as, count);
             float *part = nullptr;
+            Held held;
             if (pbytes > 0) {
-                rc = workspace_for(dev, stream, pbytes, &part);
+                rc = workspace_for(dev, stream, pbytes, &part, &held);
                 if (rc != ORTH_OK) return rc;
             }
             hipError_t e = launch_split_group(as, spl, count, part, stream);
@@ -712,13 +735,13 @@ int host_device(int *dev, int *cus) {
     if (rc == ORTH_OK) *cus = g_dev[*dev].cus;
     return rc;
 }
-int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p) {
+int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p, std::unique_lock<std::mutex> *held) {
     float *f = nullptr;
-    int rc = workspace_for(dev, stream, bytes, &f);
+    int rc = workspace_for(dev, stream, bytes, &f, held);
     *p = f;
     return rc;
 }
-int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p) {
+int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p, std::unique_lock<std::mutex> *held) {
     *p = nullptr;
     if (count > kCounters)
         return fail(ORTH_ERR_UNSUPPORTED, "a call needs %lld counters, more than %lld", (long long)count, (long long)kCounters);
@@ -729,8 +752,7 @@ int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p) {
         *p = static_cast<uint32_t *>(g_dev[dev].counters);
         return ORTH_OK;
     }
-    std::lock_guard<std::mutex> lk(g_ws_mu);
-    Workspace &w = g_ws[{dev, static_cast<void *>(stream)}];
+    Workspace &w = stream_workspace(dev, stream, held);
     if (!w.counters) {
         void *mem = nullptr;
         hipError_t e = hipMalloc(&mem, kCounters * sizeof(uint32_t));

@@ -6,15 +6,19 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace orth {
 
 int host_fail(int status, const char *message);
 int host_fail_hip(hipError_t e, const char *what);
 void host_begin();  // clears the thread's error message
 int host_device(int *dev, int *cus);
-int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p);
+// Both take the stream's workspace into `held`, which the caller keeps until
+// the call's last launch: other threads' calls on the stream wait there.
+int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p, std::unique_lock<std::mutex> *held);
 // Counters that are zero between calls (each kernel that counts in them leaves
 // zeros): the stream's own, or, under capture, those of all captured calls.
-int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p);
+int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p, std::unique_lock<std::mutex> *held);
 
 }  // namespace orth

@@ -172,9 +172,10 @@ int orth_paged_attention_hip(const orth_hip_cache_t *c, const orth_hip_attend_t 
         void *work = nullptr;
         uint32_t *counters = nullptr;
         int64_t groups = 0;
+        std::unique_lock<std::mutex> held;
         const int64_t bytes = attention_workspace_bytes(*c, *a, cus, &groups);
-        if ((rc = host_workspace(dev, static_cast<hipStream_t>(stream), bytes, &work)) != ORTH_OK) return rc;
-        if ((rc = host_counters(dev, static_cast<hipStream_t>(stream), groups, &counters)) != ORTH_OK) return rc;
+        if ((rc = host_workspace(dev, static_cast<hipStream_t>(stream), bytes, &work, &held)) != ORTH_OK) return rc;
+        if ((rc = host_counters(dev, static_cast<hipStream_t>(stream), groups, &counters, &held)) != ORTH_OK) return rc;
         hipError_t e = launch_paged_attention(*c, *a, cus, work, counters, static_cast<hipStream_t>(stream));
         return e == hipSuccess ? (int)ORTH_OK : host_fail_hip(e, "paged attention launch");
     });
@@ -211,8 +212,10 @@ int orth_adapter_add_hip(const orth_hip_adapter_t *a, void *stream) {
         int rc = host_device(&dev, &cus);
         if (rc != ORTH_OK) return rc;
         void *work = nullptr;
+        std::unique_lock<std::mutex> held;
         const int64_t bytes = adapter_workspace_bytes(*a, cus);
-        if (bytes > 0 && (rc = host_workspace(dev, static_cast<hipStream_t>(stream), bytes, &work)) != ORTH_OK) return rc;
+        if (bytes > 0 && (rc = host_workspace(dev, static_cast<hipStream_t>(stream), bytes, &work, &held)) != ORTH_OK)
+            return rc;
         hipError_t e = launch_adapter_add(*a, cus, work, static_cast<hipStream_t>(stream));
         return e == hipSuccess ? (int)ORTH_OK : host_fail_hip(e, "adapter launch");
     });
