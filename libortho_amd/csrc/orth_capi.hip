@@ -207,6 +207,17 @@ static __device__ __align__(256) unsigned char scratch[ORTH_NOALLOC_SCRATCH_BYTE
 constexpr int64_t kCounters = 4096;
 static __device__ uint32_t counters[kCounters];
 
+// A stream's name among the host's records: its handle, but hipStreamPerThread
+// is one handle for a stream of each thread, so it is named by the thread (odd
+// numbers, which no handle of a stream is; never given again, as a thread's
+// last calls may outlive it, so its workspace stays allocated).
+void *stream_name(hipStream_t stream) {
+    if (stream != hipStreamPerThread) return static_cast<void *>(stream);
+    static std::atomic<uintptr_t> next{17};
+    thread_local const uintptr_t name = next.fetch_add(2, std::memory_order_relaxed);
+    return reinterpret_cast<void *>(name);
+}
+
 // Per-device check that the current device is a gfx950 (the only code object
 // this library carries), one-time kernel attribute set-up, and the device
 // address of the scratch array.
@@ -220,7 +231,7 @@ struct DeviceState {
     // its stream), so that a call on another stream waits for it before it
     // touches the scratch array
     hipEvent_t noalloc_done = nullptr;
-    hipStream_t noalloc_stream = nullptr;
+    void *noalloc_stream = nullptr;  // (stream_name)
     bool noalloc_recorded = false;
     std::mutex noalloc_mu;
 };
@@ -301,7 +312,7 @@ Workspace &stream_workspace(int dev, hipStream_t stream, Held *held) {
     Workspace *w;
     {
         std::lock_guard<std::mutex> lk(g_ws_mu);
-        w = &g_ws[{dev, static_cast<void *>(stream)}];
+        w = &g_ws[{dev, stream_name(stream)}];
     }
     if (!held->owns_lock()) *held = Held(w->mu);
     return *w;
@@ -513,7 +524,7 @@ int forward_impl(const orth_hip_layer_t *layer, const void *plan, int64_t plan_b
         if (noalloc_order) {
             DeviceState &st = g_dev[dev];
             noalloc_lk = std::unique_lock<std::mutex>(st.noalloc_mu);
-            if (st.noalloc_recorded && st.noalloc_stream != stream) {
+            if (st.noalloc_recorded && st.noalloc_stream != stream_name(stream)) {
                 ce = hipStreamWaitEvent(stream, st.noalloc_done, 0);
                 if (ce != hipSuccess) return fail_hip(ce, "hipStreamWaitEvent (no-allocation ordering)");
             }
@@ -524,7 +535,7 @@ int forward_impl(const orth_hip_layer_t *layer, const void *plan, int64_t plan_b
         DeviceState &st = g_dev[dev];
         hipError_t ce = hipEventRecord(st.noalloc_done, stream);
         if (ce != hipSuccess) return fail_hip(ce, "hipEventRecord (no-allocation ordering)");
-        st.noalloc_stream = stream;
+        st.noalloc_stream = stream_name(stream);
         st.noalloc_recorded = true;
     }
     if (rc != ORTH_OK) return rc;

@@ -2,6 +2,7 @@
 // time, over the stand-ins of threads_stubs.hip.
 #include <cstdio>
 #include <functional>
+#include <set>
 #include <thread>
 #include <vector>
 
@@ -79,6 +80,14 @@ int main() {
     // streams of their own do not wait for each other
     run({[&] { return adapter(one); }, [&] { return adapter(two); }}, "two streams");
     expect(threads::together > 0, "two streams at once");
+
+    // hipStreamPerThread is one handle and a stream of each thread: no memory in common
+    run({[&] { return adapter(hipStreamPerThread); }, [&] { return attend(hipStreamPerThread); }}, "streams per thread");
+    expect(threads::works.size() == 2, "two threads");
+    {
+        const std::set<void *> &a = threads::works.begin()->second, &b = threads::works.rbegin()->second;
+        for (void *p : a) expect(b.count(p) == 0, "the workspaces of two threads' own streams");
+    }
 
     if (failures) return 1;
     std::printf("threads ok\n");
