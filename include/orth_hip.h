@@ -310,8 +310,11 @@ int orth_sieve_hdiag_hip(const void *x, int32_t x_dtype, int64_t rows, int64_t i
  * whose projections orth_layers_forward_hip computes.  All pointers are
  * device memory, strides count elements, and the calls are asynchronous on
  * `stream`; several host threads may call on one stream (a call's launches
- * stay together).  Contents of index arrays are checked on the device: an index
- * outside its range is skipped as each entry says, never followed.
+ * stay together).  Captured calls on one GPU share memory: graph replays that
+ * overlap one another, and calls on parallel branches of one graph, must be
+ * ordered by the caller; nothing carries over from one to the next.  Contents
+ * of index arrays are checked on the device: an index outside its range is
+ * skipped as each entry says, never followed.
  *
  * A paged key-value cache: `pages` pages of `page_size` token slots, each
  * slot holding kv_heads vectors of head_dim elements in k_cache and in

@@ -754,9 +754,11 @@ hipError_t attend_by_width(const AttendArgs &g, int64_t groups, hipStream_t stre
 }  // namespace
 
 int64_t attention_workspace_bytes(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, int64_t *groups) {
-    const AttendArgs g = attend_args(c, a, cus, groups);
-    return *groups * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2))) +
-           (*groups + kPieces - 1) / kPieces * (int64_t)sizeof(int4);
+    int64_t n = 0;
+    const AttendArgs g = attend_args(c, a, cus, &n);
+    *groups = attend_units(g) > 1 ? n : 0;  // (items of one unit are not split)
+    return n * (2 * g.nh * (g.gt * (int64_t)c.head_dim * 4 + 16 * (int64_t)sizeof(float2))) +
+           (n + kPieces - 1) / kPieces * (int64_t)sizeof(int4);
 }
 
 hipError_t launch_paged_attention(const orth_hip_cache_t &c, const orth_hip_attend_t &a, int cus, void *work, uint32_t *counters,

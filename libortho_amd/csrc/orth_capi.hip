@@ -202,10 +202,14 @@ int resolve(const orth_hip_layer_t *L, const void *input, void *output, int64_t 
 // is used.
 static __device__ __align__(256) unsigned char scratch[ORTH_NOALLOC_SCRATCH_BYTES];
 
-// Counters of captured calls (host_counters), zero from the start; by their
-// device address, as above.
+// Counters of captured calls (host_counters); by their device address, as
+// above.  Each call clears those that it takes: replays that overlapped, or
+// calls on parallel branches of a graph, may have left any counts there.
 constexpr int64_t kCounters = 4096;
 static __device__ uint32_t counters[kCounters];
+static __global__ void clear_counters(uint32_t *p, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
+}
 
 // A stream's name among the host's records: its handle, but hipStreamPerThread
 // is one handle for a stream of each thread, so it is named by the thread (odd
@@ -291,7 +295,8 @@ int current_device_ok(int *dev_out) {
 // calls on that stream size (allocated only for requests larger than the
 // scratch array), else the call is refused.  Eager calls never touch either,
 // so a graph replayed on any stream, beside eager calls on any stream, does
-// not race with them; replays of graphs that overlap one another, or
+// not race with them; replays of graphs that overlap one another, calls on
+// parallel branches of one graph, or
 // no-allocation calls, on the same GPU share that memory and must be
 // ordered by the caller.
 struct Workspace {
@@ -754,14 +759,18 @@ int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p, std::un
 }
 int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p, std::unique_lock<std::mutex> *held) {
     *p = nullptr;
+    if (count == 0) return ORTH_OK;
     if (count > kCounters)
         return fail(ORTH_ERR_UNSUPPORTED, "a call needs %lld counters, more than %lld", (long long)count, (long long)kCounters);
     bool cap = false;
     int rc = capturing(stream, &cap);
     if (rc != ORTH_OK) return rc;
     if (cap) {
+        stream_workspace(dev, stream, held);
         *p = static_cast<uint32_t *>(g_dev[dev].counters);
-        return ORTH_OK;
+        clear_counters<<<1, 256, 0, stream>>>(*p, (int)count);
+        hipError_t e = hipGetLastError();
+        return e == hipSuccess ? (int)ORTH_OK : fail_hip(e, "counters' launch");
     }
     Workspace &w = stream_workspace(dev, stream, held);
     if (!w.counters) {

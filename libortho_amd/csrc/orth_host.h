@@ -17,8 +17,10 @@ int host_device(int *dev, int *cus);
 // Both take the stream's workspace into `held`, which the caller keeps until
 // the call's last launch: other threads' calls on the stream wait there.
 int host_workspace(int dev, hipStream_t stream, int64_t bytes, void **p, std::unique_lock<std::mutex> *held);
-// Counters that are zero between calls (each kernel that counts in them leaves
-// zeros): the stream's own, or, under capture, those of all captured calls.
+// Counters that are zero when the call's kernels begin: the stream's own,
+// which each kernel that counts in them leaves at zero, or, under capture,
+// those of all captured calls, cleared by a launch in front (a graph's replays
+// find whatever other graphs left there).
 int host_counters(int dev, hipStream_t stream, int64_t count, uint32_t **p, std::unique_lock<std::mutex> *held);
 
 }  // namespace orth

@@ -14,6 +14,7 @@ const hipStream_t kCapturing = reinterpret_cast<hipStream_t>(0x4000);
 // launches inside on each stream; how often one came in while another of its
 // stream, or of any stream, was inside
 extern std::atomic<int> inside[kStreams], overlaps, together, all;
+extern std::atomic<int> kernels;  // launched by the host side itself
 extern std::mutex mu;
 extern std::map<void *, std::set<void *>> works;
 void launch(hipStream_t stream, void *work);

@@ -89,6 +89,11 @@ int main() {
         for (void *p : a) expect(b.count(p) == 0, "the workspaces of two threads' own streams");
     }
 
+    // captured attention records the clearing of its counters, eager attention none
+    threads::kernels = 0;
+    expect(attend(one) == ORTH_OK && threads::kernels == 0, "eager counters");
+    expect(attend(threads::kCapturing) == ORTH_OK && threads::kernels == 1, "captured counters start from zero");
+
     if (failures) return 1;
     std::printf("threads ok\n");
     return 0;
