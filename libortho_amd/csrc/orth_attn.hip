@@ -168,12 +168,29 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t part[kPart
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             typedef f16 f16x2 __attribute__((ext_vector_type(2)));
-            const f16x2 h = {(f16)x, (f16)y};
+            f16x2 h = {(f16)x, (f16)y};
+            // (a first part is not zero, so that a weight times an infinite
+            // value is infinite; the second part takes it back)
+            if (k == 0) h = __builtin_elementwise_max(h, f16x2{(f16)0x1p-24f, (f16)0x1p-24f});
             part[k] = __builtin_bit_cast(uint32_t, h);
             x -= (float)h[0];
             y -= (float)h[1];
         }
     }
+}
+
+// 16-bit elements with infinities (and NaN) as the type's largest numbers: what
+// the parts behind the first of a split factor are multiplied with.  A zero
+// part times an infinity would be a NaN, and one of the other sign would turn
+// the first part's infinity into one.  (As whole numbers, values without a
+// sign bit lie below 2^15 in order, those with one above.)
+template <bool BF>
+__device__ __forceinline__ u32x4 finite16(u32x4 v) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+    constexpr int16_t most = BF ? 0x7f7f : 0x7bff;
+    const u16x8 u = __builtin_elementwise_min(__builtin_bit_cast(u16x8, v), (u16x8)(uint16_t)(most | 0x8000));
+    return __builtin_bit_cast(u32x4, __builtin_elementwise_min(__builtin_bit_cast(i16x8, u), (i16x8)most));
 }
 
 // KS: steps of 32 elements over head_dim; PG8: page_size is a multiple of 8,
@@ -466,6 +483,10 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                     for (int k = 0; k < kParts<BF>; k++) {
                         o[2 * c] = mfma<BF>(a, p[k], o[2 * c]);
                         o[2 * c + 1] = mfma<BF>(b, p[k], o[2 * c + 1]);
+                        if (k == 0) {
+                            a = finite16<BF>(a);
+                            b = finite16<BF>(b);
+                        }
                     }
                 }
             }

@@ -90,3 +90,40 @@ def test_adapter_keeps_the_bits_of_its_low_rank_values(gpu, M, r, dtype):
     assert float(want.abs().max()) > 2.0 ** -8
     err = (got - want).abs()
     assert bool((err <= bound).all()), (float((err - bound).max()), float(err.max()))
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D,P,n", [(128, 16, 300), (64, 7, 90), (80, 16, 40), (256, 8, 33), (128, 16, 9000), (128, 32, 20)])
+def test_attention_of_infinite_values_in_sight(gpu, D, P, n, dtype):
+    # a value of a key in sight that is infinite makes its element infinite for
+    # every query head of that key head, two of opposite signs or a NaN a NaN;
+    # all other elements stay as they are without them
+    dt = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(D + n)
+    G, H = 2, 6
+    pages = -(-n // P)
+    q = (2 * torch.randn(1, H, D, generator=g, device="cuda")).to(dt)
+    kc, vc = (torch.randn(pages, P, G, D, generator=g, device="cuda").to(dt) for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    pos = i32([n - 1])
+    plain = _C_ops.paged_attention(q, kc, vc, table, pos)
+    flat = vc.flatten(0, 1)  # (a view)
+    put = {(0, 3): {0: INF}, (0, 4): {n - 1: -INF}, (0, 5): {0: INF, n // 2: INF}, (1, 3): {n // 3: NAN},
+           (1, 0): {1: INF, n - 1: -INF}, (1, D - 1): {n // 2: -INF}}
+    for (h, d), keys in put.items():
+        for j, v in keys.items():
+            flat[j, h, d] = v
+    got = _C_ops.paged_attention(q, kc, vc, table, pos)
+    for h in range(H):
+        for d in range(D):
+            vals = put.get((h // (H // G), d))
+            if vals is None:
+                continue
+            want = sum(vals.values())
+            x = float(got[0, h, d])
+            assert (x != x) if want != want else x == want, (h, d, x, want)
+            plain[0, h, d] = got[0, h, d] = 0
+    assert torch.equal(got, plain)
