@@ -554,13 +554,14 @@ __device__ __forceinline__ int low_parts(int kks, u32x4 *dst) {
         float top = 0.f;
         for (int x = 0; x < 2 * kks; x++) {  // (two parts: no word between)
             const f32x4 v = __builtin_bit_cast(f32x4, dst[x * 64 + lane]);
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fabsf(v[e]) < __builtin_inff() ? fmaxf(top, fabsf(v[e])) : top;
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        // the largest to 2^14: its parts are normal numbers and so are those
+        // the largest finite one to 2^14: its parts are normal numbers and so are those
         // of values 2^-17 of it
-        if (top > 0.f && top < __builtin_inff()) sh = 15 - __builtin_amdgcn_frexp_expf(top);
+        if (top > 0.f) sh = 15 - __builtin_amdgcn_frexp_expf(top);
     }
     for (int kk = 0; kk < kks; kk++) {
         u32x4 *word = dst + kk * kLowParts<BF> * 64 + lane;
@@ -749,8 +750,9 @@ __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(Adap
                                 const u32x4 p = word[64 * j];
 #pragma unroll
                                 for (int t = 0; t < 4; t++) d[t] = mfma<BF>(bv[i][k][t], p, d[t]);
-                                // (a part at a time: three together take registers for a third wave a SIMD)
-                                if constexpr (CB == 1 && BF) __builtin_amdgcn_sched_barrier(0);
+                                // (a part at a time: three together take registers that a third wave a
+                                // SIMD, or outputs that are not vectors, have need of)
+                                if constexpr (BF && (CB == 1 || !YV)) __builtin_amdgcn_sched_barrier(0);
                             }
                         }
                     if (tokens >> col & 1) {
@@ -761,6 +763,40 @@ __global__ __launch_bounds__(CB == 1 ? 256 : 512, 2) void adapter_up_kernel(Adap
         }
         next();
         load_b(0);
+    }
+    // An infinite element of B times a zero part, or one of another sign than
+    // the first part, makes a NaN of the sum: those sums are formed again of
+    // the whole low-rank values, one a lane at a time.
+#pragma unroll
+    for (int c = 0; c < CB; c++) {
+        float none[2] = {0.f, 0.f};  // (a NaN where a sum is infinite or a NaN)
+#pragma unroll
+        for (int e = 0; e < 16; e++) none[e & 1] = __builtin_fmaf(acc[c][e >> 2][e & 3], 0.f, none[e & 1]);
+        if (!__any(none[0] != none[1])) continue;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int e = 0; e < 16; e++) odd |= (uint32_t)(acc[c][e >> 2][e & 3] != acc[c][e >> 2][e & 3]) << e;
+        const int id = CB == 1 ? mine : __shfl(mine, 16 * c + col, 64);
+#pragma unroll 1
+        for (; __any(odd != 0); odd &= odd - 1) {
+            const int at = odd ? __ffs(odd) - 1 : 0;
+            float sum = 0.f;
+            if (odd && id >= 0 && n + at < N) {
+                const uint16_t *b = (const uint16_t *)g.a.b + ((int64_t)id * N + n + at) * g.a.rank;
+#pragma unroll 1
+                for (int j = 0; j < g.a.rank; j++) {
+                    const u32x4 *word = parts + c * each + (j >> 5) * PT * 64 + (j >> 3 & 3) * 16 + col;
+                    float low = 0.f;
+#pragma unroll
+                    for (int k = 0; k < PT; k++) low += load16<BF>(reinterpret_cast<const uint16_t *>(word + 64 * k)[j & 7]);
+                    sum += low * load16<BF>(b[j]);
+                    if (sum != sum) break;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (odd && e == at) acc[c][e >> 2][e & 3] = sum;
+        }
     }
 #pragma unroll
     for (int c = 0; c < CB; c++) {

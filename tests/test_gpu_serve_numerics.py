@@ -127,3 +127,35 @@ def test_attention_of_infinite_values_in_sight(gpu, D, P, n, dtype):
             assert (x != x) if want != want else x == want, (h, d, x, want)
             plain[0, h, d] = got[0, h, d] = 0
     assert torch.equal(got, plain)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,r,N", [(3, 16, 264), (40, 40, 100), (600, 64, 264), (70, 200, 72), (900, 20, 130), (530, 3, 33)])
+def test_adapters_of_infinite_weights(gpu, M, r, N, dtype):
+    # an infinite element of B makes its output infinite (with the sign of the
+    # low-rank value), of A whatever the formula says, one of the adapter's low-rank
+    # values infinite and the others as large as they were
+    dt = DT[dtype]
+    K, n = 72, 2
+    g = torch.Generator(device="cuda").manual_seed(M + r)
+    x = (torch.rand(M, K, generator=g, device="cuda") + 0.5).to(dt)
+    a = (torch.rand(n, r, K, generator=g, device="cuda") + 0.5).to(dt)
+    b = (torch.rand(n, N, r, generator=g, device="cuda") + 0.5).to(dt)
+    y = torch.randn(M, N, generator=g, device="cuda").to(dt)
+    ids = (torch.arange(M, device="cuda") % n).int()
+    plain = _C_ops.adapter_add(y, x, a, b, ids)
+    b[0, 5, 0], b[0, 6, r - 1], b[0, 7, 1] = INF, -INF, NAN
+    got = _C_ops.adapter_add(y, x, a, b, ids)
+    of = (ids == 0).nonzero().flatten()
+    assert bool((got[of, 5] == INF).all()) and bool((got[of, 6] == -INF).all()) and bool(got[of, 7].isnan().all())
+    got[of, 5:8] = plain[of, 5:8] = 0
+    assert torch.equal(got, plain)
+    # one infinite low-rank value, the others past FP16's largest number
+    big = 200.0
+    x2, a2 = (x * big).to(dt), (a * big).to(dt)
+    a2[1, 0, 3] = INF
+    b2 = torch.ones_like(b)
+    b2[:, :, 1:] = -1.0
+    got = _C_ops.adapter_add(y, x2, a2, b2, ids)
+    of = (ids == 1).nonzero().flatten()
+    assert bool((got[of] == INF).all())
