@@ -596,7 +596,8 @@ def sieve_hdiag(inputs: torch.Tensor, ieee_div: bool = False) -> torch.Tensor:
 # ------------------------------------------------- serving many requests at once
 #
 # What stands between a block's projections; none of it has a counterpart in
-# the reference, whose only operator is ``forward``.
+# the reference, whose only operator is ``forward``.  No gradients: a tensor
+# that requires one is refused unless gradients are switched off.
 
 def _stride(t: torch.Tensor, d: int) -> int:
     return int(t.stride(d)) if t.shape[d] > 1 else 0  # one element: no stride
@@ -605,6 +606,14 @@ def _stride(t: torch.Tensor, d: int) -> int:
 def _index(t: torch.Tensor, dev, n, dtype, msg: str) -> None:
     _req(t.device == dev and t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and (n is None or t.shape[0] == n),
          msg)
+
+
+def _no_gradient(op: str, **tensors) -> None:
+    """None of the operators has a gradient: a tensor that wants one is refused rather than forgotten."""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            _req(t is None or not t.requires_grad,
+                 f"{op} has no gradient: {name} requires one (detach it, or call under torch.no_grad())")
 
 
 def _cache(k: torch.Tensor, v: torch.Tensor) -> _lib.OrthHipCache:
@@ -700,6 +709,7 @@ def cache_append(k, v, k_cache, v_cache, slots, q=None, positions=None, cos_sin=
     T = _lib.torch_ops()
     if T is not None:
         return T.cache_append(k, v, k_cache, v_cache, slots, q, positions, cos_sin, interleaved, q_out)
+    _no_gradient("cache_append", k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q, cos_sin=cos_sin, q_out=q_out)
     c = _cache(k_cache, v_cache)
     dev = k_cache.device
     _req(k.dim() == 3, "k" + _LIKE.format("kv_heads"))
@@ -753,6 +763,7 @@ def paged_attention(q, k_cache, v_cache, block_table, positions, rows=None, scal
     T = _lib.torch_ops()
     if T is not None:
         return T.paged_attention(q, k_cache, v_cache, block_table, positions, rows, scale, window, out)
+    _no_gradient("paged_attention", q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     c = _cache(k_cache, v_cache)
     dev = k_cache.device
     _req(q.dim() == 3, "q" + _LIKE.format("q_heads"))
@@ -792,6 +803,7 @@ def adapter_add(y, x, a, b, adapters, scales=None, out=None):
     T = _lib.torch_ops()
     if T is not None:
         return T.adapter_add(y, x, a, b, adapters, scales, out)
+    _no_gradient("adapter_add", y=y, x=x, a=a, b=b, scales=scales, out=out)
     _req(x.is_cuda, "x must be on a ROCm GPU")
     dev = x.device
     _req(x.dtype in (torch.float16, torch.bfloat16), "adapters take float16 or bfloat16 activations")

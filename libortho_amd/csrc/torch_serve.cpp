@@ -7,6 +7,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 #include <tuple>
 
@@ -27,6 +28,22 @@ bool given(const Opt &t) { return t.has_value() && t->defined(); }
 int64_t stride_of(const at::Tensor &t, int64_t d);
 
 void *ptr(const at::Tensor &t) { return t.numel() > 0 ? t.data_ptr() : nullptr; }
+
+// None of the operators has a gradient: a tensor that wants one is refused
+// rather than forgotten.
+struct Named {
+    const char *name;
+    const at::Tensor *t;
+};
+Named named(const char *name, const at::Tensor &t) { return {name, &t}; }
+Named named(const char *name, const Opt &t) { return {name, given(t) ? &*t : nullptr}; }
+void no_gradient(const char *op, std::initializer_list<Named> tensors) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Named &n : tensors)
+        if (n.t && n.t->requires_grad())
+            throw std::runtime_error(std::string(op) + " has no gradient: " + n.name +
+                                     " requires one (detach it, or call under torch.no_grad())");
+}
 
 hipStream_t stream_of(const at::Device &dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
 
@@ -133,6 +150,8 @@ page_step(const at::Tensor &lengths, const at::Tensor &new_tokens, const at::Ten
 Opt cache_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cache, const at::Tensor &v_cache,
                  const at::Tensor &slots, const Opt &q, const Opt &positions, const Opt &cos_sin, bool interleaved,
                  const Opt &q_out) {
+    no_gradient("cache_append", {named("k", k), named("v", v), named("k_cache", k_cache), named("v_cache", v_cache),
+                                 named("q", q), named("cos_sin", cos_sin), named("q_out", q_out)});
     const orth_hip_cache_t c = cache_of(k_cache, v_cache);
     const at::Device dev = k_cache.device();
     req(k.dim() == 3, "k must be [tokens, kv_heads, head_dim] of the cache's dtype on its device, vectors contiguous");
@@ -189,6 +208,7 @@ Opt cache_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_c
 at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
                            const at::Tensor &table, const at::Tensor &positions, const Opt &rows,
                            const c10::optional<double> &scale, int64_t window, const Opt &out_) {
+    no_gradient("paged_attention", {named("q", q), named("k_cache", k_cache), named("v_cache", v_cache), named("out", out_)});
     const orth_hip_cache_t c = cache_of(k_cache, v_cache);
     const at::Device dev = k_cache.device();
     req(q.dim() == 3, "q must be [tokens, q_heads, head_dim] of the cache's dtype on its device, vectors contiguous");
@@ -232,6 +252,8 @@ at::Tensor paged_attention(const at::Tensor &q, const at::Tensor &k_cache, const
 
 at::Tensor adapter_add(const at::Tensor &y, const at::Tensor &x, const at::Tensor &a, const at::Tensor &b,
                        const at::Tensor &adapters, const Opt &scales, const Opt &out_) {
+    no_gradient("adapter_add", {named("y", y), named("x", x), named("a", a), named("b", b), named("scales", scales),
+                                named("out", out_)});
     req(x.is_cuda(), "x must be on a ROCm GPU");
     const at::Device dev = x.device();
     orth_hip_adapter_t g{};
