@@ -21,7 +21,11 @@ int guarded(F &&body) noexcept {
         host_begin();
         return body();
     } catch (...) {
-        return ORTH_ERR_HIP;
+        try {
+            return host_fail(ORTH_ERR_HIP, "out of host memory");
+        } catch (...) {
+            return ORTH_ERR_HIP;
+        }
     }
 }
 

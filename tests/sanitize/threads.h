@@ -15,6 +15,7 @@ const hipStream_t kCapturing = reinterpret_cast<hipStream_t>(0x4000);
 // stream, or of any stream, was inside
 extern std::atomic<int> inside[kStreams], overlaps, together, all;
 extern std::atomic<int> kernels;  // launched by the host side itself
+extern std::atomic<bool> throws;      // launchers throw, as an allocation does
 extern std::mutex mu;
 extern std::map<void *, std::set<void *>> works;
 void launch(hipStream_t stream, void *work);

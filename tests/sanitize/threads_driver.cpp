@@ -94,6 +94,13 @@ int main() {
     expect(attend(one) == ORTH_OK && threads::kernels == 0, "eager counters");
     expect(attend(threads::kCapturing) == ORTH_OK && threads::kernels == 1, "captured counters start from zero");
 
+    // an exception ends as a status with a message, and the workspace is free again
+    threads::throws = true;
+    expect(adapter(one) == ORTH_ERR_HIP && orth_hip_last_error()[0] != 0, "an exception under adapter_add");
+    expect(attend(one) == ORTH_ERR_HIP && orth_hip_last_error()[0] != 0, "an exception under paged_attention");
+    threads::throws = false;
+    run({[&] { return adapter(one); }}, "after an exception");
+
     if (failures) return 1;
     std::printf("threads ok\n");
     return 0;

@@ -6,6 +6,7 @@
 
 #include <cstdlib>
 #include <cstring>
+#include <new>
 
 #include "orth_common.h"
 #include "orth_serve.h"
@@ -13,10 +14,12 @@
 
 namespace threads {
 std::atomic<int> inside[kStreams], overlaps{0}, together{0}, all{0}, kernels{0};
+std::atomic<bool> throws{false};
 std::mutex mu;
 std::map<void *, std::set<void *>> works;  // of each thread's tag
 
 void launch(hipStream_t stream, void *work) {
+    if (throws) throw std::bad_alloc();
     const int i = (int)((uintptr_t)stream % kStreams);
     if (inside[i]++ != 0) overlaps++;
     if (all++ != 0) together++;
