@@ -913,7 +913,7 @@ hipError_t up_launch(const AdapterArgs &g, unsigned groups, hipStream_t stream) 
 template <bool BF>
 hipError_t adapter_launch(const AdapterArgs &g, hipStream_t stream) {
     const int64_t padded = g.chunk > 0 ? (int64_t)g.chunk * 8 : g.tiles, parts = (int64_t)g.slices * g.slots;
-    if (padded * (g.blocks > parts ? g.blocks : parts) > INT32_MAX) return hipErrorInvalidConfiguration;
+    if (padded * (g.blocks > parts ? g.blocks : parts) > (int64_t)UINT32_MAX / 512) return hipErrorInvalidConfiguration;
     const unsigned down = (unsigned)(padded * parts), up = (unsigned)(padded * g.blocks);
     if (g.a.count > 0) {
         hipError_t e = g.a.rank <= 16 ? down_launch<1, BF>(g, down, stream)
@@ -924,19 +924,46 @@ hipError_t adapter_launch(const AdapterArgs &g, hipStream_t stream) {
     return g.few ? up_launch<1, BF>(g, up, stream) : up_launch<4, BF>(g, up, stream);
 }
 
+// The tokens of a pair of launches: a launch holds fewer than 2^32 threads (one
+// past that runs another number of workgroups, without an error), which leaves
+// room for 2^5 workgroups a 64-token tile, or for outputs of 512 GB.
+constexpr int64_t kLaunchTokens = 1 << 24;
+
+// Tokens t .. of a call, as a call of their own.
+orth_hip_adapter_t adapter_part(const orth_hip_adapter_t &a, int64_t t) {
+    orth_hip_adapter_t p = a;
+    p.x = (const uint16_t *)a.x + t * a.x_stride;
+    p.y = (const uint16_t *)a.y + t * a.y_stride;
+    p.out = (uint16_t *)a.out + t * a.out_stride;
+    p.adapters = a.adapters + t;
+    p.tokens = a.tokens - t < kLaunchTokens ? a.tokens - t : kLaunchTokens;
+    return p;
+}
+
 }  // namespace
 
 int64_t adapter_workspace_bytes(const orth_hip_adapter_t &a, int cus) {
     if (a.count == 0) return 0;
-    const AdapterArgs g = adapter_args(a, cus);
-    return (int64_t)g.slices * a.tokens * a.rank * 4 + (g.order_by == ORDER_GROUP ? a.tokens * 4 : 0);
+    int64_t most = 0;
+    const int64_t last = (a.tokens - 1) / kLaunchTokens * kLaunchTokens;
+    for (int64_t t = 0; t <= last; t += last > 0 ? last : 1) {  // (all parts but the last are alike)
+        const orth_hip_adapter_t p = adapter_part(a, t);
+        const AdapterArgs g = adapter_args(p, cus);
+        const int64_t bytes = (int64_t)g.slices * p.tokens * p.rank * 4 + (g.order_by == ORDER_GROUP ? p.tokens * 4 : 0);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 hipError_t launch_adapter_add(const orth_hip_adapter_t &a, int cus, void *work, hipStream_t stream) {
-    AdapterArgs g = adapter_args(a, cus);
-    g.low = static_cast<float *>(work);
-    if (g.order_by == ORDER_GROUP) g.order = reinterpret_cast<int *>(g.low + (int64_t)g.slices * a.tokens * a.rank);
-    return a.dtype == ORTH_DT_BF16 ? adapter_launch<true>(g, stream) : adapter_launch<false>(g, stream);
+    for (int64_t t = 0; t < a.tokens; t += kLaunchTokens) {
+        AdapterArgs g = adapter_args(adapter_part(a, t), cus);
+        g.low = static_cast<float *>(work);
+        if (g.order_by == ORDER_GROUP) g.order = reinterpret_cast<int *>(g.low + (int64_t)g.slices * g.a.tokens * g.a.rank);
+        const hipError_t e = a.dtype == ORTH_DT_BF16 ? adapter_launch<true>(g, stream) : adapter_launch<false>(g, stream);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace orth

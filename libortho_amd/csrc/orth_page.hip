@@ -336,12 +336,27 @@ hipError_t launch_cache_append(const orth_hip_cache_t &c, const orth_hip_append_
     // a workgroup for every head group where tokens alone leave CUs idle,
     // else one a token
     const int parts = (heads + g.lanes - 1) / g.lanes;
-    const int y = a.tokens >= 2 * cus ? 1 : parts;
-    const dim3 grid((unsigned)a.tokens, (unsigned)y);
-    if (V == 8) append_launch<8>(g, grid, stream);
-    else if (V == 4) append_launch<4>(g, grid, stream);
-    else append_launch<1>(g, grid, stream);
-    return hipGetLastError();
+    const int y = a.tokens >= 2 * cus ? 1 : parts < 65535 ? parts : 65535;
+    // (a launch holds fewer than 2^32 threads along x: one past that runs
+    // another number of workgroups, without an error)
+    constexpr int64_t kLaunch = 1 << 23;
+    for (int64_t t = 0; t < a.tokens; t += kLaunch) {
+        const dim3 grid((unsigned)(a.tokens - t < kLaunch ? a.tokens - t : kLaunch), (unsigned)y);
+        if (V == 8) append_launch<8>(g, grid, stream);
+        else if (V == 4) append_launch<4>(g, grid, stream);
+        else append_launch<1>(g, grid, stream);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        if (a.q) {
+            g.a.q = (const uint16_t *)g.a.q + kLaunch * a.q_strides[0];
+            g.a.q_out = (uint16_t *)g.a.q_out + kLaunch * a.q_out_strides[0];
+        }
+        g.a.k = (const uint16_t *)g.a.k + kLaunch * a.k_strides[0];
+        g.a.v = (const uint16_t *)g.a.v + kLaunch * a.v_strides[0];
+        g.a.slots += kLaunch;
+        if (a.cos_sin) g.a.positions += kLaunch;
+    }
+    return hipSuccess;
 }
 
 }  // namespace orth

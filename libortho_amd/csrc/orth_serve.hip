@@ -121,6 +121,8 @@ int orth_cache_append_hip(const orth_hip_cache_t *c, const orth_hip_append_t *a,
             return invalid("q is given without cos_sin");
         }
         if (a->q && a->q_heads < 1) return invalid("q_heads must be positive");
+        if ((int64_t)(a->q ? a->q_heads : 0) + 2 * (int64_t)c->kv_heads > (1 << 30))
+            return host_fail(ORTH_ERR_UNSUPPORTED, "q_heads + 2 * kv_heads passes 2^30");
         if (a->tokens > 0 && (!a->k || !a->v || !a->slots)) return invalid("k, v or slots is NULL");
         if (a->tokens > 0 && a->q && !a->q_out) return invalid("q_out is NULL");
         if (!aligned(a->q, 2) || !aligned(a->k, 2) || !aligned(a->v, 2) || !aligned(a->q_out, 2))
