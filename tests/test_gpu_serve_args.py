@@ -107,3 +107,12 @@ def test_adapters_of_more_tokens_than_one_grid_holds(gpu):
         assert got[t].tolist() == [8.0 * (1 + t % 2)] * N, t
         got[t] = 0
     assert not bool(got.any())
+
+
+def test_what_a_server_keeps_between_steps_does_not_hold_the_step(gpu):
+    n, T = 2, 70000
+    z = torch.zeros(n, dtype=torch.int32, device="cuda")
+    lengths, pool, *_ = _C_ops.page_step(z, i32([T - 1, 1]), torch.zeros(n, 5000, dtype=torch.int32, device="cuda"),
+                                         torch.arange(8000, dtype=torch.int32, device="cuda"), i32([0, 0]), 16, T)
+    assert lengths.tolist() == [T - 1, 1] and pool.tolist() == [-(-(T - 1) // 16) + 1, 0]
+    assert lengths.untyped_storage().nbytes() <= 64 and pool.untyped_storage().nbytes() <= 64
