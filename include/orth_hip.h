@@ -419,8 +419,9 @@ int orth_cache_append_hip(const orth_hip_cache_t *cache, const orth_hip_append_t
  * token whose position is negative or whose row lies outside the table gets
  * zeros; keys past the table's width or in a page outside [0, pages) are not
  * seen (a token that sees no key gets zeros).  table_width * page_size is at
- * most 2^31 - 512.  Softmax statistics and sums are FP32; nothing the mask
- * hides reaches the result, whatever it holds. */
+ * most 2^31 - 512.  Softmax statistics and sums are FP32 (scores are to stay
+ * below 2^127, sums of weights times BF16 values below 2^144); nothing the
+ * mask hides reaches the result, whatever it holds. */
 typedef struct {
     const void *q;               /* [tokens, q_heads, head_dim], the cache's dtype */
     void *out;

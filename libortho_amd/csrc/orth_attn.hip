@@ -23,7 +23,9 @@
 // The weights enter the second product as FP32 values do: as 16-bit parts,
 // three in BF16 and two in FP16 (split_pair), whose products with the values
 // are exact and add up in FP32.  FP16 ones are held 2^14 times larger, which
-// keeps the parts of small weights normal numbers.
+// keeps the parts of small weights normal numbers, BF16 ones 2^16 times
+// smaller: sums of 2^16 of the type's largest numbers do not overflow before
+// they are divided by l, and products with its smallest are numbers of FP32.
 //
 // Bound by reading the cache once.  The work is cut evenly over the resident
 // workgroups by the keys the tokens really see, which only the device knows:
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
     constexpr int EL = KS <= 2 ? 4 : KS <= 4 ? 8 : 16;  // elements of a value vector per lane
     constexpr int VW = EL / 2;                          // words of them
     constexpr bool VTAIL = TAIL || 16 * EL != 32 * KS;
-    constexpr float kShift = BF ? 0.f : 14.f;
+    constexpr float kHeld = BF ? 0x1p-16f : 0x1p14f;  // (multiplied, not added to the exponent, which would lose its low bits)
     // o [waves][gt][16 EL + 4], then (m, l) [waves][16]; both start at 16 bytes, and so does each row of o
     extern __shared__ __align__(16) float lds[];
     static_assert((16 * EL + 4) % 4 == 0, "rows of o");
@@ -460,11 +462,10 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
                         for (int i = 0; i < 4; i++) o[e][i] *= keep;
                     m = top;
                 }
-                const float base = m - kShift;
                 u32x4 p[kParts<BF>];
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(x[i] - base), p1 = __builtin_amdgcn_exp2f(x[i + 1] - base);
+                    const float p0 = kHeld * __builtin_amdgcn_exp2f(x[i] - m), p1 = kHeld * __builtin_amdgcn_exp2f(x[i + 1] - m);
                     l += p0 + p1;
                     uint32_t part[kParts<BF>];
                     split_pair<BF>(p0, p1, part);

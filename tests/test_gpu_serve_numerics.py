@@ -159,3 +159,21 @@ def test_adapters_of_infinite_weights(gpu, M, r, N, dtype):
     got = _C_ops.adapter_add(y, x2, a2, b2, ids)
     of = (ids == 1).nonzero().flatten()
     assert bool((got[of] == INF).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", [1, 64, 40000])
+def test_attention_of_the_types_largest_and_smallest_values(gpu, n, dtype):
+    # equal weights over equal values: the value, however many
+    dt, P, D = DT[dtype], 16, 64
+    pages = -(-n // P)
+    kc = torch.zeros(pages, P, 1, D, dtype=dt, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    q = torch.ones(1, 3, D, dtype=dt, device="cuda")
+    for v in (torch.finfo(dt).max, torch.finfo(dt).min):
+        got = _C_ops.paged_attention(q, kc, torch.full_like(kc, v), table, i32([n - 1]))
+        assert bool((got == v).all()), (v, float(got[0, 0, 0]))
+    least = 4 * TINY[dt]  # two of the smallest steps
+    got = _C_ops.paged_attention(q, kc, torch.full_like(kc, least), table, i32([n - 1])).double()
+    # (FP32 steps of 2^-149 a key in BF16: with the weights' 2^16 half a step of the type)
+    assert bool(((got - least).abs() <= 2 * TINY[dt]).all())
