@@ -7,8 +7,8 @@
 //   down  low[m, j] = sum_k x[m, k] A_i[j, k]
 //   up    out[m, n] = y[m, n] + sum_j (scale_i low[m, j]) B_i[n, j]
 //
-// Both go through v_mfma_f32_16x16x32 with 16 consecutive tokens as the
-// columns: x, A and B enter by 16-byte loads as they lie; products are exact,
+// Both go through v_mfma_f32_16x16x32 with 16 tokens as the columns
+// (consecutive ones, or neighbours in their adapters' order: Order): x, A and B enter by 16-byte loads as they lie; products are exact,
 // sums FP32.  For every adapter among the 16 tokens (found by ballots) the
 // product is formed for all columns and kept in those of its own tokens: a
 // run of one prompt's tokens is one product, a decode batch of 16 requests
@@ -25,10 +25,12 @@
 // Measured (one MI355X, a call among others): one token, 4096 -> 4096, rank
 // 16, FP16: 8.9 us, two chains of latencies (number, weights, join; number,
 // partials, store); 48 tokens of 24 adapters, 4096 -> 11008, rank 32, BF16:
-// 16.4 us (23.7 MB, 1.5 TB/s; down 6, up 10.5); 2,048 tokens in five runs,
-// 11008 -> 4096, rank 64, FP16: 37.3 us (86 MB, 2.3 TB/s; down 19, up 19: the
-// partials' round trip and the launches' starts and ends, with one round of
-// workgroups each).  A wave per low-rank value and a thread per output took
+// 16.2 us (23.7 MB, 1.5 TB/s; down 6, up 10.5); 2,048 tokens in five runs,
+// 11008 -> 4096, rank 64, FP16: 37.5 us (86 MB, 2.3 TB/s; down 19, up 19: the
+// partials, which each of the second launch's output blocks adds up again, and
+// the launches' starts and ends, with one round of workgroups each).  HBM reads
+// by counter: 6.3 MB (A is 6.3) and 17.9 (B and y 17.9) at 48 tokens, 62.6 (x
+// and A 52) and 27.4 (B and y 19.4, partials 4) at 2,048.  A wave per low-rank value and a thread per output took
 // 12, 57 and 2,500 us.
 #include <type_traits>
 
@@ -269,9 +271,10 @@ __device__ __forceinline__ void down_one(const AdapterArgs &g, int m, int id, ui
 // adapter in turn, the products kept in their own tokens' columns.
 template <int RB, bool BF, int W>
 __device__ __forceinline__ void down_all(const AdapterArgs &g, int64_t m0, int rank0, int slice, float *lds) {
-    // adapters whose loads are in flight together (with eight, and two in the
-    // up launch, 538 tokens of 24 adapters in turn, 4000 -> 11008, rank 16,
-    // take 82 us; with four and one 91)
+    // adapters whose loads are in flight together (538 tokens of 24 adapters
+    // in turn, 4000 -> 11008, rank 16, BF16, low-rank values in two parts: with
+    // eight, and two in the up launch, 82 us, with four and one 91; with the
+    // three parts of now 87)
     constexpr int IDS = RB == 1 ? 8 : 2;
     const int lane = threadIdx.x & 63, col = lane & 15, lg = lane >> 4;
     const int64_t K = g.a.in_features;

@@ -29,18 +29,22 @@
 //
 // Bound by reading the cache once.  The work is cut evenly over the resident
 // workgroups by the keys the tokens really see, which only the device knows:
-// every wave sums up the tokens' units of 256 keys and finds its workgroup's
-// share (of some 100 tokens in one load and one scan).  A share that ends
+// every wave sums up the tokens' units (two tiles for each wave that shares a
+// head tile: 64, 128 or 256 keys) and finds its workgroup's share (of 128
+// tokens in one load and one scan).  A share that ends
 // inside a (token, key head) leaves a piece (m, l, o); the workgroup that
 // writes an item's last piece joins them, or a second launch where an item
 // has many.  Whole items are written at once.
 //
 // Measured (one MI355X, a call among others, inputs from HBM): 128 requests
-// of 2,048 to 16,384 keys, 8 of 64 heads of 128, BF16: 590 us, 5.7 TB/s of
-// keys and values; 32 ragged requests up to 4,096 keys, 32 heads, FP16: 73.6
-// us, 4.6 TB/s; one of 32,768 keys, 8 of 32 heads: 37.1 us (32 the keys, 5
-// the join of 64 pieces a key head), 3.6 TB/s; one of 190 keys, 32 heads: 9.2 us,
-// a chain of latencies (position 1.2, share 0.7, table 1.6, keys 2, join 1).
+// of 2,048 to 16,384 keys, 8 of 64 heads of 128, BF16: 594 us, 5.6 TB/s (a
+// kernel that only reads reaches 5.7); 32 ragged requests up to 4,096 keys, 32
+// heads, FP16: 73.8 us, 4.6 TB/s; one of 32,768 keys, 8 of 32 heads: 37.3 us
+// (32 the keys, 5 the join of 64 pieces a key head), 3.6 TB/s; one of 190
+// keys, 32 heads: 8.9 us, a chain of latencies (position 1.2, share 0.7, table
+// 1.6, keys 2, join 1).  HBM reads by counter: 3.37 GB, 344 MB and 135 MB for
+// the first three, as their keys and values.  Several tokens of one request
+// read its keys each for itself (2,048 tokens of one prompt: 853 us).
 // A wave per query head on the vector unit (no matrix products, no split)
 // took 35,500, 7,900, 57,500 and 164 us.
 #include "orth_serve.h"
@@ -115,8 +119,9 @@ __device__ __forceinline__ Keys keys_of(const AttendArgs &g, int64_t t) {
 }
 
 // Inclusive sums of the units of tokens t0 + 2 lane, + 1, whose keys are in k[2].  (32 bits
-// hold them: a token has at most 2^24 units of four tiles, or of one tile
-// where the launch has seen that its table holds no more than 2^28 keys.)
+// hold them: a token has at most 2^23 units of 256 keys, or 2^22 of 64 where
+// the launch has seen that its table holds no more than 2^28 keys, and a scan
+// takes 128 tokens.)
 constexpr int kScan = 128;
 __device__ __forceinline__ uint32_t block_units(const AttendArgs &g, int64_t t0, int lane, Keys k[2]) {
 #pragma unroll

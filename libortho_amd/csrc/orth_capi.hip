@@ -296,9 +296,8 @@ int current_device_ok(int *dev_out) {
 // scratch array), else the call is refused.  Eager calls never touch either,
 // so a graph replayed on any stream, beside eager calls on any stream, does
 // not race with them; replays of graphs that overlap one another, calls on
-// parallel branches of one graph, or
-// no-allocation calls, on the same GPU share that memory and must be
-// ordered by the caller.
+// parallel branches of one graph, or no-allocation calls, on the same GPU
+// share that memory and must be ordered by the caller.
 struct Workspace {
     std::mutex mu;  // held by a call (Held); in front of g_ws_mu where both are
     void *buf = nullptr;
