@@ -441,6 +441,74 @@ typedef struct {
 } orth_hip_attend_t;
 int orth_paged_attention_hip(const orth_hip_cache_t *cache, const orth_hip_attend_t *attend, void *stream);
 
+/* The same cache held in 4 bits.  A vector of head_dim elements (a multiple of
+ * 8, at most 256) is cut into groups of group_size: head_dim itself, or 32, 64
+ * or 128 where that divides it.  A group is a pair of FP16 numbers (scale,
+ * low) and a code u = 0 .. 15 an element; it stands for low + u * scale.
+ * Codes: a row of 16 units of W bytes, W = 2, 3, 4 or 8, the least with 32 W
+ * >= head_dim (ORTH_INT4_ROW_BYTES); byte b of unit r holds element 32 b + r
+ * in its low nibble and 32 b + 16 + r in its high one (elements past head_dim:
+ * zeros are written, anything may be read).  A unit is what a lane of the
+ * attention's matrix products takes of a vector.  Slot s of page p, head h has
+ * its codes at p * code_strides[0] + s * code_strides[1] + h * code_strides[2]
+ * bytes and its head_dim / group_size pairs, contiguous, at so many FP16
+ * elements by scale_strides.  Codes are 16-byte aligned with strides that are
+ * multiples of 16, pairs 4-byte aligned with even strides.
+ *
+ * A group is quantised from FP16 values x (BF16 ones and turned keys are
+ * rounded to FP16, what passes +-65504 saturates): low = min x, scale =
+ * (max x - min x) / 15 rounded to FP16 (the next number below where low + 15 *
+ * scale would pass 65504), u = (x - low) / scale to the nearest, halves up; a
+ * scale of 0 has codes 0.  A group with an element that is not finite is held
+ * as NaN (scale and low NaN). */
+#define ORTH_INT4_ROW_BYTES(head_dim) \
+    ((head_dim) <= 64 ? 32 : (head_dim) <= 96 ? 48 : (head_dim) <= 128 ? 64 : 128)
+typedef struct {
+    void *k_codes;
+    void *v_codes;
+    void *k_scales;
+    void *v_scales;
+    int32_t page_size;           /* >= 1 */
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t group_size;
+    int64_t pages;
+    int64_t k_code_strides[3];   /* page, slot, head: bytes */
+    int64_t v_code_strides[3];
+    int64_t k_scale_strides[3];  /* page, slot, head: FP16 elements */
+    int64_t v_scale_strides[3];
+} orth_hip_int4_cache_t;
+
+/* orth_cache_append_hip for that cache; q, k, v and q_out hold `dtype`
+ * (ORTH_DT_F16 or ORTH_DT_BF16).  q is turned as there; k is turned in 64 bits
+ * and rounded to FP16 once (a last place may move a code).  Two tokens with
+ * one slot leave a mixture of both there. */
+int orth_cache_append_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_append_t *append, int32_t dtype,
+                               void *stream);
+
+/* The vectors of `count` slots, low + u * scale in FP32 rounded to `dtype`:
+ * k_out[i, h] and v_out[i, h] from slot slots[i], zeros where it lies outside
+ * the cache.  Strides are [slot, head] of the outputs, 16-byte aligned
+ * pointers with strides that are multiples of 8 or any others. */
+typedef struct {
+    void *k_out;                 /* [count, kv_heads, head_dim] */
+    void *v_out;
+    int64_t k_strides[2];
+    int64_t v_strides[2];
+    const int64_t *slots;        /* [count] */
+    int64_t count;
+} orth_hip_read_t;
+int orth_cache_read_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_read_t *read, int32_t dtype, void *stream);
+
+/* orth_paged_attention_hip over that cache, with the values low + u * scale as
+ * keys and values; q and out hold `dtype`.  Queries enter in FP16 with a power
+ * of two of their own vector (elements below 2^-39 of its largest lose bits).
+ * The NaN of a group of a key in sight reaches its tokens' outputs, that of a
+ * value the group's elements; a query with an element that is not finite gives
+ * NaN. */
+int orth_paged_attention_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_attend_t *attend, int32_t dtype,
+                                  void *stream);
+
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[m] = y[m] + scales[i] * (x[m] a[i]^T) b[i]^T,  i = adapters[m]
  * (out[m] = y[m] where i lies outside [0, count)); a[i] is [rank,

@@ -45,7 +45,7 @@ _DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: 
 __all__ = ["forward", "forward_planned", "forward_group", "build_plan", "dequant", "pack_base", "pack_csr", "sieve_quantize",
            "sieve_split", "sieve_hdiag", "last_kernel", "last_variant", "set_kernel_policy", "get_kernel_policy", "device_info",
            "plan_cache_clear", "plan_cache_limit", "plan_cache_info", "page_step", "cache_append", "paged_attention",
-           "adapter_add"]
+           "adapter_add", "int4_cache", "cache_append_int4", "cache_read_int4", "paged_attention_int4"]
 
 
 def _req(cond: bool, msg: str) -> None:
@@ -630,12 +630,14 @@ def _cache(k: torch.Tensor, v: torch.Tensor) -> _lib.OrthHipCache:
                              v_strides=tuple(_stride(v, d) for d in range(3)))
 
 
-def _vectors(t: torch.Tensor, cache: torch.Tensor, tokens: int, msg: str) -> None:
-    _req(t.device == cache.device and t.dtype == cache.dtype and t.dim() == 3 and t.shape[0] == tokens and
-         t.shape[2] == cache.shape[3] and (t.numel() == 0 or t.stride(2) == 1), msg)
+def _vectors(t: torch.Tensor, like, tokens: int, msg: str) -> None:
+    dev, dtype, head_dim = like
+    _req(t.device == dev and t.dtype == dtype and t.dim() == 3 and t.shape[0] == tokens and t.shape[2] == head_dim and
+         (t.numel() == 0 or t.stride(2) == 1), msg)
 
 
 _LIKE = " must be [tokens, {}, head_dim] of the cache's dtype on its device, vectors contiguous"
+_LIKE4 = " must be [tokens, {}, head_dim] of one 16-bit dtype on the cache's device, vectors contiguous"
 _TABLE = "block_table must be int32 [requests, pages] with contiguous rows that do not overlap"
 
 
@@ -644,6 +646,67 @@ def _table(t: torch.Tensor, dev, rows=None) -> int:
     _req(t.device == dev and t.dtype == torch.int32 and t.dim() == 2 and (rows is None or t.shape[0] == rows) and
          (t.numel() == 0 or (t.stride(1) == 1 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1]))), _TABLE)
     return int(t.shape[1] if t.shape[0] < 2 or t.numel() == 0 else t.stride(0))
+
+
+def _append_args(k, v, like, kv_heads, slots, q, positions, cos_sin, interleaved, q_out, text):
+    """The checked arguments of an append, q_out, and what must outlive the call."""
+    dev, _, head_dim = like
+    _req(k.dim() == 3, "k" + text.format("kv_heads"))
+    n = int(k.shape[0])
+    _vectors(k, like, n, "k" + text.format("kv_heads"))
+    _vectors(v, like, n, "v" + text.format("kv_heads"))
+    _req(k.shape[1] == kv_heads and v.shape[1] == kv_heads, "k and v must have the cache's kv_heads")
+    _index(slots, dev, n, torch.int64, "slots must be a contiguous int64 vector of tokens")
+    _req(cos_sin is not None or q is None, "q needs cos_sin")
+    _req(q_out is None or q is not None, "q_out needs q")
+    a = _lib.OrthHipAppend(k=_ptr(k), v=_ptr(v), k_strides=(_stride(k, 0), _stride(k, 1)),
+                           v_strides=(_stride(v, 0), _stride(v, 1)), slots=_ptr(slots), tokens=n,
+                           interleaved=int(bool(interleaved)))
+    none = ctypes.c_float()  # an empty table still turns the call: no position lies inside it
+    if cos_sin is not None:
+        _req(positions is not None, "cos_sin needs positions")
+        _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
+        _req(cos_sin.device == dev and cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
+             "cos_sin must be a contiguous float32 [positions, rot]")
+        _req(cos_sin.shape[1] % 2 == 0 and cos_sin.shape[1] <= head_dim, "rot must be even and at most head_dim")
+        a.positions = _ptr(positions)
+        a.cos_sin = _ptr(cos_sin) or ctypes.addressof(none)
+        a.cos_sin_rows, a.rot = cos_sin.shape
+    if q is not None:
+        _vectors(q, like, n, "q" + text.format("q_heads"))
+        _req(1 <= q.shape[1] < 1 << 31, "q must have heads")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _vectors(q_out, like, n, "q_out must be like q")
+        _req(q_out.shape[1] == q.shape[1], "q_out must be like q")
+        a.q, a.q_out, a.q_heads = _ptr(q), _ptr(q_out), q.shape[1]
+        a.q_strides, a.q_out_strides = (_stride(q, 0), _stride(q, 1)), (_stride(q_out, 0), _stride(q_out, 1))
+    return a, q_out, none
+
+
+def _attend_args(q, like, kv_heads, block_table, positions, rows, scale, window, out, text):
+    """The checked arguments of an attention, and its output."""
+    dev, _, head_dim = like
+    _req(q.dim() == 3, "q" + text.format("q_heads"))
+    n = int(q.shape[0])
+    _vectors(q, like, n, "q" + text.format("q_heads"))
+    _req(kv_heads > 0 and 0 < q.shape[1] < 1 << 31 and q.shape[1] % kv_heads == 0, "q_heads must be a multiple of kv_heads")
+    stride = _table(block_table, dev)
+    _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
+    if rows is not None:
+        _index(rows, dev, n, torch.int32, "rows must be a contiguous int32 vector of tokens")
+    _req(0 <= window < 1 << 31, "window must not be negative")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _vectors(out, like, n, "out must be like q")
+    _req(out.shape[1] == q.shape[1], "out must be like q")
+    a = _lib.OrthHipAttend(q=_ptr(q), out=_ptr(out), q_strides=(_stride(q, 0), _stride(q, 1)),
+                           out_strides=(_stride(out, 0), _stride(out, 1)), block_table=_ptr(block_table),
+                           positions=_ptr(positions), rows=None if rows is None else _ptr(rows),
+                           table_rows=block_table.shape[0], table_width=block_table.shape[1], table_stride=stride,
+                           tokens=n, q_heads=q.shape[1], window=window,
+                           scale=float(scale) if scale is not None else head_dim ** -0.5)
+    return a, out
 
 
 def page_step(lengths, new_tokens, block_table, free_pages, pool, page_size, tokens):
@@ -712,36 +775,8 @@ def cache_append(k, v, k_cache, v_cache, slots, q=None, positions=None, cos_sin=
     _no_gradient("cache_append", k=k, v=v, k_cache=k_cache, v_cache=v_cache, q=q, cos_sin=cos_sin, q_out=q_out)
     c = _cache(k_cache, v_cache)
     dev = k_cache.device
-    _req(k.dim() == 3, "k" + _LIKE.format("kv_heads"))
-    n = int(k.shape[0])
-    _vectors(k, k_cache, n, "k" + _LIKE.format("kv_heads"))
-    _vectors(v, k_cache, n, "v" + _LIKE.format("kv_heads"))
-    _req(k.shape[1] == c.kv_heads and v.shape[1] == c.kv_heads, "k and v must have the cache's kv_heads")
-    _index(slots, dev, n, torch.int64, "slots must be a contiguous int64 vector of tokens")
-    _req(cos_sin is not None or q is None, "q needs cos_sin")
-    _req(q_out is None or q is not None, "q_out needs q")
-    a = _lib.OrthHipAppend(k=_ptr(k), v=_ptr(v), k_strides=(_stride(k, 0), _stride(k, 1)),
-                           v_strides=(_stride(v, 0), _stride(v, 1)), slots=_ptr(slots), tokens=n,
-                           interleaved=int(bool(interleaved)))
-    none = ctypes.c_float()  # an empty table still turns the call: no position lies inside it
-    if cos_sin is not None:
-        _req(positions is not None, "cos_sin needs positions")
-        _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
-        _req(cos_sin.device == dev and cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
-             "cos_sin must be a contiguous float32 [positions, rot]")
-        _req(cos_sin.shape[1] % 2 == 0 and cos_sin.shape[1] <= c.head_dim, "rot must be even and at most head_dim")
-        a.positions = _ptr(positions)
-        a.cos_sin = _ptr(cos_sin) or ctypes.addressof(none)
-        a.cos_sin_rows, a.rot = cos_sin.shape
-    if q is not None:
-        _vectors(q, k_cache, n, "q" + _LIKE.format("q_heads"))
-        _req(1 <= q.shape[1] < 1 << 31, "q must have heads")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        _vectors(q_out, k_cache, n, "q_out must be like q")
-        _req(q_out.shape[1] == q.shape[1], "q_out must be like q")
-        a.q, a.q_out, a.q_heads = _ptr(q), _ptr(q_out), q.shape[1]
-        a.q_strides, a.q_out_strides = (_stride(q, 0), _stride(q, 1)), (_stride(q_out, 0), _stride(q_out, 1))
+    a, q_out, _kept = _append_args(k, v, (dev, k_cache.dtype, c.head_dim), c.kv_heads, slots, q, positions, cos_sin,
+                                    interleaved, q_out, _LIKE)
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().orth_cache_append_hip(ctypes.byref(c), ctypes.byref(a), _stream(dev)))
     return q_out
@@ -766,28 +801,120 @@ def paged_attention(q, k_cache, v_cache, block_table, positions, rows=None, scal
     _no_gradient("paged_attention", q=q, k_cache=k_cache, v_cache=v_cache, out=out)
     c = _cache(k_cache, v_cache)
     dev = k_cache.device
-    _req(q.dim() == 3, "q" + _LIKE.format("q_heads"))
-    n = int(q.shape[0])
-    _vectors(q, k_cache, n, "q" + _LIKE.format("q_heads"))
-    _req(c.kv_heads > 0 and 0 < q.shape[1] < 1 << 31 and q.shape[1] % c.kv_heads == 0,
-         "q_heads must be a multiple of kv_heads")
-    stride = _table(block_table, dev)
-    _index(positions, dev, n, torch.int32, "positions must be a contiguous int32 vector of tokens")
-    if rows is not None:
-        _index(rows, dev, n, torch.int32, "rows must be a contiguous int32 vector of tokens")
-    _req(0 <= window < 1 << 31, "window must not be negative")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _vectors(out, k_cache, n, "out must be like q")
-    _req(out.shape[1] == q.shape[1], "out must be like q")
-    a = _lib.OrthHipAttend(q=_ptr(q), out=_ptr(out), q_strides=(_stride(q, 0), _stride(q, 1)),
-                           out_strides=(_stride(out, 0), _stride(out, 1)), block_table=_ptr(block_table),
-                           positions=_ptr(positions), rows=None if rows is None else _ptr(rows),
-                           table_rows=block_table.shape[0], table_width=block_table.shape[1], table_stride=stride,
-                           tokens=n, q_heads=q.shape[1], window=window,
-                           scale=float(scale) if scale is not None else k_cache.shape[3] ** -0.5)
+    a, out = _attend_args(q, (dev, k_cache.dtype, c.head_dim), c.kv_heads, block_table, positions, rows, scale, window, out,
+                          _LIKE)
     with torch.cuda.device(dev):
         _lib.check(_lib.lib().orth_paged_attention_hip(ctypes.byref(c), ctypes.byref(a), _stream(dev)))
+    return out
+
+
+def int4_cache(pages, page_size, kv_heads, head_dim, group_size=None, device="cuda"):
+    """An empty cache of 4-bit keys and values, ``(k_codes, k_scales, v_codes,
+    v_scales)``: codes uint8 [pages, page_size, kv_heads, row bytes] and, for
+    every ``group_size`` elements of a vector, FP16 (scale, low) [pages,
+    page_size, kv_heads, groups, 2]; code u stands for low + u * scale.
+    ``group_size`` is ``head_dim``, or 32, 64 or 128 where that divides it
+    (None: 64 if it does, else ``head_dim``)."""
+    group_size = group_size if group_size is not None else 64 if head_dim % 64 == 0 else head_dim
+    _req(group_size > 0 and head_dim % group_size == 0, "group_size must divide head_dim")
+    codes = (pages, page_size, kv_heads, _int4_row_bytes(head_dim))
+    scales = (pages, page_size, kv_heads, head_dim // group_size, 2)
+    return tuple(torch.zeros(shape, dtype=dtype, device=device)
+                 for _ in "kv" for shape, dtype in ((codes, torch.uint8), (scales, torch.float16)))
+
+
+def _int4_row_bytes(head_dim: int) -> int:
+    return 32 if head_dim <= 64 else 48 if head_dim <= 96 else 64 if head_dim <= 128 else 128
+
+
+def _cache4(k_codes, k_scales, v_codes, v_scales, head_dim: int) -> _lib.OrthHipInt4Cache:
+    dev = k_codes.device
+    _req(k_codes.is_cuda and all(t.device == dev for t in (k_scales, v_codes, v_scales)),
+         "the cache's codes and scales must be on one ROCm GPU")
+    _req(8 <= head_dim <= 256 and head_dim % 8 == 0, "head_dim must be a multiple of 8, at most 256")
+    _req(all(t.dtype == torch.uint8 and t.dim() == 4 and t.shape[3] == _int4_row_bytes(head_dim) and t.stride(3) == 1
+             for t in (k_codes, v_codes)) and v_codes.shape == k_codes.shape,
+         "codes must be uint8 [pages, page_size, kv_heads, row bytes] as int4_cache gives them, rows contiguous")
+    _req(all(t.dtype == torch.float16 and t.dim() == 5 and t.shape[:3] == k_codes.shape[:3] and t.shape[3] >= 1 and
+             t.shape[4] == 2 and t.stride(4) == 1 and (t.shape[3] == 1 or t.stride(3) == 2) for t in (k_scales, v_scales)) and
+         v_scales.shape == k_scales.shape and head_dim % k_scales.shape[3] == 0,
+         "scales must be float16 [pages, page_size, kv_heads, groups, 2] as int4_cache gives them, pairs contiguous")
+    _req(k_codes.shape[1] < 1 << 31 and k_codes.shape[2] < 1 << 31, "the cache's page_size or kv_heads is too large")
+    return _lib.OrthHipInt4Cache(_ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), k_codes.shape[1],
+                                 k_codes.shape[2], head_dim, head_dim // k_scales.shape[3], k_codes.shape[0],
+                                 *(tuple(_stride(t, d) for d in range(3)) for t in (k_codes, v_codes, k_scales, v_scales)))
+
+
+def _dtype16(t: torch.Tensor, name: str) -> int:
+    _req(t.dtype in (torch.float16, torch.bfloat16), f"{name} must be float16 or bfloat16")
+    return _DT[t.dtype]
+
+
+def cache_append_int4(k, v, k_codes, k_scales, v_codes, v_scales, slots, q=None, positions=None, cos_sin=None,
+                      interleaved=False, q_out=None):
+    """:func:`cache_append` into a cache of :func:`int4_cache`: k, turned like
+    q, and v are quantised as they are written (float16 or bfloat16; elements
+    past +-65504 saturate, a group with one that is not finite is held as
+    NaN).  q comes back in its own type.  Two tokens with one slot leave a
+    mixture of both there."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.cache_append_int4(k, v, k_codes, k_scales, v_codes, v_scales, slots, q, positions, cos_sin, interleaved, q_out)
+    _no_gradient("cache_append_int4", k=k, v=v, k_scales=k_scales, v_scales=v_scales, q=q, cos_sin=cos_sin, q_out=q_out)
+    _req(k.dim() == 3, "k" + _LIKE4.format("kv_heads"))
+    c = _cache4(k_codes, k_scales, v_codes, v_scales, int(k.shape[2]))
+    dev, dtype = k_codes.device, _dtype16(k, "k")
+    a, q_out, _kept = _append_args(k, v, (dev, k.dtype, c.head_dim), c.kv_heads, slots, q, positions, cos_sin,
+                                   interleaved, q_out, _LIKE4)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_cache_append_int4_hip(ctypes.byref(c), ctypes.byref(a), dtype, _stream(dev)))
+    return q_out
+
+
+def cache_read_int4(k_codes, k_scales, v_codes, v_scales, slots, head_dim, dtype=torch.float16, k_out=None, v_out=None):
+    """The keys and values of ``slots`` (int64 [n]) of a cache of
+    :func:`int4_cache`, low + u * scale rounded once to ``dtype`` (float16 or
+    bfloat16): two tensors [n, kv_heads, head_dim], new ones or ``k_out`` and
+    ``v_out``.  A slot that is negative or past the cache reads as zeros."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.cache_read_int4(k_codes, k_scales, v_codes, v_scales, slots, head_dim, dtype, k_out, v_out)
+    _no_gradient("cache_read_int4", k_scales=k_scales, v_scales=v_scales, k_out=k_out, v_out=v_out)
+    c = _cache4(k_codes, k_scales, v_codes, v_scales, int(head_dim))
+    dev = k_codes.device
+    _index(slots, dev, None, torch.int64, "slots must be a contiguous int64 vector")
+    _req(dtype in (torch.float16, torch.bfloat16), "dtype must be float16 or bfloat16")
+    n = int(slots.shape[0])
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        t = torch.empty(n, c.kv_heads, c.head_dim, dtype=dtype, device=dev) if t is None else t
+        msg = name + " must be [slots, kv_heads, head_dim] of dtype on the cache's device, vectors contiguous"
+        _vectors(t, (dev, dtype, c.head_dim), n, msg)
+        _req(t.shape[1] == c.kv_heads, msg)
+        outs.append(t)
+    k_out, v_out = outs
+    r = _lib.OrthHipRead(_ptr(k_out), _ptr(v_out), (_stride(k_out, 0), _stride(k_out, 1)),
+                         (_stride(v_out, 0), _stride(v_out, 1)), _ptr(slots), n)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_cache_read_int4_hip(ctypes.byref(c), ctypes.byref(r), _DT[dtype], _stream(dev)))
+    return k_out, v_out
+
+
+def paged_attention_int4(q, k_codes, k_scales, v_codes, v_scales, block_table, positions, rows=None, scale=None, window=0,
+                         out=None):
+    """:func:`paged_attention` over a cache of :func:`int4_cache`, with the
+    values low + u * scale as keys and values; q and the output are float16 or
+    bfloat16."""
+    T = _lib.torch_ops()
+    if T is not None:
+        return T.paged_attention_int4(q, k_codes, k_scales, v_codes, v_scales, block_table, positions, rows, scale, window, out)
+    _no_gradient("paged_attention_int4", q=q, k_scales=k_scales, v_scales=v_scales, out=out)
+    _req(q.dim() == 3, "q" + _LIKE4.format("q_heads"))
+    c = _cache4(k_codes, k_scales, v_codes, v_scales, int(q.shape[2]))
+    dev, dtype = k_codes.device, _dtype16(q, "q")
+    a, out = _attend_args(q, (dev, q.dtype, c.head_dim), c.kv_heads, block_table, positions, rows, scale, window, out, _LIKE4)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().orth_paged_attention_int4_hip(ctypes.byref(c), ctypes.byref(a), dtype, _stream(dev)))
     return out
 
 

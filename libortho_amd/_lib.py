@@ -83,6 +83,18 @@ class OrthHipAttend(ctypes.Structure):
                 ("reserved", ctypes.c_int32)]
 
 
+class OrthHipInt4Cache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_scales", "v_scales")] + \
+               [(n, ctypes.c_int32) for n in ("page_size", "kv_heads", "head_dim", "group_size")] + \
+               [("pages", ctypes.c_int64)] + \
+               [(n, ctypes.c_int64 * 3) for n in ("k_code_strides", "v_code_strides", "k_scale_strides", "v_scale_strides")]
+
+
+class OrthHipRead(ctypes.Structure):
+    _fields_ = [("k_out", ctypes.c_void_p), ("v_out", ctypes.c_void_p), ("k_strides", ctypes.c_int64 * 2),
+                ("v_strides", ctypes.c_int64 * 2), ("slots", ctypes.c_void_p), ("count", ctypes.c_int64)]
+
+
 class OrthHipAdapter(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "out", "a", "b", "adapters", "scales")] + \
                [(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "out_stride", "tokens", "in_features",
@@ -119,6 +131,9 @@ SIGNATURES = {
     "orth_page_step_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipStep), _P]),
     "orth_cache_append_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipCache), ctypes.POINTER(OrthHipAppend), _P]),
     "orth_paged_attention_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipCache), ctypes.POINTER(OrthHipAttend), _P]),
+    "orth_cache_append_int4_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipInt4Cache), ctypes.POINTER(OrthHipAppend), _I32, _P]),
+    "orth_cache_read_int4_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipInt4Cache), ctypes.POINTER(OrthHipRead), _I32, _P]),
+    "orth_paged_attention_int4_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipInt4Cache), ctypes.POINTER(OrthHipAttend), _I32, _P]),
     "orth_adapter_add_hip": (ctypes.c_int, [ctypes.POINTER(OrthHipAdapter), _P]),
     "orth_hip_device_info": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(OrthHipDeviceInfo)]),
     "orth_hip_set_kernel_policy": (ctypes.c_int, [ctypes.c_int]),
