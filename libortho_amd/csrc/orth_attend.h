@@ -38,6 +38,7 @@ struct AttendArgs {
     float scale2;        // scale * log2(e)
     int group, gtiles;   // query heads of a key head, and their tiles of 16
     int gt;              // columns of a tile: min(group, 16), or those of a block of tokens
+    FastDiv of_chunks, of_gt;  // by head_dim / 8, by gt
     int nh, nsub;        // head tiles a workgroup takes at once, and the waves of each: nh * nsub = 4
     float *part;         // pieces [workgroups * 2][nh][gt][head_dim]
     float2 *stat;        // (m, l) [workgroups * 2][nh][16]
@@ -52,11 +53,18 @@ struct Keys {
     uint32_t units;
 };
 
-// a / b, in 32 bits where both fit (a 64-bit division takes a quarter of a
-// microsecond, and a short call is a chain of such latencies).
+// a / b.  (A 64-bit division takes a quarter of a microsecond, and a short
+// call is a chain of such latencies: below 2^22 a product with the reciprocal
+// is off by one at the most.)
 __device__ __forceinline__ uint64_t div64(uint64_t a, uint64_t b) {
     if ((a | b) >> 32) return a / b;
-    return (uint32_t)a / (uint32_t)b;
+    const uint32_t n = (uint32_t)a, d = (uint32_t)b;
+    if (n >> 22) return n / d;
+    uint32_t q = (uint32_t)((float)n * __builtin_amdgcn_rcpf((float)d));
+    const int32_t rest = (int32_t)(n - q * d);
+    if (rest < 0) q--;
+    else if ((uint32_t)rest >= d) q++;
+    return q;
 }
 
 // Memory of all XCDs: written through and read past the L2 of this one.
@@ -140,7 +148,7 @@ __device__ __forceinline__ Keys uniform(const Keys &k) {
 template <class G>
 __device__ __forceinline__ Keys keys_at(const G &g, int64_t t, int lane, int *tokens) {
     *tokens = 1;
-    if (g.block > 1 && t % g.block == 0) {
+    if (g.block > 1 && (t & (g.block - 1)) == 0) {
         Block b = block_of(g, t + (lane & (g.block - 1)));
         b.across(1, g.block);
         if (__all(b.one())) {
@@ -170,7 +178,7 @@ __device__ __forceinline__ uint32_t block_units(const G &g, int64_t t0, int lane
             b.add(block_of(g, t0 + 2 * lane + 1));
             b.across(1, g.block / 2);
             if (b.one()) {
-                if ((2 * lane) % g.block == 0) k[0] = tiles_of(g, b);
+                if ((2 * lane & (g.block - 1)) == 0) k[0] = tiles_of(g, b);
                 else k[0].units = 0;
                 k[1].units = 0;
             }
@@ -268,20 +276,20 @@ __device__ __forceinline__ bool unseen(float top, float sum) {
     else return top == -__builtin_inff();
 }
 
-// Joins the waves' sums of an item, which lie in LDS (o [waves][gt] rows of
-// row_floats, and (m, l) [waves][16]): units unit .. unit + n - 1 of it, which
+// Joins the waves' sums of an item, which lie in LDS (o: for each wave, every
+// wave_floats, gt rows of row_floats, and (m, l) [waves][16]): units unit .. unit + n - 1 of it, which
 // are written if they are all, else left as a piece, joined by the workgroup
 // that writes the last one.
 template <class G>
-__device__ __forceinline__ void finish_item(const G &g, int tid, const float *lds, const float2 *lds_stat, int row_floats, bool o16,
+__device__ __forceinline__ void finish_item(const G &g, int tid, const float *lds, const float2 *lds_stat, int row_floats, int wave_floats, bool o16,
                                             uint64_t first, uint64_t cur, uint64_t per, int64_t t, int tokens, const Keys &k,
                                             int item, uint32_t unit, uint32_t n) {
     const int D = g.c.head_dim;
     const bool whole = n == k.units;
     const int slot = (int)blockIdx.x * 2 + (cur == first ? 0 : 1);
-    const int chunks = D / 8;  // eight elements of one query head a thread
-    for (int x = tid; x < g.nh * g.gt * chunks; x += 256) {
-        const int hx = x / chunks, d = (x - hx * chunks) * 8, hh = hx / g.gt, h = hx - hh * g.gt;
+    const int chunks = D / 8, gt = g.gt;  // eight elements of one query head a thread
+    for (int x = tid; x < g.nh * gt * chunks; x += 256) {
+        const int hx = (int)quotient(x, g.of_chunks), d = (x - hx * chunks) * 8, hh = (int)quotient(hx, g.of_gt), h = hx - hh * gt;
         uint16_t *out = out_of(g, t, tokens, item * g.nh + hh, h);
         if (!out) continue;
         float top = -__builtin_inff(), sum = 0.f;
@@ -292,7 +300,7 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
             const float2 st = lds_stat[v * 16 + h];
             const float w = __builtin_amdgcn_exp2f(st.x - base);
             sum += w * st.y;
-            const float *src = lds + (v * g.gt + h) * row_floats + d;
+            const float *src = lds + v * wave_floats + h * row_floats + d;
 #pragma unroll
             for (int i = 0; i < 8; i++) r[i] += w * src[i];
         }
@@ -313,7 +321,7 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
             }
         } else {
             const int64_t piece = (int64_t)slot * g.nh + hh;
-            float *dst = g.part + (piece * g.gt + h) * D + d;
+            float *dst = g.part + (piece * gt + h) * D + d;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) store_shared(dst + i, r[i], r[i + 1]);
             if (d == 0) store_shared(&g.stat[piece * 16 + h].x, top, sum);
@@ -341,8 +349,8 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
     __syncthreads();
     if (!last_one) return;
     const int quads = D / 4;
-    for (int x = tid; x < g.nh * g.gt * quads; x += 256) {
-        const int hx = x / quads, e4 = (x - hx * quads) * 4, hh = hx / g.gt, h = hx - hh * g.gt;
+    for (int x = tid; x < g.nh * gt * quads; x += 256) {
+        const int hx = (int)quotient(x >> 1, g.of_chunks), e4 = (x - hx * quads) * 4, hh = (int)quotient(hx, g.of_gt), h = hx - hh * gt;
         uint16_t *out = out_of(g, t, tokens, item * g.nh + hh, h);
         if (!out) continue;
         float top = -__builtin_inff(), sum = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
@@ -352,7 +360,7 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
             for (int u = 0; u < 4; u++) {
                 const int i = i0 + u < to ? i0 + u : to;
                 const int64_t piece = (int64_t)(i == from ? slot0 : 2 * i) * g.nh + hh;
-                const float *src = g.part + (piece * g.gt + h) * D + e4;
+                const float *src = g.part + (piece * gt + h) * D + e4;
                 st[u] = load_shared(&g.stat[piece * 16 + h].x);
                 v[u][0] = load_shared(src);
                 v[u][1] = load_shared(src + 2);
@@ -489,6 +497,8 @@ void attend_tiles(G &g, int cus, int64_t items_of_a_head) {
     const bool few_keys = g.a.table_width <= ((int64_t)1 << 28) / g.c.page_size;  // (block_units)
     while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && items_of_a_head * (tiles / (2 * g.nh)) >= cus / 4) g.nh *= 2;
     g.nsub = kWaves / g.nh;
+    g.of_chunks = fast_div((uint32_t)g.c.head_dim / 8);
+    g.of_gt = fast_div((uint32_t)g.gt);
 }
 
 // `resident` workgroups, and no more than there can be units.

@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
             if (lg == 0) lds_stat[wave * 16 + col] = float2{m, l};
         }
         __syncthreads();
-        finish_item(g, threadIdx.x, lds, lds_stat, row_floats, o16, first, cur, per, t, 1, k, item, unit, n);
+        finish_item(g, threadIdx.x, lds, lds_stat, row_floats, g.gt * row_floats, o16, first, cur, per, t, 1, k, item, unit, n);
         __syncthreads();
         cur += n;
         unit = 0;

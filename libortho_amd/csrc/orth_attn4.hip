@@ -19,9 +19,10 @@
 //           is a whole number of steps and has its own accumulator.
 //   values  O[d] = sum_j (p_j scale_j) (u_j - 8) + sum_j p_j (low_j + 8
 //           scale_j).  A lane loads its unit of eight keys; v_perm_b32 pairs
-//           the bytes of two keys, a mask and an or make 1024 + u and 1024 +
-//           16 u, one packed subtraction u - 8 and 16 (u - 8): codes about
-//           zero, so that the sums are no larger than what they are to give.
+//           the bytes of two keys, masks make subnormal numbers of them as
+//           above, and one packed subtraction (u - 8) 2^-24 and 16 times it:
+//           codes about zero, so that the sums are no larger than what they
+//           are to give.
 //           The weights p scale enter as two FP16 parts, 2^-24 of the weight
 //           or 2^-39 of the largest of their column: the running maximum is
 //           that of score + exponent of the key's largest scale, so that
@@ -47,6 +48,7 @@ struct Attend4Args : AttendArgs<orth_hip_int4_cache_t> {
     int block;   // tokens that may share a head tile, a power of two
     int groups;  // of a vector
     int bf;
+    int wave_floats;  // of a wave's part of the LDS
     __device__ __forceinline__ uint16_t round(float v) const { return bf ? store16<true>(v) : store16<false>(v); }
 };
 
@@ -59,40 +61,52 @@ __device__ __forceinline__ void each(F &&f) {
     each_of<N>(f, std::make_integer_sequence<int, N>());
 }
 
-// Lane I's value of each row of 16 lanes.
+// Lane I's value of each quad of lanes.
 template <int I>
-__device__ __forceinline__ float from_lane(float v) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x150 + I, 0xf, 0xf, true));
+__device__ __forceinline__ float from_quad(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), I * 0x55, 0xf, 0xf, true));
 }
-
 // acc += lane I's v * x.  (The compiler folds the broadcast into a product or a
 // sum, not into a fused one.  The wait covers a v, or an x by an
 // exponential, written just before.)
 template <int I>
-__device__ __forceinline__ void add_from_lane(float &acc, float v, float x) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(acc) : "v"(v), "v"(x), "n"(I));
+__device__ __forceinline__ void add_from_quad(float &acc, float v, float x) {
+    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 quad_perm:[%3,%3,%3,%3] row_mask:0xf bank_mask:0xf" : "+v"(acc) : "v"(v), "v"(x), "n"(I));
 }
-// The same over x[0 .. 8) with lanes 8 .. 15.
-__device__ __forceinline__ void add_from_lanes(float &acc, float v, const float *x) {
+// The same over x[0 .. 4) with lanes 0 .. 3 of v and x[4 .. 8) with those of w.
+__device__ __forceinline__ void add_from_quads(float &acc, float v, float w, const float *x) {
     asm("s_nop 1\n\t"
-        "v_fmac_f32_dpp %0, %1, %2 row_newbcast:8 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %3 row_newbcast:9 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %4 row_newbcast:10 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %5 row_newbcast:11 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %6 row_newbcast:12 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %7 row_newbcast:13 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %8 row_newbcast:14 row_mask:0xf bank_mask:0xf\n\t"
-        "v_fmac_f32_dpp %0, %1, %9 row_newbcast:15 row_mask:0xf bank_mask:0xf"
+        "v_fmac_f32_dpp %0, %1, %3 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %1, %4 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %1, %5 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %1, %6 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %2, %7 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %2, %8 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %2, %9 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %0, %2, %10 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf"
         : "+v"(acc)
-        : "v"(v), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+        : "v"(v), "v"(w), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
 }
-// lane I's v * x + y, as a product and a sum (see add_from_lane; x may be a
+// lane I's v * x + y, as a product and a sum (see add_from_quad; x may be a
 // matrix product's result, whose wait only the compiler knows).
 template <int I>
-__device__ __forceinline__ float sum_from_lane(float v, float x, float y) {
+__device__ __forceinline__ float sum_from_quad(float v, float x, float y) {
 #pragma clang fp contract(off)
-    const float z = from_lane<I>(v) * x;
+    const float z = from_quad<I>(v) * x;
     return z + y;
+}
+// The value of the lane whose column is eight further.
+__device__ __forceinline__ float other_half(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true));
+}
+
+// w - part[H].
+template <int H>
+__device__ __forceinline__ float rest(float w, f16x2 part) {
+    float r;
+    if constexpr (H == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(part), "v"(w));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(part), "v"(w));
+    return r;
 }
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
@@ -105,6 +119,8 @@ __device__ __forceinline__ uint32_t two_bytes(const uint32_t *w) {
     return __builtin_amdgcn_perm(w[B / 4], w[A / 4], 0x0c000c00u | (A % 4) | (4 + B % 4) << 16);
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef const __attribute__((address_space(4))) int32_t *ConstInts;  // (scalar loads: nothing writes there meanwhile)
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -127,20 +143,54 @@ __device__ __forceinline__ void load_words(uint32_t *w, const void *p) {
     if constexpr (N % 2) w[N - 1] = s[N - 1];
 }
 
-// Workgroups that a CU holds at once (by registers).
-template <int W>
-constexpr int kResident = W > 4 ? 1 : 2;
+// N words, or the 16 bits of half a word, at base + at + more.
+template <int N>
+__device__ __forceinline__ void load_from(uint32_t *w, const uint8_t *base, uint32_t at, uint32_t more) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, -1, 0x00020000);
+    int i = 0;
+#pragma unroll
+    for (; i + 4 <= N; i += 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(at + 4 * i), (int)more, 0);
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[i + c] = v[c];
+    }
+    if constexpr (N % 4 == 3) {
+        typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+        const u32x3 v = __builtin_amdgcn_raw_buffer_load_b96(r, (int)at, (int)more, 0);
+        w[0] = v[0], w[1] = v[1], w[2] = v[2];
+    } else if constexpr (N % 4 == 2) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, (int)more, 0);
+        w[0] = v[0], w[1] = v[1];
+    } else if constexpr (N == 1) {
+        w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, (int)more, 0);
+    }
+}
+__device__ __forceinline__ uint32_t load_half_from(const uint8_t *base, uint32_t at, uint32_t more) {
+    return __builtin_amdgcn_raw_buffer_load_b16(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, -1, 0x00020000),
+                                                (int)at, (int)more, 0);
+}
 
-// W: bytes of a unit; GS: steps of 32 elements of a group; PG8: page_size is a
-// multiple of 8, so eight keys from a multiple of 8 lie in one page and one
-// table entry serves them.
-template <int W, int GS, bool PG8>
-__global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args g) {
+// Workgroups that a CU holds at once (by registers).
+template <int W, bool PG16>
+constexpr int kResident = W > 4 ? (PG16 ? 2 : 1) : 3;
+
+// W: bytes of a unit; GS: steps of 32 elements of a group.
+// PG16: page_size is a multiple of 16, so 16 keys from a multiple of 16 lie in
+// one page: a scalar table entry and scalar addresses serve them, and lanes
+// add offsets that stay the same for the whole item.
+// SETS = 2: no more than eight columns are used, so the other eight take a
+// second tile of keys, and one softmax serves both: the query's columns, and
+// later the weights', are masked to the tile's half, whose sums stay apart
+// until the item ends.
+template <int W, int GS, bool PG16, int SETS>
+__global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Attend4Args g) {
     constexpr int NG = W / GS, VD = (W + 3) / 4;
     constexpr int row_floats = 32 * W + 4;
-    // o [waves][gt][32 W + 4], then (m, l) [waves][16]; both start at 16 bytes, and so does each row of o
+    // o [waves][gt][32 W + 4], in its place before, for each wave, its queries as
+    // the products take them, then (m, l) [waves][16]; all start at 16 bytes, and
+    // so does each row of o
     extern __shared__ __align__(16) float lds[];
-    float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.gt * row_floats);
+    float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.wave_floats);
     const int D = g.c.head_dim;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int lane = threadIdx.x & 63;
@@ -152,79 +202,245 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
     const uint64_t first = uniform64(w.cur), stop = uniform64(w.stop), per = uniform64(w.per);
     uint64_t cur = w.cur;
     int64_t t = w.t;
-    Keys k = w.k;
+    Keys k = uniform(w.k);
     int item = __builtin_amdgcn_readfirstlane(w.item), tokens = 1;
     uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)w.unit);
-    if (g.block > 1) k = keys_at(g, t, lane, &tokens);
     cur = uniform64(cur), t = uniform64(t);
+    if (g.block > 1) k = keys_at(g, t, lane, &tokens);
 
     while (cur < stop) {
         // (the empty asm: nothing that follows from the lane is kept in registers
         // from one item to the next)
         asm volatile("" : "+v"(lane));
-        const int col = lane & 15, lg = lane >> 4;
-        const int64_t k_slot = g.c.k_code_strides[1], v_slot = g.c.v_code_strides[1];
+        // columns: queries (SETS = 2: `col` of half `set`)
+        const int set = SETS == 2 ? lane >> 3 & 1 : 0, col16 = lane & 15, col = SETS == 2 ? lane & 7 : col16, lg = lane >> 4;
         const bool q8 = ((reinterpret_cast<uintptr_t>(g.a.q) | (uintptr_t)(g.a.q_strides[0] * 2) | (uintptr_t)(g.a.q_strides[1] * 2)) & 7) == 0;
         const bool o16 = ((reinterpret_cast<uintptr_t>(g.a.out) | (uintptr_t)(g.a.out_strides[0] * 2) | (uintptr_t)(g.a.out_strides[1] * 2)) & 15) == 0;
-        // this lane's pairs: the keys' (col < 8) or the values'
-        const bool of_value = col >= 8;
-        const int64_t s_page = of_value ? g.c.v_scale_strides[0] : g.c.k_scale_strides[0];
-        const int64_t s_slot = of_value ? g.c.v_scale_strides[1] : g.c.k_scale_strides[1];
-        // held with the codes' 2^-24 of the scores (keys), or the weights' 2^14 (values, whose codes are 8 less)
-        const float s_held = of_value ? 0x1p14f : 0x1p24f, s_middle = of_value ? 8.f : 0.f;
         // (W == 3: the last unit is read from a byte earlier, so that its word ends with the row)
-        const int v_at = W == 3 && col == 15 ? 44 : W * col, v_shift = W == 3 && col == 15 ? 8 : 0;
+        const int v_at = W == 3 && col16 == 15 ? 44 : W * col16, v_shift = W == 3 && col16 == 15 ? 8 : 0;
+
         const uint64_t left = stop - cur;
         const uint32_t n = k.units - unit < left ? k.units - unit : (uint32_t)left;
         const int ht = item * g.nh + hw, kvh = g.gtiles == 1 ? ht : ht / g.gtiles, gt0 = (ht - kvh * g.gtiles) * 16;  // first query head of the tile
         const int cols = tokens > 1 ? tokens * g.group : g.group - gt0 < 16 ? g.group - gt0 : 16;
         const int64_t row = g.a.rows ? (int64_t)__builtin_amdgcn_readfirstlane(g.a.rows[t]) : t;
 
+        const uint32_t first_half = set ? 0u : ~0u;
         // this column's query, and the keys its token sees
-        u32x4 q[W];
+        u32x4 *const q = reinterpret_cast<u32x4 *>(lds + wave * g.wave_floats);  // [W][lanes], then zeros
+        const int j = tokens > 1 && col < cols ? col / g.group : 0;
+        uint2 raw[W][2];  // elements 32 s + 16 h + 4 lg .. + 3
+        {
+            // (columns and elements that there are not: the first one's again, cleared below)
+            const int head = col < cols ? col - j * g.group : 0;
+            const uint16_t *p = (const uint16_t *)g.a.q + (t + j) * g.a.q_strides[0] + ((int64_t)kvh * g.group + gt0 + head) * g.a.q_strides[1];
+            if (q8) {
+#pragma unroll
+                for (int x = 0; x < 2 * W; x++) {
+                    const int d = 16 * x + 4 * lg;
+                    raw[x / 2][x % 2] = *reinterpret_cast<const uint2 *>(p + (d < D ? d : 0));
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < 2 * W; x++) {
+                    const int d = 16 * x + 4 * lg;
+                    const uint16_t *e = p + (d < D ? d : 0);
+                    raw[x / 2][x % 2] = uint2{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16};
+                }
+            }
+        }
         float qs[NG], unscale;  // scale2 times the sums of the groups' elements; scale2 / the query's power of two
         int begin = k.begin, end = k.end, most_begin = k.begin, least_end = k.end;
-        {
-            const int j = tokens > 1 && col < cols ? col / g.group : 0;
-            const uint16_t *p = (const uint16_t *)g.a.q + (t + j) * g.a.q_strides[0] + ((int64_t)kvh * g.group + gt0 + (col - j * g.group)) * g.a.q_strides[1];
-            float x[W][8], top = 0.f, odd = 0.f;
+
+        const ConstInts table = (ConstInts)(g.a.block_table + row * g.a.table_stride);
+        const uint8_t *kbase = (const uint8_t *)g.c.k_codes + kvh * g.c.k_code_strides[2];
+        const uint8_t *vbase = (const uint8_t *)g.c.v_codes + kvh * g.c.v_code_strides[2];
+        const uint8_t *ksbase = (const uint8_t *)((const uint16_t *)g.c.k_scales + kvh * g.c.k_scale_strides[2]);
+        const uint8_t *vsbase = (const uint8_t *)((const uint16_t *)g.c.v_scales + kvh * g.c.v_scale_strides[2]);
+        const int last = k.end - 1;
+        const uint64_t upto = (uint64_t)(unit + n) * (kPair * g.nsub);
+        const int tiles = (int)(upto < (uint64_t)k.tiles ? upto : (uint64_t)k.tiles);
+        // a wave's passes of SETS tiles
+        const int step = g.nsub, pass_end = (tiles + SETS - 1) / SETS;
+        int pass = (int)unit * (kPair / SETS * g.nsub) + sub;
+        const uint32_t key_first = (uint32_t)k.tile0 * kTile;
+
+        f32x4 o[2 * W];
+        float m = -__builtin_inff(), l = 0.f, lows[NG];  // lows: sum p (low + 8 scale)
 #pragma unroll
-            for (int s = 0; s < W; s++)
+        for (int e = 0; e < 2 * W; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int d = 32 * s + 16 * h + 4 * lg;
-                    uint16_t e[4] = {0, 0, 0, 0};
-                    if (col < cols && d < D) {
-                        if (q8) {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(p + d);
-                            e[0] = (uint16_t)v.x, e[1] = (uint16_t)(v.x >> 16), e[2] = (uint16_t)v.y, e[3] = (uint16_t)(v.y >> 16);
-                        } else {
+        for (int i = 0; i < NG; i++) lows[i] = 0.f;
+
+        // what a wave holds of a pass until it is taken
+        uint32_t kc[SETS][2][W];   // units 4 lg .. of keys 32 set + 16 tau + col16
+        uint32_t vc[SETS][8][VD];  // unit col16 of keys 32 set + 16 tau + 4 lg + i, as 4 tau + i
+        uint32_t kp[2][NG], vp[2][NG];  // (scale, low) of key and value 32 set + 16 tau + 4 lg + lane % 4
+        uint32_t seen8 = 0xff;     // which of this column's eight keys lie in a page of the cache
+        int32_t page[SETS][2];     // with PG16: the pages of the next pass to load
+
+        // keys past the last are taken as the last (with PG16 the first key of
+        // sixteen stands for all: they lie in its page also where the last key
+        // ends inside it)
+        const uint32_t limit = (uint32_t)(PG16 ? last & ~15 : last);
+        auto entry = [&](uint32_t key) -> int32_t { return table[quotient(key < limit ? key : limit, g.page)]; };
+        auto inside = [&](uint32_t key) -> uint32_t {  // a key's slot in its page
+            key = key < limit ? key : limit;
+            return key - quotient(key, g.page) * g.page.d;
+        };
+        auto known = [&](int32_t pg) -> int64_t { return (uint32_t)pg < (uint64_t)g.c.pages ? (int64_t)pg : 0; };
+        auto key_of = [&](int ps, int s, int tau) -> uint32_t { return key_first + (uint32_t)ps * (kTile * SETS) + kTile * s + 16 * tau; };
+        auto load_entries = [&](int ps) {
+            if constexpr (PG16) {
 #pragma unroll
-                            for (int c = 0; c < 4; c++) e[c] = p[d + c];
-                        }
-                    }
+                for (int s = 0; s < SETS; s++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const float v = g.bf ? load16<true>(e[c]) : load16<false>(e[c]);
-                        x[s][4 * h + c] = v;
-                        top = fmaxf(top, fabsf(v));
-                        odd += v * 0.f;  // NaN from what is not finite
+                    for (int tau = 0; tau < 2; tau++) page[s][tau] = entry(key_of(ps, s, tau));
+            }
+        };
+        // (with PG16 strides are those of the keys and the values, and 32-bit)
+        const uint32_t slot = (uint32_t)g.c.k_code_strides[1], scale_slot = (uint32_t)g.c.k_scale_strides[1] * 2;
+        const uint32_t k_at = (uint32_t)col16 * slot + lg * 4 * W, v_first = 4 * lg * slot + v_at;
+        const uint32_t s_at = (4 * lg + (lane & 3)) * scale_slot;
+        auto code_place = [&](uint32_t key, int32_t pg) -> uint64_t {
+            return (uint64_t)(uint32_t)known(pg) * (uint32_t)g.c.k_code_strides[0] + inside(key) * slot;
+        };
+        auto scale_place = [&](uint32_t key, int32_t pg) -> uint64_t {
+            return (uint64_t)(uint32_t)known(pg) * (uint32_t)(g.c.k_scale_strides[0] * 2) + inside(key) * scale_slot;
+        };
+        auto load_k = [&](int ps) {
+#pragma unroll
+            for (int s = 0; s < SETS; s++)
+#pragma unroll
+                for (int tau = 0; tau < 2; tau++) {
+                    const uint32_t key = key_of(ps, s, tau);
+                    if constexpr (PG16) {
+                        load_from<W>(kc[s][tau], kbase + code_place(key, page[s][tau]), k_at, 0);
+                    } else {
+                        const uint32_t x = key + col16;
+                        load_words<W>(kc[s][tau], kbase + known(entry(x)) * g.c.k_code_strides[0] + (int64_t)inside(x) * g.c.k_code_strides[1] + lg * 4 * W);
                     }
                 }
+        };
+        auto load_pairs = [&](uint32_t *pair, const uint8_t *p) {
+            if constexpr (W == 8) {  // (only vectors past 128 elements may have fewer groups than steps)
+#pragma unroll
+                for (int i = 0; i < NG; i++) pair[i] = reinterpret_cast<const uint32_t *>(p)[i < g.groups ? i : g.groups - 1];
+            } else {
+                load_words<NG>(pair, p);
+            }
+        };
+        auto load_v = [&](int ps) {
+#pragma unroll
+            for (int tau = 0; tau < 2; tau++) {
+                if constexpr (PG16) {
+                    uint64_t at = scale_place(key_of(ps, 0, tau), page[0][tau]);
+                    if constexpr (SETS == 2) {
+                        const uint64_t at1 = scale_place(key_of(ps, 1, tau), page[1][tau]);
+                        at = set ? at1 : at;
+                    }
+                    at += s_at;
+                    load_pairs(kp[tau], ksbase + at);
+                    load_pairs(vp[tau], vsbase + at);
+                } else {
+                    const uint32_t x = key_of(ps, 0, tau) + 4 * lg + (lane & 3);
+                    const int64_t pg = known(entry(x)), in = inside(x);
+                    load_pairs(kp[tau], ksbase + 2 * (pg * g.c.k_scale_strides[0] + in * g.c.k_scale_strides[1]));
+                    load_pairs(vp[tau], vsbase + 2 * (pg * g.c.v_scale_strides[0] + in * g.c.v_scale_strides[1]));
+                }
+            }
+            seen8 = 0;
+#pragma unroll
+            for (int s = 0; s < SETS; s++)
+#pragma unroll
+                for (int tau = 0; tau < 2; tau++) {
+                    const uint32_t key = key_of(ps, s, tau);
+                    const uint8_t *p = vbase;
+                    if constexpr (PG16) {
+                        p += code_place(key, page[s][tau]);
+                        if ((uint32_t)page[s][tau] < (uint64_t)g.c.pages) seen8 |= 0xfu << (4 * tau + 8 * s);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t *dst = vc[s][4 * tau + i];
+                        if constexpr (PG16 && W != 3) {
+                            if constexpr (W == 2) dst[0] = load_half_from(p, v_first, i * slot);
+                            else load_from<VD>(dst, p, v_first, i * slot);
+                        } else {
+                            const uint8_t *x = p + (v_first + i * slot);
+                            if constexpr (!PG16) {
+                                const uint32_t y = key + 4 * lg + i;
+                                const int32_t pg = entry(y);
+                                x = p + known(pg) * g.c.v_code_strides[0] + (int64_t)inside(y) * g.c.v_code_strides[1] + v_at;
+                                seen8 |= (uint32_t)((uint32_t)pg < (uint64_t)g.c.pages) << (4 * tau + i);
+                            }
+                            if constexpr (W == 2) dst[0] = *reinterpret_cast<const uint16_t *>(x);
+                            else if constexpr (W == 3) __builtin_memcpy(dst, x, 4);
+                            else load_words<VD>(dst, x);
+                        }
+                    }
+                }
+        };
+
+        if (pass < pass_end) {
+            load_entries(pass);
+            load_k(pass);
+            load_v(pass);
+            load_entries(pass + step);
+        }
+        {
+            float x[W][8];
+            uint32_t most = 0;  // the largest of the elements' bits but for their signs, in each half
+#pragma unroll
+            for (int y = 0; y < 2 * W; y++) {
+                uint2 &w2 = raw[y / 2][y % 2];
+                if (col >= cols || 16 * y + 4 * lg >= D) w2 = uint2{0u, 0u};
+                typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                auto more = [&](uint32_t v) {
+                    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, v & 0x7fff7fffu)));
+                };
+                more(w2.x);
+                more(w2.y);
+            }
+            most = most >> 16 > (most & 0xffff) ? most >> 16 : most & 0xffff;
+            float top;
+            if (g.bf) {
+#pragma unroll
+                for (int y = 0; y < 2 * W; y++) {
+                    const uint2 v = raw[y / 2][y % 2];
+                    float *dst = &x[y / 2][4 * (y % 2)];
+                    dst[0] = __uint_as_float(v.x << 16), dst[1] = __uint_as_float(v.x & 0xffff0000u);
+                    dst[2] = __uint_as_float(v.y << 16), dst[3] = __uint_as_float(v.y & 0xffff0000u);
+                }
+                top = __uint_as_float(most << 16);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 2 * W; y++) {
+                    const f16x2 v0 = __builtin_bit_cast(f16x2, raw[y / 2][y % 2].x), v1 = __builtin_bit_cast(f16x2, raw[y / 2][y % 2].y);
+                    float *dst = &x[y / 2][4 * (y % 2)];
+                    dst[0] = (float)v0[0], dst[1] = (float)v0[1], dst[2] = (float)v1[0], dst[3] = (float)v1[1];
+                }
+                top = load16<false>((uint16_t)most);
+            }
+            const float odd = column_sum(top * 0.f);  // NaN where an element is not finite
             const int up = 15 - __builtin_amdgcn_frexp_expf(column_max(top));
-            unscale = ldexpf(g.scale2, -up) + column_sum(odd);
+            unscale = ldexpf(g.scale2, -up) + odd;
 #pragma unroll
             for (int s = 0; s < W; s++) {
                 float y[8];
 #pragma unroll
                 for (int c = 0; c < 8; c++) y[c] = ldexpf(x[s][c], c < 4 ? up : up - 4);
+                u32x4 v;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     // elements 4 lg + 0, 1; 16 on; 4 lg + 2, 3; 16 on
-                    const f16x2 h = {(f16)y[c == 0 ? 0 : c == 1 ? 4 : c == 2 ? 2 : 6], (f16)y[c == 0 ? 1 : c == 1 ? 5 : c == 2 ? 3 : 7]};
-                    q[s][c] = __builtin_bit_cast(uint32_t, h);
+                    const int e = c == 0 ? 0 : c == 1 ? 4 : c == 2 ? 2 : 6;
+                    v[c] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{y[e], y[e + 1]}, f16x2));
                 }
+                q[64 * s + lane] = v;
             }
+            if (SETS == 2 && lane == 0) q[64 * W] = u32x4{0u, 0u, 0u, 0u};
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 float sum = 0.f;
@@ -249,120 +465,8 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
                 least_end = __builtin_amdgcn_readfirstlane(least_end);
             }
         }
-
-        const int32_t *table = g.a.block_table + row * g.a.table_stride;
-        const uint8_t *kbase = (const uint8_t *)g.c.k_codes + kvh * g.c.k_code_strides[2];
-        const uint8_t *vbase = (const uint8_t *)g.c.v_codes + kvh * g.c.v_code_strides[2];
-        const uint16_t *sbase = of_value ? (const uint16_t *)g.c.v_scales + kvh * g.c.v_scale_strides[2]
-                                         : (const uint16_t *)g.c.k_scales + kvh * g.c.k_scale_strides[2];
-        const int last = k.end - 1;
-        const uint64_t upto = (uint64_t)(unit + n) * (kPair * g.nsub);
-        const int step = g.nsub, tile_end = k.tile0 + (int)(upto < (uint64_t)k.tiles ? upto : (uint64_t)k.tiles);
-        int tile = k.tile0 + (int)unit * (kPair * g.nsub) + sub;
-
-        f32x4 o[2 * W];
-        float m = -__builtin_inff(), l = 0.f, lows[NG];  // lows: sum p (low + 8 scale)
-#pragma unroll
-        for (int e = 0; e < 2 * W; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NG; i++) lows[i] = 0.f;
-
-        // a key's page (-1: outside the cache) and its place; keys past the last
-        // are taken as the last (with PG8 the first key of a group of eight
-        // stands for all: the group lies in its page also where the last key
-        // ends inside it)
-        const int limit = PG8 ? last & ~7 : last;
-        auto entry = [&](int key) -> int32_t { return table[quotient((uint32_t)(key < limit ? key : limit), g.page)]; };
-        auto place = [&](int key, int32_t page, int64_t s0, int64_t s1) -> int64_t {
-            key = key < limit ? key : limit;
-            const uint32_t in = (uint32_t)key - quotient((uint32_t)key, g.page) * g.page.d;
-            return ((uint32_t)page < (uint64_t)g.c.pages ? (int64_t)page : 0) * s0 + (int64_t)in * s1;
-        };
-
-        // what a wave holds of a tile until it is taken
-        uint32_t kc[2][W];        // units 4 lg .. of keys 8 (col / 4) + col % 4 and + 4
-        uint32_t vc[8][VD];       // unit col of keys 8 lg ..
-        uint32_t pair[NG];        // (scale, low) of key (col < 8) or value 8 lg + col % 8
-        int32_t page = 0;         // of keys 8 lg ..
-        uint32_t seen8 = 0xff;    // (without PG8: which of them lie in a page of the cache)
-        int32_t ke = 0, ve = 0;   // with PG8: the pages of the next tile to load
-
-        auto load_entries = [&](int tl) {
-            if constexpr (PG8) {
-                ke = entry(tl * kTile + (col >> 2) * 8);
-                ve = entry(tl * kTile + lg * 8);
-            }
-        };
-        auto load_k = [&](int tl) {
-            const int key = tl * kTile + (col >> 2) * 8;
-            const uint8_t *p[2];
-            if constexpr (PG8) {
-                p[0] = kbase + place(key, ke, g.c.k_code_strides[0], k_slot) + (col & 3) * k_slot;
-                p[1] = p[0] + 4 * k_slot;
-            } else {
-#pragma unroll
-                for (int tau = 0; tau < 2; tau++) {
-                    const int x = key + 4 * tau + (col & 3);
-                    p[tau] = kbase + place(x, entry(x), g.c.k_code_strides[0], k_slot);
-                }
-            }
-#pragma unroll
-            for (int tau = 0; tau < 2; tau++) load_words<W>(kc[tau], p[tau] + lg * 4 * W);
-        };
-        auto load_v = [&](int tl) {
-            const int key = tl * kTile + lg * 8;
-            const uint8_t *p = vbase;
-            const uint16_t *sp = sbase;
-            if constexpr (PG8) {
-                page = ve;
-                p += place(key, ve, g.c.v_code_strides[0], v_slot);
-                sp += place(key, ve, s_page, s_slot) + (col & 7) * s_slot;
-            } else {
-                seen8 = 0;
-                const int x = key + (col & 7);
-                sp += place(x, entry(x), s_page, s_slot);
-            }
-            if constexpr (W == 8) {  // (only vectors past 128 elements may have fewer groups than steps)
-#pragma unroll
-                for (int i = 0; i < NG; i++) pair[i] = reinterpret_cast<const uint32_t *>(sp)[i < g.groups ? i : g.groups - 1];
-            } else {
-                load_words<NG>(pair, sp);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint8_t *x = p;
-                if constexpr (PG8) {
-                    x += i * v_slot;
-                } else {
-                    const int32_t pg = entry(key + i);
-                    x += place(key + i, pg, g.c.v_code_strides[0], v_slot);
-                    seen8 |= (uint32_t)((uint32_t)pg < (uint64_t)g.c.pages) << i;
-                }
-                x += v_at;
-                if constexpr (W == 2) vc[i][0] = *reinterpret_cast<const uint16_t *>(x);
-                else if constexpr (W == 3) __builtin_memcpy(&vc[i][0], x, 4);
-                else load_words<VD>(vc[i], x);
-            }
-        };
-
-        if (tile < tile_end) {
-            load_entries(tile);
-            load_k(tile);
-            load_v(tile);
-            load_entries(tile + step);
-        }
-        for (; tile < tile_end; tile += step) {
-            // scores
-            float sc[NG], lo[NG], size = 0.f;
-#pragma unroll
-            for (int i = 0; i < NG; i++) {
-                const f16x2 v = __builtin_bit_cast(f16x2, pair[i]);
-                const float scale = (float)v[0];
-                size = fmaxf(size, fabsf(scale));
-                sc[i] = scale * s_held;
-                lo[i] = fmaf(scale, s_middle, (float)v[1]);
-            }
-            const float expo = (float)__builtin_amdgcn_frexp_expf(size);
+        for (; pass < pass_end; pass += step) {
+            // scores: lane (col, lg) of half `set` gets those of its eight keys
             float x[8], offset[8];
             each<NG>([&](auto group) {
                 constexpr int C = group.value;
@@ -372,45 +476,66 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
                 each<GS>([&](auto b) {
                     constexpr int B = C * GS + b.value;
 #pragma unroll
-                    for (int tau = 0; tau < 2; tau++) {
-                        const uint32_t y = two_bytes<B, W + B>(kc[tau]), z = two_bytes<2 * W + B, 3 * W + B>(kc[tau]);
-                        acc[tau] = mfma16(u32x4{y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u}, q[B], acc[tau]);
+                    for (int s = 0; s < SETS; s++) {
+                        const u32x4 qm = q[SETS == 1 || set == s ? 64 * B + lane : 64 * W];
+#pragma unroll
+                        for (int tau = 0; tau < 2; tau++) {
+                            const uint32_t y = two_bytes<B, W + B>(kc[s][tau]), z = two_bytes<2 * W + B, 3 * W + B>(kc[s][tau]);
+                            acc[tau] = mfma16(u32x4{y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u}, qm, acc[tau]);
+                        }
                     }
                 });
+                float sc[2], lo[2];
+#pragma unroll
+                for (int tau = 0; tau < 2; tau++) {
+                    const f16x2 v = __builtin_bit_cast(f16x2, kp[tau][C]);
+                    sc[tau] = (float)v[0] * 0x1p24f;  // (the codes' 2^-24)
+                    lo[tau] = (float)v[1];
+                }
                 each<8>([&](auto i) {
-                    constexpr int I = i.value;
+                    constexpr int I = i.value, T = I >> 2;
                     if constexpr (C == 0) {
-                        x[I] = from_lane<I>(sc[0]) * acc[I >> 2][I & 3];
-                        offset[I] = from_lane<I>(lo[0]) * qs[0];
+                        x[I] = from_quad<(I & 3)>(sc[T]) * acc[T][I & 3];
+                        offset[I] = from_quad<(I & 3)>(lo[T]) * qs[0];
                     } else {
-                        x[I] = sum_from_lane<I>(sc[C], acc[I >> 2][I & 3], x[I]);
-                        add_from_lane<I>(offset[I], lo[C], qs[C]);
+                        x[I] = sum_from_quad<(I & 3)>(sc[T], acc[T][I & 3], x[I]);
+                        add_from_quad<(I & 3)>(offset[I], lo[T], qs[C]);
                     }
                 });
             });
             __builtin_amdgcn_sched_barrier(0);
-            load_k(tile + step);  // (past the end: the last keys again)
+            load_k(pass + step);  // (past the end: the last keys again)
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = fmaf(unscale, x[i], offset[i]);
 
-            const int key0 = tile * kTile;
-            const bool paged = PG8 ? (uint32_t)page < (uint64_t)g.c.pages : seen8 == 0xff;
-            const bool masked = key0 < most_begin || key0 + kTile > least_end || !__all(paged);
+            const int key0 = (int)key_of(pass, 0, 0);
+            const bool masked = (key0 < most_begin) | (key0 > least_end - kTile * SETS) | !__all(seen8 == (SETS == 2 ? 0xffffu : 0xffu));
             uint32_t in8 = 0xff;  // which of the lane's keys its column sees
             if (masked) {
-                asm volatile("");  // (a branch: tiles at the ends of a range are few)
+                asm volatile("");  // (a branch: passes at the ends of a range are few)
                 in8 = 0;
+                const int mine = key0 + kTile * set + 4 * lg;
+                const uint32_t paged = seen8 >> 8 * set;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int key = key0 + 8 * lg + i;
-                    const bool in = key >= begin && key < end && (PG8 ? paged : (seen8 >> i & 1) != 0);
+                    const int key = mine + 16 * (i >> 2) + (i & 3);
+                    const bool in = key >= begin && key < end && (paged >> i & 1) != 0;
                     in8 |= (uint32_t)in << i;
                     if (!in) x[i] = -__builtin_inff();
                 }
+                asm volatile("" : "+v"(in8));  // (kept as bits)
+            }
+            float expo[2];
+#pragma unroll
+            for (int tau = 0; tau < 2; tau++) {
+                float size = 0.f;
+#pragma unroll
+                for (int i = 0; i < NG; i++) size = fmaxf(size, fabsf((float)__builtin_bit_cast(f16x2, vp[tau][i])[0]));
+                expo[tau] = (float)__builtin_amdgcn_frexp_expf(size);
             }
             float top = -__builtin_inff();
-            each<8>([&](auto i) { top = fmaxf(top, x[i.value] + from_lane<8 + i.value>(expo)); });
+            each<8>([&](auto i) { top = fmaxf(top, x[i.value] + from_quad<(i.value & 3)>(expo[i.value >> 2])); });
             top = fmaxf(fmaxf(column_max(top), kLeast), m);
             if (__any(top > m)) {
                 const float keep = __builtin_amdgcn_exp2f(m - top);
@@ -430,16 +555,26 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
             }
             each<NG>([&](auto group) {
                 constexpr int C = group.value;
-                float weight[8];
-                float sum = 0.f;
-                add_from_lanes(sum, lo[C], x);
-                each<8>([&](auto i) { weight[i.value] = from_lane<8 + i.value>(sc[C]) * x[i.value]; });
+                float sc[2], lo[2];
+#pragma unroll
+                for (int tau = 0; tau < 2; tau++) {
+                    const f16x2 v = __builtin_bit_cast(f16x2, vp[tau][C]);
+                    const float scale = (float)v[0];
+                    sc[tau] = scale * 0x1p14f;  // (held so, as FP16)
+                    lo[tau] = fmaf(scale, 8.f, (float)v[1]);
+                }
+                float weight[8], sum = 0.f;
+                add_from_quads(sum, lo[0], lo[1], x);
+                each<8>([&](auto i) { weight[i.value] = from_quad<(i.value & 3)>(sc[i.value >> 2]) * x[i.value]; });
+                // (taken here, not once for each side of the branch, where they lose the broadcast that a product takes in)
+                asm volatile("" : "+v"(weight[0]), "+v"(weight[1]), "+v"(weight[2]), "+v"(weight[3]), "+v"(weight[4]),
+                             "+v"(weight[5]), "+v"(weight[6]), "+v"(weight[7]));
                 if (masked) {  // once more without the hidden keys, whose numbers may be anything
                     asm volatile("");
                     sum = 0.f;
                     each<8>([&](auto i) {
                         const bool in = in8 >> i.value & 1;
-                        const float scale = from_lane<8 + i.value>(sc[C]), low = from_lane<8 + i.value>(lo[C]);
+                        const float scale = from_quad<(i.value & 3)>(sc[i.value >> 2]), low = from_quad<(i.value & 3)>(lo[i.value >> 2]);
                         weight[i.value] = in ? scale * x[i.value] : 0.f;
                         sum += in ? low * x[i.value] : 0.f;
                     });
@@ -448,54 +583,82 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
                 u32x4 part[2];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const f16x2 big = {(f16)weight[2 * i], (f16)weight[2 * i + 1]};
-                    const f16x2 small = {(f16)(weight[2 * i] - (float)big[0]), (f16)(weight[2 * i + 1] - (float)big[1])};
+                    const f16x2 big = __builtin_convertvector(f32x2{weight[2 * i], weight[2 * i + 1]}, f16x2);
+                    const f16x2 small = __builtin_convertvector(f32x2{rest<0>(weight[2 * i], big), rest<1>(weight[2 * i + 1], big)}, f16x2);
                     part[0][i] = __builtin_bit_cast(uint32_t, big);
                     part[1][i] = __builtin_bit_cast(uint32_t, small);
                 }
-                each<GS>([&](auto b) {
-                    constexpr int B = C * GS + b.value;
-                    u32x4 even, odd;  // elements 32 B + col and 16 on of the lane's eight keys
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t w2[2] = {W == 3 ? vc[2 * i][B / 4] >> v_shift : vc[2 * i][B / 4],
-                                                W == 3 ? vc[2 * i + 1][B / 4] >> v_shift : vc[2 * i + 1][B / 4]};
-                        const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
-                        const f16x2 e = __builtin_bit_cast(f16x2, (y & 0x000f000fu) | 0x64006400u) - f16x2{(f16)1032.f, (f16)1032.f};
-                        const f16x2 h = __builtin_bit_cast(f16x2, (y & 0x00f000f0u) | 0x64006400u) - f16x2{(f16)1152.f, (f16)1152.f};
-                        even[i] = __builtin_bit_cast(uint32_t, e);
-                        odd[i] = __builtin_bit_cast(uint32_t, h);
-                    }
+                for (int s = 0; s < SETS; s++) {
+                    u32x4 pm[2] = {part[0], part[1]};
+                    if constexpr (SETS == 2)
 #pragma unroll
-                    for (int z = 0; z < 2; z++) {
-                        o[2 * B] = mfma16(even, part[z], o[2 * B]);
-                        o[2 * B + 1] = mfma16(odd, part[z], o[2 * B + 1]);
-                    }
-                });
+                        for (int z = 0; z < 2; z++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) pm[z][c] &= s ? ~first_half : first_half;
+                    each<GS>([&](auto b) {
+                        constexpr int B = C * GS + b.value;
+                        u32x4 even, odd;  // elements 32 B + col16 and 16 on of the lane's eight keys
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t w2[2] = {W == 3 ? vc[s][2 * i][B / 4] >> v_shift : vc[s][2 * i][B / 4],
+                                                    W == 3 ? vc[s][2 * i + 1][B / 4] >> v_shift : vc[s][2 * i + 1][B / 4]};
+                            const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
+                            const f16x2 e = __builtin_bit_cast(f16x2, y & 0x000f000fu) - f16x2{(f16)0x8p-24f, (f16)0x8p-24f};
+                            const f16x2 h = __builtin_bit_cast(f16x2, y & 0x00f000f0u) - f16x2{(f16)0x80p-24f, (f16)0x80p-24f};
+                            even[i] = __builtin_bit_cast(uint32_t, e);
+                            odd[i] = __builtin_bit_cast(uint32_t, h);
+                        }
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {
+                            o[2 * B] = mfma16(even, pm[z], o[2 * B]);
+                            o[2 * B + 1] = mfma16(odd, pm[z], o[2 * B + 1]);
+                        }
+                    });
+                }
             });
             __builtin_amdgcn_sched_barrier(0);
-            load_v(tile + step);
-            load_entries(tile + 2 * step);
+            load_v(pass + step);
+            load_entries(pass + 2 * step);
             __builtin_amdgcn_sched_barrier(0);
         }
 
+        if constexpr (SETS == 2) {  // the halves' sums together
+            const float top = fmaxf(m, other_half(m)), base = top == -__builtin_inff() ? 0.f : top;
+            const float keep = __builtin_amdgcn_exp2f(m - base);
+            l *= keep;
+            l += other_half(l);
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                lows[i] *= keep;
+                lows[i] += other_half(lows[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2 * W; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    o[e][i] *= keep;
+                    o[e][i] += other_half(o[e][i]);
+                }
+            m = top;
+        }
         // join the waves of each head tile
         l = column_sum(l);
 #pragma unroll
         for (int i = 0; i < NG; i++) lows[i] = column_sum(lows[i]);
-        if (col < cols) {
-            float *dst = lds + (wave * g.gt + col) * row_floats + 4 * lg;
+        if (col < cols && set == 0) {
+            float *dst = lds + wave * g.wave_floats + col * row_floats + 4 * lg;
 #pragma unroll
             for (int e = 0; e < 2 * W; e++) {
-                const float f = e % 2 ? 0x1p-18f : 0x1p-14f, b = lows[e / (2 * GS)];
+                const float f = e % 2 ? 0x1p6f : 0x1p10f, b = lows[e / (2 * GS)];
                 *reinterpret_cast<f32x4 *>(dst + 16 * e) = f32x4{fmaf(o[e][0], f, b), fmaf(o[e][1], f, b), fmaf(o[e][2], f, b), fmaf(o[e][3], f, b)};
             }
             if (lg == 0) lds_stat[wave * 16 + col] = float2{m, l};
         }
         __syncthreads();
-        finish_item(g, wave * 64 + lane, lds, lds_stat, row_floats, o16, first, cur, per, t, tokens, k, item, unit, n);
+        finish_item(g, wave * 64 + lane, lds, lds_stat, row_floats, g.wave_floats, o16, first, cur, per, t, tokens, k, item, unit, n);
         __syncthreads();
-        cur += n;
+        cur = uniform64(cur + n);
         unit = 0;
         if (++item == items) {
             item = 0;
@@ -503,6 +666,16 @@ __global__ __launch_bounds__(256, kResident<W>) void attend4_kernel(Attend4Args 
             if (cur < stop) k = keys_at(g, t, lane, &tokens);
         }
     }
+}
+
+// Whether sixteen keys lie in one page, keys and values lie alike, and a
+// page's offsets are 32-bit.
+bool by_sixteen(const orth_hip_int4_cache_t &c) {
+    constexpr int64_t most = (int64_t)1 << 31;
+    for (int i = 0; i < 2; i++)
+        if (c.k_code_strides[i] != c.v_code_strides[i] || c.k_scale_strides[i] != c.v_scale_strides[i]) return false;
+    return c.page_size % 16 == 0 && c.k_code_strides[0] < most && c.k_scale_strides[0] < most / 2 &&
+           c.k_code_strides[1] < most / c.page_size && c.k_scale_strides[1] < most / 2 / c.page_size;
 }
 
 // What both the workspace and the launch go by.
@@ -515,12 +688,17 @@ Attend4Args attend4_args(const orth_hip_int4_cache_t &c, const orth_hip_attend_t
     g.group = a.q_heads / c.kv_heads;
     g.gtiles = (g.group + 15) / 16;
     g.groups = c.head_dim / c.group_size;
+    // Neighbouring tokens share a product where some request must have several:
+    // more tokens than requests.  (Else the columns are those of one token, and
+    // with eight or fewer of them two tiles of keys share one.)
     g.block = 1;
-    if (a.rows && a.tokens > 1)
+    if (a.rows && a.tokens > a.table_rows)
         while (2 * g.block * g.group <= 16) g.block *= 2;
     g.gt = g.block * g.group < 16 ? g.block * g.group : 16;
     attend_tiles(g, cus, a.tokens);
-    *groups = attend_groups(g, (int64_t)cus * (c.head_dim > 128 ? kResident<8> : kResident<4>), g.block);
+    const int resident = by_sixteen(c) ? c.head_dim > 128 ? kResident<8, true> : kResident<4, true>
+                                       : c.head_dim > 128 ? kResident<8, false> : kResident<4, false>;
+    *groups = attend_groups(g, (int64_t)cus * resident, g.block);
     return g;
 }
 
@@ -541,7 +719,9 @@ hipError_t launch_paged_attention4(const orth_hip_int4_cache_t &c, const orth_hi
     g.bf = dtype == ORTH_DT_BF16;
     const hipError_t e = by_int4_layout(c, [&](auto unit, auto steps) -> hipError_t {
         constexpr int W = decltype(unit)::value, GS = decltype(steps)::value;
-        const size_t lds = (size_t)kWaves * g.gt * (32 * W + 4) * 4 + kWaves * 16 * sizeof(float2);
+        const int rows = g.gt * (32 * W + 4), queries = 256 * W + 4;
+        g.wave_floats = rows > queries ? rows : queries;
+        const size_t lds = (size_t)kWaves * g.wave_floats * 4 + kWaves * 16 * sizeof(float2);
         auto go = [&](auto kernel) -> hipError_t {
             if (lds > 48 * 1024) {
                 hipError_t s = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -551,7 +731,8 @@ hipError_t launch_paged_attention4(const orth_hip_int4_cache_t &c, const orth_hi
             kernel<<<dim3((unsigned)groups), 256, lds, stream>>>(g);
             return hipGetLastError();
         };
-        return c.page_size % 8 == 0 ? go(attend4_kernel<W, GS, true>) : go(attend4_kernel<W, GS, false>);
+        if (!by_sixteen(c)) return go(attend4_kernel<W, GS, false, 1>);
+        return g.gt <= 8 && W <= 4 ? go(attend4_kernel<W, GS, true, W <= 4 ? 2 : 1>) : go(attend4_kernel<W, GS, true, 1>);
     });
     if (e != hipSuccess) return e;
     return attend_joins(g, groups, g.block) ? launch_join(g, groups, stream) : hipSuccess;
