@@ -66,6 +66,7 @@ int orth_cache_read_int4_hip(const orth_hip_int4_cache_t *c, const orth_hip_read
         if ((rc = check_heads(r->k_strides, r->count, c->kv_heads, "a stride of k_out is negative or too large")) != ORTH_OK ||
             (rc = check_heads(r->v_strides, r->count, c->kv_heads, "a stride of v_out is negative or too large")) != ORTH_OK)
             return rc;
+        if (c->kv_heads > (1 << 24)) return host_fail(ORTH_ERR_UNSUPPORTED, "kv_heads passes 2^24");
         if (r->count == 0) return ORTH_OK;
         if (!apart(r->k_strides, r->count, c->kv_heads, c->head_dim) || !apart(r->v_strides, r->count, c->kv_heads, c->head_dim))
             return invalid("the vectors of k_out or v_out overlap");
