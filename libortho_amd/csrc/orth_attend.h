@@ -490,12 +490,13 @@ int64_t attend_units(const G &g, int64_t block = 1) {
 // (128 requests: 569 us in the kernel, 605 with one tile).  Few items are
 // cut along the keys instead, so that their pieces are few (40 requests of
 // four heads at four tiles a workgroup: 21.9 us, at two 15.9).
+// `least`: the items that are enough.
 template <class G>
-void attend_tiles(G &g, int cus, int64_t items_of_a_head) {
+void attend_tiles(G &g, int64_t least, int64_t items_of_a_head) {
     const int64_t tiles = (int64_t)g.c.kv_heads * g.gtiles;
     g.nh = 1;
     const bool few_keys = g.a.table_width <= ((int64_t)1 << 28) / g.c.page_size;  // (block_units)
-    while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && items_of_a_head * (tiles / (2 * g.nh)) >= cus / 4) g.nh *= 2;
+    while (few_keys && g.nh < kWaves && tiles % (2 * g.nh) == 0 && items_of_a_head * (tiles / (2 * g.nh)) >= least) g.nh *= 2;
     g.nsub = kWaves / g.nh;
     g.of_chunks = fast_div((uint32_t)g.c.head_dim / 8);
     g.of_gt = fast_div((uint32_t)g.gt);

@@ -397,7 +397,7 @@ Attend16<BF> attend_args(const orth_hip_cache_t &c, const orth_hip_attend_t &a, 
     g.group = a.q_heads / c.kv_heads;
     g.gtiles = (g.group + 15) / 16;
     g.gt = g.group < 16 ? g.group : 16;
-    attend_tiles(g, cus, a.tokens);
+    attend_tiles(g, cus / 4, a.tokens);
     *groups = attend_groups(g, (int64_t)cus * (c.head_dim > 128 ? 1 : c.head_dim > 64 ? 2 : 3));
     return g;
 }

@@ -695,7 +695,13 @@ Attend4Args attend4_args(const orth_hip_int4_cache_t &c, const orth_hip_attend_t
     if (a.rows && a.tokens > a.table_rows)
         while (2 * g.block * g.group <= 16) g.block *= 2;
     g.gt = g.block * g.group < 16 ? g.block * g.group : 16;
-    attend_tiles(g, cus, a.tokens);
+    // The pieces of a full tile are twice as long, so there neighbouring heads
+    // go together from two items a CU on, else from one for four CUs (8 key
+    // heads with 16 columns each; one, two and four heads a workgroup: 1,024
+    // items of a head, 128 tokens of four prompts 108, 112 and 135 us, 8 tokens
+    // of 64 prompts 143, 117 and 140; 128 requests 132, 105 and 126; 4,096
+    // items, 512 tokens of four prompts: 330, 306 and 305).
+    attend_tiles(g, g.gt > 8 ? 2 * cus : cus / 4, (a.tokens + g.block - 1) / g.block);
     const int resident = by_sixteen(c) ? c.head_dim > 128 ? kResident<8, true> : kResident<4, true>
                                        : c.head_dim > 128 ? kResident<8, false> : kResident<4, false>;
     *groups = attend_groups(g, (int64_t)cus * resident, g.block);
