@@ -17,12 +17,9 @@
 //           (the matrix units take them exactly; the query's elements beside
 //           the latter are divided by 16).  A step is 32 elements, so a group
 //           is a whole number of steps and has its own accumulator.
-//   values  O[d] = sum_j (p_j scale_j) (u_j - 8) + sum_j p_j (low_j + 8
-//           scale_j).  A lane loads its unit of eight keys; v_perm_b32 pairs
-//           the bytes of two keys, masks make subnormal numbers of them as
-//           above, and one packed subtraction (u - 8) 2^-24 and 16 times it:
-//           codes about zero, so that the sums are no larger than what they
-//           are to give.
+//   values  O[d] = sum_j (p_j scale_j) u_j + sum_j p_j low_j.  A lane loads
+//           its unit of eight keys; v_perm_b32 pairs the bytes of two keys,
+//           and masks make subnormal numbers of them as above.
 //           The weights p scale enter as two FP16 parts, 2^-24 of the weight
 //           or 2^-39 of the largest of their column: the running maximum is
 //           that of score + exponent of the key's largest scale, so that
@@ -266,7 +263,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         const uint32_t key_first = (uint32_t)k.tile0 * kTile;
 
         f32x4 o[2 * W];
-        float m = -__builtin_inff(), l = 0.f, lows[NG];  // lows: sum p (low + 8 scale)
+        float m = -__builtin_inff(), l = 0.f, lows[NG];  // lows: sum p low
 #pragma unroll
         for (int e = 0; e < 2 * W; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -559,9 +556,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 #pragma unroll
                 for (int tau = 0; tau < 2; tau++) {
                     const f16x2 v = __builtin_bit_cast(f16x2, vp[tau][C]);
-                    const float scale = (float)v[0];
-                    sc[tau] = scale * 0x1p14f;  // (held so, as FP16)
-                    lo[tau] = fmaf(scale, 8.f, (float)v[1]);
+                    sc[tau] = (float)v[0] * 0x1p14f;  // (held so, as FP16)
+                    lo[tau] = (float)v[1];
                 }
                 float weight[8], sum = 0.f;
                 add_from_quads(sum, lo[0], lo[1], x);
@@ -604,10 +600,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                             const uint32_t w2[2] = {W == 3 ? vc[s][2 * i][B / 4] >> v_shift : vc[s][2 * i][B / 4],
                                                     W == 3 ? vc[s][2 * i + 1][B / 4] >> v_shift : vc[s][2 * i + 1][B / 4]};
                             const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
-                            const f16x2 e = __builtin_bit_cast(f16x2, y & 0x000f000fu) - f16x2{(f16)0x8p-24f, (f16)0x8p-24f};
-                            const f16x2 h = __builtin_bit_cast(f16x2, y & 0x00f000f0u) - f16x2{(f16)0x80p-24f, (f16)0x80p-24f};
-                            even[i] = __builtin_bit_cast(uint32_t, e);
-                            odd[i] = __builtin_bit_cast(uint32_t, h);
+                            even[i] = y & 0x000f000fu;
+                            odd[i] = y & 0x00f000f0u;
                         }
 #pragma unroll
                         for (int z = 0; z < 2; z++) {
