@@ -486,7 +486,8 @@ typedef struct {
 int orth_cache_append_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_append_t *append, int32_t dtype,
                                void *stream);
 
-/* The vectors of `count` slots, low + u * scale in FP32 rounded to `dtype`:
+/* The vectors of `count` slots, low + u * scale rounded to `dtype` (to FP16
+ * once, to BF16 from FP32):
  * k_out[i, h] and v_out[i, h] from slot slots[i], zeros where it lies outside
  * the cache.  Strides are [slot, head] of the outputs, 16-byte aligned
  * pointers with strides that are multiples of 8 or any others. */

@@ -445,31 +445,21 @@ hipError_t launch_cache_read4(const orth_hip_int4_cache_t &c, const orth_hip_rea
     // takes several (six requests' keys and values, 260 MB: 69 us with one
     // round, 61 with four, 57 with eight and with a slot a turn)
     const int64_t rounds = (r.count + g.at_once - 1) / g.at_once, fill = (int64_t)cus * 8 * 8 / (2 * parts) + 1;
-    const int64_t turns = (rounds + fill - 1) / fill;
-    g.per_group = (int)(g.at_once * (turns < 1 ? 1 : turns > 1 << 16 ? 1 << 16 : turns));
-    const int64_t groups = kLaunch / parts, slots = groups * g.per_group;  // of a launch
-    for (int64_t i = 0; i < r.count; i += slots) {
-        const int64_t rest = (r.count - i + g.per_group - 1) / g.per_group;
-        const dim3 grid((unsigned)((rest < groups ? rest : groups) * parts), 2);
-        auto go = [&](auto unit, auto uni) {
-            constexpr int U = decltype(unit)::value;
-            constexpr bool S = decltype(uni)::value != 0;
-            if (dtype == ORTH_DT_BF16) cache_read4_kernel<U, true, S><<<grid, 256, 0, stream>>>(g);
-            else cache_read4_kernel<U, false, S><<<grid, 256, 0, stream>>>(g);
-        };
-        auto by = [&](auto unit) { each % 64 == 0 ? go(unit, Int<1>()) : go(unit, Int<0>()); };
-        if (W == 2) by(Int<2>());
-        else if (W == 3) by(Int<3>());
-        else if (W == 4) by(Int<4>());
-        else by(Int<8>());
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        g.r.slots += slots;
-        g.r.count -= slots;
-        g.r.k_out = (uint16_t *)g.r.k_out + slots * r.k_strides[0];
-        g.r.v_out = (uint16_t *)g.r.v_out + slots * r.v_strides[0];
-    }
-    return hipSuccess;
+    const int64_t turns = (rounds + fill - 1) / fill, groups = (rounds + turns - 1) / turns;
+    g.per_group = (int)(g.at_once * turns);          // (fill is 1 only where at_once is: no more than the slots)
+    const dim3 grid((unsigned)(groups * parts), 2);  // (one launch: no more than 2^20 parts)
+    auto go = [&](auto unit, auto uni) {
+        constexpr int U = decltype(unit)::value;
+        constexpr bool S = decltype(uni)::value != 0;
+        if (dtype == ORTH_DT_BF16) cache_read4_kernel<U, true, S><<<grid, 256, 0, stream>>>(g);
+        else cache_read4_kernel<U, false, S><<<grid, 256, 0, stream>>>(g);
+    };
+    auto by = [&](auto unit) { each % 64 == 0 ? go(unit, Int<1>()) : go(unit, Int<0>()); };
+    if (W == 2) by(Int<2>());
+    else if (W == 3) by(Int<3>());
+    else if (W == 4) by(Int<4>());
+    else by(Int<8>());
+    return hipGetLastError();
 }
 
 }  // namespace orth
