@@ -471,6 +471,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             }
         }
         for (; pass < pass_end; pass += step) {
+            if (g.nsub == 1) __builtin_amdgcn_s_barrier();
             taken++;
             if (taken == quarter) __builtin_amdgcn_s_setprio(2);
             else if (taken == 2 * quarter) __builtin_amdgcn_s_setprio(1);
