@@ -276,6 +276,11 @@ __device__ __forceinline__ bool unseen(float top, float sum) {
     else return top == -__builtin_inff();
 }
 
+// Where a piece's row of D elements holds the pair from element e: the first
+// pairs of every eight elements, then the second ones, so that the threads of
+// a row, eight elements each, write whole lines through.
+__device__ __forceinline__ int pair_at(int D, int e) { return (e & 7) / 2 * (D / 4) + e / 8 * 2; }
+
 // Joins the waves' sums of an item, which lie in LDS (o: for each wave, every
 // wave_floats, gt rows of row_floats, and (m, l) [waves][16]): units unit .. unit + n - 1 of it, which
 // are written if they are all, else left as a piece, joined by the workgroup
@@ -321,9 +326,9 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
             }
         } else {
             const int64_t piece = (int64_t)slot * g.nh + hh;
-            float *dst = g.part + (piece * gt + h) * D + d;
+            float *dst = g.part + (piece * gt + h) * D;
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) store_shared(dst + i, r[i], r[i + 1]);
+            for (int i = 0; i < 8; i += 2) store_shared(dst + pair_at(D, d + i), r[i], r[i + 1]);
             if (d == 0) store_shared(&g.stat[piece * 16 + h].x, top, sum);
         }
     }
@@ -360,10 +365,10 @@ __device__ __forceinline__ void finish_item(const G &g, int tid, const float *ld
             for (int u = 0; u < 4; u++) {
                 const int i = i0 + u < to ? i0 + u : to;
                 const int64_t piece = (int64_t)(i == from ? slot0 : 2 * i) * g.nh + hh;
-                const float *src = g.part + (piece * gt + h) * D + e4;
+                const float *src = g.part + (piece * gt + h) * D;
                 st[u] = load_shared(&g.stat[piece * 16 + h].x);
-                v[u][0] = load_shared(src);
-                v[u][1] = load_shared(src + 2);
+                v[u][0] = load_shared(src + pair_at(D, e4));
+                v[u][1] = load_shared(src + pair_at(D, e4 + 2));
             }
             float most = top;
 #pragma unroll
@@ -433,7 +438,10 @@ __global__ __launch_bounds__(256) void join_kernel(G g) {
 #pragma unroll
                 for (int u = 0; u < 8; u++) {
                     const int x = i + u * at_once < m ? i + u * at_once : i;
-                    v[u] = *reinterpret_cast<const f32x4 *>(g.part + (piece(i0 + x) * g.gt + h) * D + 4 * q);
+                    const float *src = g.part + (piece(i0 + x) * g.gt + h) * D;
+                    const float2 a = *reinterpret_cast<const float2 *>(src + pair_at(D, 4 * q));
+                    const float2 b = *reinterpret_cast<const float2 *>(src + pair_at(D, 4 * q + 2));
+                    v[u] = f32x4{a.x, a.y, b.x, b.y};
                 }
 #pragma unroll
                 for (int u = 0; u < 8; u++) {
