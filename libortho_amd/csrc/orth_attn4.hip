@@ -92,11 +92,6 @@ __device__ __forceinline__ float sum_from_quad(float v, float x, float y) {
     const float z = from_quad<I>(v) * x;
     return z + y;
 }
-// The value of the lane whose column is eight further.
-__device__ __forceinline__ float other_half(float v) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true));
-}
-
 // w - part[H].
 template <int H>
 __device__ __forceinline__ float rest(float w, f16x2 part) {
@@ -175,16 +170,12 @@ constexpr int kResident = W > 4 ? (PG16 ? 2 : 1) : 3;
 // PG16: page_size is a multiple of 16, so 16 keys from a multiple of 16 lie in
 // one page: a scalar table entry and scalar addresses serve them, and lanes
 // add offsets that stay the same for the whole item.
-// SETS = 2: no more than eight columns are used, so the other eight take a
-// second tile of keys, and one softmax serves both: the query's columns, and
-// later the weights', are masked to the tile's half, whose sums stay apart
-// until the item ends.
-template <int W, int GS, bool PG16, int SETS>
+template <int W, int GS, bool PG16>
 __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Attend4Args g) {
     constexpr int NG = W / GS, VD = (W + 3) / 4;
     constexpr int row_floats = 32 * W + 4;
     // o [waves][gt][32 W + 4], in its place before, for each wave, its queries as
-    // the products take them, then (m, l) [waves][16]; all start at 16 bytes, and
+    // the products take them, and (m, l) [waves][16]; all start at 16 bytes, and
     // so does each row of o
     extern __shared__ __align__(16) float lds[];
     float2 *lds_stat = reinterpret_cast<float2 *>(lds + kWaves * g.wave_floats);
@@ -210,19 +201,18 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
     // between 116 and 274 us): a wave that is through a quarter of its share
     // gives way to those that are not (128 requests: 264 -> 258 us, 128 tokens
     // of four prompts 104 -> 99).
-    const uint32_t quarter = (uint32_t)(stop - first) * (kPair / SETS) / 4 + 1;
+    const uint32_t quarter = (uint32_t)(stop - first) * kPair / 4 + 1;
     uint32_t taken = 0;
     __builtin_amdgcn_s_setprio(3);
     while (cur < stop) {
         // (the empty asm: nothing that follows from the lane is kept in registers
         // from one item to the next)
         asm volatile("" : "+v"(lane));
-        // columns: queries (SETS = 2: `col` of half `set`)
-        const int set = SETS == 2 ? lane >> 3 & 1 : 0, col16 = lane & 15, col = SETS == 2 ? lane & 7 : col16, lg = lane >> 4;
+        const int col = lane & 15, lg = lane >> 4;  // columns: queries
         const bool q8 = ((reinterpret_cast<uintptr_t>(g.a.q) | (uintptr_t)(g.a.q_strides[0] * 2) | (uintptr_t)(g.a.q_strides[1] * 2)) & 7) == 0;
         const bool o16 = ((reinterpret_cast<uintptr_t>(g.a.out) | (uintptr_t)(g.a.out_strides[0] * 2) | (uintptr_t)(g.a.out_strides[1] * 2)) & 15) == 0;
         // (W == 3: the last unit is read from a byte earlier, so that its word ends with the row)
-        const int v_at = W == 3 && col16 == 15 ? 44 : W * col16, v_shift = W == 3 && col16 == 15 ? 8 : 0;
+        const int v_at = W == 3 && col == 15 ? 44 : W * col, v_shift = W == 3 && col == 15 ? 8 : 0;
 
         const uint64_t left = stop - cur;
         const uint32_t n = k.units - unit < left ? k.units - unit : (uint32_t)left;
@@ -230,9 +220,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         const int cols = tokens > 1 ? tokens * g.group : g.group - gt0 < 16 ? g.group - gt0 : 16;
         const int64_t row = g.a.rows ? (int64_t)__builtin_amdgcn_readfirstlane(g.a.rows[t]) : t;
 
-        const uint32_t first_half = set ? 0u : ~0u;
         // this column's query, and the keys its token sees
-        u32x4 *const q = reinterpret_cast<u32x4 *>(lds + wave * g.wave_floats);  // [W][lanes], then zeros
+        u32x4 *const q = reinterpret_cast<u32x4 *>(lds + wave * g.wave_floats);  // [W][lanes]
         const int j = tokens > 1 && col < cols ? col / g.group : 0;
         uint2 raw[W][2];  // elements 32 s + 16 h + 4 lg .. + 3
         {
@@ -265,9 +254,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         const int last = k.end - 1;
         const uint64_t upto = (uint64_t)(unit + n) * (kPair * g.nsub);
         const int tiles = (int)(upto < (uint64_t)k.tiles ? upto : (uint64_t)k.tiles);
-        // a wave's passes of SETS tiles
-        const int step = g.nsub, pass_end = (tiles + SETS - 1) / SETS;
-        int pass = (int)unit * (kPair / SETS * g.nsub) + sub;
+        const int step = g.nsub;
+        int pass = (int)unit * (kPair * g.nsub) + sub;
         const uint32_t key_first = (uint32_t)k.tile0 * kTile;
 
         f32x4 o[2 * W];
@@ -278,11 +266,11 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         for (int i = 0; i < NG; i++) lows[i] = 0.f;
 
         // what a wave holds of a pass until it is taken
-        uint32_t kc[SETS][2][W];   // units 4 lg .. of keys 32 set + 16 tau + col16
-        uint32_t vc[SETS][8][VD];  // unit col16 of keys 32 set + 16 tau + 4 lg + i, as 4 tau + i
-        uint32_t kp[2][NG], vp[2][NG];  // (scale, low) of key and value 32 set + 16 tau + 4 lg + lane % 4
+        uint32_t kc[2][W];   // units 4 lg .. of keys 16 tau + col
+        uint32_t vc[8][VD];  // unit col of keys 16 tau + 4 lg + i, as 4 tau + i
+        uint32_t kp[2][NG], vp[2][NG];  // (scale, low) of key and value 16 tau + 4 lg + lane % 4
         uint32_t seen8 = 0xff;     // which of this column's eight keys lie in a page of the cache
-        int32_t page[SETS][2];     // with PG16: the pages of the next pass to load
+        int32_t page[2];           // with PG16: the pages of the next pass to load
 
         // keys past the last are taken as the last (with PG16 the first key of
         // sixteen stands for all: they lie in its page also where the last key
@@ -294,18 +282,16 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             return key - quotient(key, g.page) * g.page.d;
         };
         auto known = [&](int32_t pg) -> int64_t { return (uint32_t)pg < (uint64_t)g.c.pages ? (int64_t)pg : 0; };
-        auto key_of = [&](int ps, int s, int tau) -> uint32_t { return key_first + (uint32_t)ps * (kTile * SETS) + kTile * s + 16 * tau; };
+        auto key_of = [&](int ps, int tau) -> uint32_t { return key_first + (uint32_t)ps * kTile + 16 * tau; };
         auto load_entries = [&](int ps) {
             if constexpr (PG16) {
 #pragma unroll
-                for (int s = 0; s < SETS; s++)
-#pragma unroll
-                    for (int tau = 0; tau < 2; tau++) page[s][tau] = entry(key_of(ps, s, tau));
+                for (int tau = 0; tau < 2; tau++) page[tau] = entry(key_of(ps, tau));
             }
         };
         // (with PG16 strides are those of the keys and the values, and 32-bit)
         const uint32_t slot = (uint32_t)g.c.k_code_strides[1], scale_slot = (uint32_t)g.c.k_scale_strides[1] * 2;
-        const uint32_t k_at = (uint32_t)col16 * slot + lg * 4 * W, v_first = 4 * lg * slot + v_at;
+        const uint32_t k_at = (uint32_t)col * slot + lg * 4 * W, v_first = 4 * lg * slot + v_at;
         const uint32_t s_at = (4 * lg + (lane & 3)) * scale_slot;
         auto code_place = [&](uint32_t key, int32_t pg) -> uint64_t {
             return (uint64_t)(uint32_t)known(pg) * (uint32_t)g.c.k_code_strides[0] + inside(key) * slot;
@@ -315,17 +301,15 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         };
         auto load_k = [&](int ps) {
 #pragma unroll
-            for (int s = 0; s < SETS; s++)
-#pragma unroll
-                for (int tau = 0; tau < 2; tau++) {
-                    const uint32_t key = key_of(ps, s, tau);
-                    if constexpr (PG16) {
-                        load_from<W>(kc[s][tau], kbase + code_place(key, page[s][tau]), k_at, 0);
-                    } else {
-                        const uint32_t x = key + col16;
-                        load_words<W>(kc[s][tau], kbase + known(entry(x)) * g.c.k_code_strides[0] + (int64_t)inside(x) * g.c.k_code_strides[1] + lg * 4 * W);
-                    }
+            for (int tau = 0; tau < 2; tau++) {
+                const uint32_t key = key_of(ps, tau);
+                if constexpr (PG16) {
+                    load_from<W>(kc[tau], kbase + code_place(key, page[tau]), k_at, 0);
+                } else {
+                    const uint32_t x = key + col;
+                    load_words<W>(kc[tau], kbase + known(entry(x)) * g.c.k_code_strides[0] + (int64_t)inside(x) * g.c.k_code_strides[1] + lg * 4 * W);
                 }
+            }
         };
         auto load_pairs = [&](uint32_t *pair, const uint8_t *p) {
             if constexpr (W == 8) {  // (only vectors past 128 elements may have fewer groups than steps)
@@ -339,16 +323,11 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 #pragma unroll
             for (int tau = 0; tau < 2; tau++) {
                 if constexpr (PG16) {
-                    uint64_t at = scale_place(key_of(ps, 0, tau), page[0][tau]);
-                    if constexpr (SETS == 2) {
-                        const uint64_t at1 = scale_place(key_of(ps, 1, tau), page[1][tau]);
-                        at = set ? at1 : at;
-                    }
-                    at += s_at;
+                    const uint64_t at = scale_place(key_of(ps, tau), page[tau]) + s_at;
                     load_pairs(kp[tau], ksbase + at);
                     load_pairs(vp[tau], vsbase + at);
                 } else {
-                    const uint32_t x = key_of(ps, 0, tau) + 4 * lg + (lane & 3);
+                    const uint32_t x = key_of(ps, tau) + 4 * lg + (lane & 3);
                     const int64_t pg = known(entry(x)), in = inside(x);
                     load_pairs(kp[tau], ksbase + 2 * (pg * g.c.k_scale_strides[0] + in * g.c.k_scale_strides[1]));
                     load_pairs(vp[tau], vsbase + 2 * (pg * g.c.v_scale_strides[0] + in * g.c.v_scale_strides[1]));
@@ -356,38 +335,36 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             }
             seen8 = 0;
 #pragma unroll
-            for (int s = 0; s < SETS; s++)
+            for (int tau = 0; tau < 2; tau++) {
+                const uint32_t key = key_of(ps, tau);
+                const uint8_t *p = vbase;
+                if constexpr (PG16) {
+                    p += code_place(key, page[tau]);
+                    if ((uint32_t)page[tau] < (uint64_t)g.c.pages) seen8 |= 0xfu << 4 * tau;
+                }
 #pragma unroll
-                for (int tau = 0; tau < 2; tau++) {
-                    const uint32_t key = key_of(ps, s, tau);
-                    const uint8_t *p = vbase;
-                    if constexpr (PG16) {
-                        p += code_place(key, page[s][tau]);
-                        if ((uint32_t)page[s][tau] < (uint64_t)g.c.pages) seen8 |= 0xfu << (4 * tau + 8 * s);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t *dst = vc[s][4 * tau + i];
-                        if constexpr (PG16 && W != 3) {
-                            if constexpr (W == 2) dst[0] = load_half_from(p, v_first, i * slot);
-                            else load_from<VD>(dst, p, v_first, i * slot);
-                        } else {
-                            const uint8_t *x = p + (v_first + i * slot);
-                            if constexpr (!PG16) {
-                                const uint32_t y = key + 4 * lg + i;
-                                const int32_t pg = entry(y);
-                                x = p + known(pg) * g.c.v_code_strides[0] + (int64_t)inside(y) * g.c.v_code_strides[1] + v_at;
-                                seen8 |= (uint32_t)((uint32_t)pg < (uint64_t)g.c.pages) << (4 * tau + i);
-                            }
-                            if constexpr (W == 2) dst[0] = *reinterpret_cast<const uint16_t *>(x);
-                            else if constexpr (W == 3) __builtin_memcpy(dst, x, 4);
-                            else load_words<VD>(dst, x);
+                for (int i = 0; i < 4; i++) {
+                    uint32_t *dst = vc[4 * tau + i];
+                    if constexpr (PG16 && W != 3) {
+                        if constexpr (W == 2) dst[0] = load_half_from(p, v_first, i * slot);
+                        else load_from<VD>(dst, p, v_first, i * slot);
+                    } else {
+                        const uint8_t *x = p + (v_first + i * slot);
+                        if constexpr (!PG16) {
+                            const uint32_t y = key + 4 * lg + i;
+                            const int32_t pg = entry(y);
+                            x = p + known(pg) * g.c.v_code_strides[0] + (int64_t)inside(y) * g.c.v_code_strides[1] + v_at;
+                            seen8 |= (uint32_t)((uint32_t)pg < (uint64_t)g.c.pages) << (4 * tau + i);
                         }
+                        if constexpr (W == 2) dst[0] = *reinterpret_cast<const uint16_t *>(x);
+                        else if constexpr (W == 3) __builtin_memcpy(dst, x, 4);
+                        else load_words<VD>(dst, x);
                     }
                 }
+            }
         };
 
-        if (pass < pass_end) {
+        if (pass < tiles) {
             load_entries(pass);
             load_k(pass);
             load_v(pass);
@@ -444,7 +421,6 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 }
                 q[64 * s + lane] = v;
             }
-            if (SETS == 2 && lane == 0) q[64 * W] = u32x4{0u, 0u, 0u, 0u};
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
             for (int i = 0; i < NG; i++) {
@@ -470,13 +446,13 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 least_end = __builtin_amdgcn_readfirstlane(least_end);
             }
         }
-        for (; pass < pass_end; pass += step) {
+        for (; pass < tiles; pass += step) {
             if (g.nsub == 1) __builtin_amdgcn_s_barrier();
             taken++;
             if (taken == quarter) __builtin_amdgcn_s_setprio(2);
             else if (taken == 2 * quarter) __builtin_amdgcn_s_setprio(1);
             else if (taken == 3 * quarter) __builtin_amdgcn_s_setprio(0);
-            // scores: lane (col, lg) of half `set` gets those of its eight keys
+            // scores: lane (col, lg) gets those of its eight keys
             float x[8], offset[8];
             each<NG>([&](auto group) {
                 constexpr int C = group.value;
@@ -485,14 +461,11 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 for (int tau = 0; tau < 2; tau++) acc[tau] = f32x4{0.f, 0.f, 0.f, 0.f};
                 each<GS>([&](auto b) {
                     constexpr int B = C * GS + b.value;
+                    const u32x4 qb = q[64 * B + lane];
 #pragma unroll
-                    for (int s = 0; s < SETS; s++) {
-                        const u32x4 qm = q[SETS == 1 || set == s ? 64 * B + lane : 64 * W];
-#pragma unroll
-                        for (int tau = 0; tau < 2; tau++) {
-                            const uint32_t y = two_bytes<B, W + B>(kc[s][tau]), z = two_bytes<2 * W + B, 3 * W + B>(kc[s][tau]);
-                            acc[tau] = mfma16(u32x4{y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u}, qm, acc[tau]);
-                        }
+                    for (int tau = 0; tau < 2; tau++) {
+                        const uint32_t y = two_bytes<B, W + B>(kc[tau]), z = two_bytes<2 * W + B, 3 * W + B>(kc[tau]);
+                        acc[tau] = mfma16(u32x4{y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u}, qb, acc[tau]);
                     }
                 });
                 float sc[2], lo[2];
@@ -519,18 +492,17 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = fmaf(unscale, x[i], offset[i]);
 
-            const int key0 = (int)key_of(pass, 0, 0);
-            const bool masked = (key0 < most_begin) | (key0 > least_end - kTile * SETS) | !__all(seen8 == (SETS == 2 ? 0xffffu : 0xffu));
+            const int key0 = (int)key_of(pass, 0);
+            const bool masked = (key0 < most_begin) | (key0 > least_end - kTile) | !__all(seen8 == 0xffu);
             uint32_t in8 = 0xff;  // which of the lane's keys its column sees
             if (masked) {
                 asm volatile("");  // (a branch: passes at the ends of a range are few)
                 in8 = 0;
-                const int mine = key0 + kTile * set + 4 * lg;
-                const uint32_t paged = seen8 >> 8 * set;
+                const int mine = key0 + 4 * lg;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int key = mine + 16 * (i >> 2) + (i & 3);
-                    const bool in = key >= begin && key < end && (paged >> i & 1) != 0;
+                    const bool in = key >= begin && key < end && (seen8 >> i & 1) != 0;
                     in8 |= (uint32_t)in << i;
                     if (!in) x[i] = -__builtin_inff();
                 }
@@ -597,32 +569,23 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                     part[0][i] = __builtin_bit_cast(uint32_t, big);
                     part[1][i] = __builtin_bit_cast(uint32_t, small);
                 }
+                each<GS>([&](auto b) {
+                    constexpr int B = C * GS + b.value;
+                    u32x4 even, odd;  // elements 32 B + col and 16 on of the lane's eight keys
 #pragma unroll
-                for (int s = 0; s < SETS; s++) {
-                    u32x4 pm[2] = {part[0], part[1]};
-                    if constexpr (SETS == 2)
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t w2[2] = {W == 3 ? vc[2 * i][B / 4] >> v_shift : vc[2 * i][B / 4],
+                                                W == 3 ? vc[2 * i + 1][B / 4] >> v_shift : vc[2 * i + 1][B / 4]};
+                        const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
+                        even[i] = y & 0x000f000fu;
+                        odd[i] = y & 0x00f000f0u;
+                    }
 #pragma unroll
-                        for (int z = 0; z < 2; z++)
-#pragma unroll
-                            for (int c = 0; c < 4; c++) pm[z][c] &= s ? ~first_half : first_half;
-                    each<GS>([&](auto b) {
-                        constexpr int B = C * GS + b.value;
-                        u32x4 even, odd;  // elements 32 B + col16 and 16 on of the lane's eight keys
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t w2[2] = {W == 3 ? vc[s][2 * i][B / 4] >> v_shift : vc[s][2 * i][B / 4],
-                                                    W == 3 ? vc[s][2 * i + 1][B / 4] >> v_shift : vc[s][2 * i + 1][B / 4]};
-                            const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
-                            even[i] = y & 0x000f000fu;
-                            odd[i] = y & 0x00f000f0u;
-                        }
-#pragma unroll
-                        for (int z = 0; z < 2; z++) {
-                            o[2 * B] = mfma16(even, pm[z], o[2 * B]);
-                            o[2 * B + 1] = mfma16(odd, pm[z], o[2 * B + 1]);
-                        }
-                    });
-                }
+                    for (int z = 0; z < 2; z++) {
+                        o[2 * B] = mfma16(even, part[z], o[2 * B]);
+                        o[2 * B + 1] = mfma16(odd, part[z], o[2 * B + 1]);
+                    }
+                });
             });
             __builtin_amdgcn_sched_barrier(0);
             load_v(pass + step);
@@ -630,30 +593,11 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        if constexpr (SETS == 2) {  // the halves' sums together
-            const float top = fmaxf(m, other_half(m)), base = top == -__builtin_inff() ? 0.f : top;
-            const float keep = __builtin_amdgcn_exp2f(m - base);
-            l *= keep;
-            l += other_half(l);
-#pragma unroll
-            for (int i = 0; i < NG; i++) {
-                lows[i] *= keep;
-                lows[i] += other_half(lows[i]);
-            }
-#pragma unroll
-            for (int e = 0; e < 2 * W; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    o[e][i] *= keep;
-                    o[e][i] += other_half(o[e][i]);
-                }
-            m = top;
-        }
         // join the waves of each head tile
         l = column_sum(l);
 #pragma unroll
         for (int i = 0; i < NG; i++) lows[i] = column_sum(lows[i]);
-        if (col < cols && set == 0) {
+        if (col < cols) {
             float *dst = lds + wave * g.wave_floats + col * row_floats + 4 * lg;
 #pragma unroll
             for (int e = 0; e < 2 * W; e++) {
@@ -696,8 +640,7 @@ Attend4Args attend4_args(const orth_hip_int4_cache_t &c, const orth_hip_attend_t
     g.gtiles = (g.group + 15) / 16;
     g.groups = c.head_dim / c.group_size;
     // Neighbouring tokens share a product where some request must have several:
-    // more tokens than requests.  (Else the columns are those of one token, and
-    // with eight or fewer of them two tiles of keys share one.)
+    // more tokens than requests.
     g.block = 1;
     if (a.rows && a.tokens > a.table_rows)
         while (2 * g.block * g.group <= 16) g.block *= 2;
@@ -732,7 +675,7 @@ hipError_t launch_paged_attention4(const orth_hip_int4_cache_t &c, const orth_hi
     g.bf = dtype == ORTH_DT_BF16;
     const hipError_t e = by_int4_layout(c, [&](auto unit, auto steps) -> hipError_t {
         constexpr int W = decltype(unit)::value, GS = decltype(steps)::value;
-        const int rows = g.gt * (32 * W + 4), queries = 256 * W + 4;
+        const int rows = g.gt * (32 * W + 4), queries = 256 * W;
         g.wave_floats = rows > queries ? rows : queries;
         const size_t lds = (size_t)kWaves * g.wave_floats * 4 + kWaves * 16 * sizeof(float2);
         auto go = [&](auto kernel) -> hipError_t {
@@ -744,8 +687,7 @@ hipError_t launch_paged_attention4(const orth_hip_int4_cache_t &c, const orth_hi
             kernel<<<dim3((unsigned)groups), 256, lds, stream>>>(g);
             return hipGetLastError();
         };
-        if (!by_sixteen(c)) return go(attend4_kernel<W, GS, false, 1>);
-        return g.gt <= 8 && W <= 4 ? go(attend4_kernel<W, GS, true, W <= 4 ? 2 : 1>) : go(attend4_kernel<W, GS, true, 1>);
+        return by_sixteen(c) ? go(attend4_kernel<W, GS, true>) : go(attend4_kernel<W, GS, false>);
     });
     if (e != hipSuccess) return e;
     return attend_joins(g, groups, g.block) ? launch_join(g, groups, stream) : hipSuccess;
