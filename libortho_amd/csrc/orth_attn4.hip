@@ -27,8 +27,19 @@
 //
 // Queries are multiplied by the power of two that brings their largest element
 // to 2^14 and beyond, so that BF16 ones fit FP16.  Scale and low of the tile's
-// keys and values are held by one lane each (16 lanes of a group: eight keys,
-// eight values) and broadcast within the row of 16 lanes by DPP.
+// keys and values are held by four lanes of a score's column each, two keys and
+// two values a lane, and broadcast within quads of lanes by DPP.
+//
+// Bound by memory and instructions about equally where there are many keys
+// (128 requests of 2,048 to 16,384 keys, 8 of 64 heads, 943 MB: 232 us, 4.1
+// TB/s).  A head's row of a slot is half a line of 128 bytes, so the waves of
+// neighbouring heads keep step (a barrier a tile) and find each other's lines
+// in the L1 (without: 258 us, 1,258 MB read; 1,088 with it, the rest (scale,
+// low) pairs whose lines hold the heads of two workgroups).  Few keys: a chain
+// of latencies (190 keys, 32 heads: 13 us).
+// Two tiles of keys in one product where no more than eight columns are used,
+// and one softmax for both, was 2% faster at the largest call and up to 15%
+// slower at the others; four workgroups a CU 3% slower than three.
 #include "orth_attend.h"
 #include "orth_serve4.h"
 
@@ -447,7 +458,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             }
         }
         for (; pass < tiles; pass += step) {
-            if (g.nsub == 1) __builtin_amdgcn_s_barrier();
+            if (g.nsub == 1) __builtin_amdgcn_s_barrier();  // (each wave has a head, and all the same tiles)
             taken++;
             if (taken == quarter) __builtin_amdgcn_s_setprio(2);
             else if (taken == 2 * quarter) __builtin_amdgcn_s_setprio(1);
