@@ -23,9 +23,10 @@ constexpr int64_t kLaunch = 1 << 23;  // workgroups of 256 along x (2^32 threads
 // and 64 bits those (one key in some 800, one code in some 30,000).
 //
 // An element is read once and, of keys and values, a quarter of it written;
-// bound by instructions (2,048 tokens, 32 + 8 heads of 128: 45 MB in 15.3 us,
-// 2.9 TB/s; written and read back 19 us, and 24 while what only numbers next
-// to a border need was worked out beforehand, in 95 registers instead of 63).
+// bound by memory where there are many tokens (32 + 8 heads of 128: 8,192
+// tokens in 46 us, 3.9 TB/s; 2,048 in 14.5 to 15.3, 3 TB/s, and 5 more while
+// what only numbers next to a border need was worked out beforehand, in 95
+// registers instead of 63).
 struct Append4Args {
     orth_hip_int4_cache_t c;
     orth_hip_append_t a;
@@ -403,7 +404,8 @@ hipError_t launch_cache_append4(const orth_hip_int4_cache_t &c, const orth_hip_a
     const bool plain = g.vec && (a.interleaved ? g.a.rot % 8 == 0 : g.a.rot % 16 == 0);
     const int64_t heads = (a.q ? (int64_t)a.q_heads : 0) + 2 * (int64_t)c.kv_heads, parts = (heads + vecs - 1) / vecs;
     // a workgroup for every 16 (or 8) vectors where tokens alone leave CUs
-    // idle, else one a token
+    // idle, else one a token (32 + 8 heads of 128, three a token and one: 64
+    // tokens 5.5 and 6.3 us, 512 6.7 and 6.9, 700 8.6 and 7.9, 8,192 64 and 46)
     const int y = a.tokens >= 2 * cus ? 1 : (int)(parts < 65535 ? parts : 65535);
     for (int64_t t = 0; t < a.tokens; t += kLaunch) {
         const dim3 grid((unsigned)(a.tokens - t < kLaunch ? a.tokens - t : kLaunch), (unsigned)y);
