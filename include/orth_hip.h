@@ -490,7 +490,8 @@ int orth_cache_append_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hi
  * once, to BF16 from FP32):
  * k_out[i, h] and v_out[i, h] from slot slots[i], zeros where it lies outside
  * the cache.  Strides are [slot, head] of the outputs, 16-byte aligned
- * pointers with strides that are multiples of 8 or any others. */
+ * pointers with strides that are multiples of 8 or any others; the two do not
+ * overlap. */
 typedef struct {
     void *k_out;                 /* [count, kv_heads, head_dim] */
     void *v_out;
