@@ -7,19 +7,20 @@
 // tokens of one request come together, those of up to 16 / heads neighbouring
 // tokens, each with its own range of keys.
 //
-// Keys and values are low + u * scale.  The codes u enter the products, exact
-// in FP16; scales and lows stay outside, in FP32:
+// Keys and values are low + u * scale = mid + c * scale with c = u - 8 and mid
+// = low + 8 scale: sums about the middle are no larger than what they give.
+// The c enter the products, exact in FP16; scales and mids stay outside, in
+// FP32:
 //
-//   scores  S[key] = scale2 (sum_g scale_g (q . u)_g + low_g sum_g q).  A lane
+//   scores  S[key] = scale2 (sum_g scale_g (q . c)_g + mid_g sum_g q).  A lane
 //           loads units 4 lg .. 4 lg + 3 of its key; byte b of them is step b
 //           of the product: one v_perm_b32 pairs the bytes of two units, two
-//           masks make their nibbles subnormal numbers u 2^-24 and 16 u 2^-24
-//           (the matrix units take them exactly; the query's elements beside
-//           the latter are divided by 16).  A step is 32 elements, so a group
-//           is a whole number of steps and has its own accumulator.
-//   values  O[d] = sum_j (p_j scale_j) u_j + sum_j p_j low_j.  A lane loads
+//           masks and two packed subtractions make their c of them.  A step is
+//           32 elements, so a group is a whole number of steps and has its own
+//           accumulator.
+//   values  O[d] = sum_j (p_j scale_j) c_j + sum_j p_j mid_j.  A lane loads
 //           its unit of eight keys; v_perm_b32 pairs the bytes of two keys,
-//           and masks make subnormal numbers of them as above.
+//           and their c are taken as above.
 //           The weights p scale enter as two FP16 parts, 2^-24 of the weight
 //           or 2^-39 of the largest of their column: the running maximum is
 //           that of score + exponent of the key's largest scale, so that
@@ -116,10 +117,26 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4 &a, const u32x4 &b, const f3
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Bytes A and B of the words that `w` holds, as 16-bit halves.
+// Bytes A and B of the words that `w` holds, below bits that are set.
 template <int A, int B>
 __device__ __forceinline__ uint32_t two_bytes(const uint32_t *w) {
-    return __builtin_amdgcn_perm(w[B / 4], w[A / 4], 0x0c000c00u | (A % 4) | (4 + B % 4) << 16);
+    return __builtin_amdgcn_perm(w[B / 4], w[A / 4], 0x0d000d00u | (A % 4) | (4 + B % 4) << 16);
+}
+// Their low and their high nibbles, less 8, as FP16 numbers: 1024 + u and
+// 64 + u with exponents left from the bits above, then less 1032 and 72, exactly.
+// (The nibbles alone are subnormal numbers, which the matrix units take as well
+// and which save the subtraction: 128 requests 231 us for 239, 128 tokens of
+// four prompts 95 for 103.  But a matrix product aligns what it sums by
+// exponents, a subnormal number's is that of 2^-14 whatever it is, and what
+// falls off below 24 bits of the largest is lost: sums came out 2^-17 of their
+// magnitude short.  Of 128 requests' 1,048,576 elements 8,493 were not the
+// rounded 64-bit ones, with u as normal numbers 1,010, with u - 8 108, and 113
+// where everything is FP32.)
+__device__ __forceinline__ uint32_t low_codes(uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, y & 0x640f640fu) - f16x2{(f16)1032.f, (f16)1032.f});
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, y & 0x54f054f0u) - f16x2{(f16)72.f, (f16)72.f});
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -270,11 +287,11 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         const uint32_t key_first = (uint32_t)k.tile0 * kTile;
 
         f32x4 o[2 * W];
-        float m = -__builtin_inff(), l = 0.f, lows[NG];  // lows: sum p low
+        float m = -__builtin_inff(), l = 0.f, mids[NG];  // mids: sum p mid
 #pragma unroll
         for (int e = 0; e < 2 * W; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < NG; i++) lows[i] = 0.f;
+        for (int i = 0; i < NG; i++) mids[i] = 0.f;
 
         // what a wave holds of a pass until it is taken
         uint32_t kc[2][W];   // units 4 lg .. of keys 16 tau + col
@@ -422,7 +439,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             for (int s = 0; s < W; s++) {
                 float y[8];
 #pragma unroll
-                for (int c = 0; c < 8; c++) y[c] = ldexpf(x[s][c], c < 4 ? up : up - 4);
+                for (int c = 0; c < 8; c++) y[c] = ldexpf(x[s][c], up);
                 u32x4 v;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -476,24 +493,24 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 #pragma unroll
                     for (int tau = 0; tau < 2; tau++) {
                         const uint32_t y = two_bytes<B, W + B>(kc[tau]), z = two_bytes<2 * W + B, 3 * W + B>(kc[tau]);
-                        acc[tau] = mfma16(u32x4{y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u}, qb, acc[tau]);
+                        acc[tau] = mfma16(u32x4{low_codes(y), high_codes(y), low_codes(z), high_codes(z)}, qb, acc[tau]);
                     }
                 });
-                float sc[2], lo[2];
+                float sc[2], mid[2];
 #pragma unroll
                 for (int tau = 0; tau < 2; tau++) {
                     const f16x2 v = __builtin_bit_cast(f16x2, kp[tau][C]);
-                    sc[tau] = (float)v[0] * 0x1p24f;  // (the codes' 2^-24)
-                    lo[tau] = (float)v[1];
+                    sc[tau] = (float)v[0];
+                    mid[tau] = fmaf((float)v[0], 8.f, (float)v[1]);
                 }
                 each<8>([&](auto i) {
                     constexpr int I = i.value, T = I >> 2;
                     if constexpr (C == 0) {
                         x[I] = from_quad<(I & 3)>(sc[T]) * acc[T][I & 3];
-                        offset[I] = from_quad<(I & 3)>(lo[T]) * qs[0];
+                        offset[I] = from_quad<(I & 3)>(mid[T]) * qs[0];
                     } else {
                         x[I] = sum_from_quad<(I & 3)>(sc[T], acc[T][I & 3], x[I]);
-                        add_from_quad<(I & 3)>(offset[I], lo[T], qs[C]);
+                        add_from_quad<(I & 3)>(offset[I], mid[T], qs[C]);
                     }
                 });
             });
@@ -534,7 +551,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 const float keep = __builtin_amdgcn_exp2f(m - top);
                 l *= keep;
 #pragma unroll
-                for (int i = 0; i < NG; i++) lows[i] *= keep;
+                for (int i = 0; i < NG; i++) mids[i] *= keep;
 #pragma unroll
                 for (int e = 0; e < 2 * W; e++)
 #pragma unroll
@@ -548,15 +565,15 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             }
             each<NG>([&](auto group) {
                 constexpr int C = group.value;
-                float sc[2], lo[2];
+                float sc[2], mid[2];
 #pragma unroll
                 for (int tau = 0; tau < 2; tau++) {
                     const f16x2 v = __builtin_bit_cast(f16x2, vp[tau][C]);
                     sc[tau] = (float)v[0] * 0x1p14f;  // (held so, as FP16)
-                    lo[tau] = (float)v[1];
+                    mid[tau] = fmaf((float)v[0], 8.f, (float)v[1]);
                 }
                 float weight[8], sum = 0.f;
-                add_from_quads(sum, lo[0], lo[1], x);
+                add_from_quads(sum, mid[0], mid[1], x);
                 each<8>([&](auto i) { weight[i.value] = from_quad<(i.value & 3)>(sc[i.value >> 2]) * x[i.value]; });
                 // (taken here, not once for each side of the branch, where they lose the broadcast that a product takes in)
                 asm volatile("" : "+v"(weight[0]), "+v"(weight[1]), "+v"(weight[2]), "+v"(weight[3]), "+v"(weight[4]),
@@ -566,12 +583,12 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                     sum = 0.f;
                     each<8>([&](auto i) {
                         const bool in = in8 >> i.value & 1;
-                        const float scale = from_quad<(i.value & 3)>(sc[i.value >> 2]), low = from_quad<(i.value & 3)>(lo[i.value >> 2]);
+                        const float scale = from_quad<(i.value & 3)>(sc[i.value >> 2]), middle = from_quad<(i.value & 3)>(mid[i.value >> 2]);
                         weight[i.value] = in ? scale * x[i.value] : 0.f;
-                        sum += in ? low * x[i.value] : 0.f;
+                        sum += in ? middle * x[i.value] : 0.f;
                     });
                 }
-                lows[C] += sum;
+                mids[C] += sum;
                 u32x4 part[2];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -588,8 +605,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                         const uint32_t w2[2] = {W == 3 ? vc[2 * i][B / 4] >> v_shift : vc[2 * i][B / 4],
                                                 W == 3 ? vc[2 * i + 1][B / 4] >> v_shift : vc[2 * i + 1][B / 4]};
                         const uint32_t y = two_bytes<B % 4, 4 + B % 4>(w2);
-                        even[i] = y & 0x000f000fu;
-                        odd[i] = y & 0x00f000f0u;
+                        even[i] = low_codes(y);
+                        odd[i] = high_codes(y);
                     }
 #pragma unroll
                     for (int z = 0; z < 2; z++) {
@@ -607,12 +624,13 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
         // join the waves of each head tile
         l = column_sum(l);
 #pragma unroll
-        for (int i = 0; i < NG; i++) lows[i] = column_sum(lows[i]);
+        for (int i = 0; i < NG; i++) mids[i] = column_sum(mids[i]);
         if (col < cols) {
             float *dst = lds + wave * g.wave_floats + col * row_floats + 4 * lg;
 #pragma unroll
             for (int e = 0; e < 2 * W; e++) {
-                const float f = e % 2 ? 0x1p6f : 0x1p10f, b = lows[e / (2 * GS)];
+                constexpr float f = 0x1p-14f;  // (the weights' 2^14)
+                const float b = mids[e / (2 * GS)];
                 *reinterpret_cast<f32x4 *>(dst + 16 * e) = f32x4{fmaf(o[e][0], f, b), fmaf(o[e][1], f, b), fmaf(o[e][2], f, b), fmaf(o[e][3], f, b)};
             }
             if (lg == 0) lds_stat[wave * 16 + col] = float2{m, l};
