@@ -504,7 +504,8 @@ int orth_cache_read_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_
 
 /* orth_paged_attention_hip over that cache, with the values low + u * scale as
  * keys and values; q and out hold `dtype`.  Queries enter in FP16 with a power
- * of two of their own vector (elements below 2^-39 of its largest lose bits).
+ * of two of their own vector: elements down to 2^-28 of its largest (of BF16
+ * ones 2^-31) keep all their bits, smaller ones are off by at most 2^-39 of it.
  * The NaN of a group of a key in sight reaches its tokens' outputs, that of a
  * value the group's elements; a query with an element that is not finite gives
  * NaN. */

@@ -27,7 +27,8 @@
 //           weights are at most 1 whatever the values' size is.
 //
 // Queries are multiplied by the power of two that brings their largest element
-// to 2^14 and beyond, so that BF16 ones fit FP16.  Scale and low of the tile's
+// to 2^14 and beyond, so that BF16 ones fit FP16: elements below 2^-28 of it are
+// subnormal there, multiples of 2^-24.  Scale and low of the tile's
 // keys and values are held by four lanes of a score's column each, two keys and
 // two values a lane, and broadcast within quads of lanes by DPP.
 //
@@ -75,14 +76,24 @@ template <int I>
 __device__ __forceinline__ float from_quad(float v) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), I * 0x55, 0xf, 0xf, true));
 }
-// acc += lane I's v * x.  (The compiler folds the broadcast into a product or a
-// sum, not into a fused one.  The wait covers a v, or an x by an
-// exponential, written just before.)
-template <int I>
-__device__ __forceinline__ void add_from_quad(float &acc, float v, float x) {
-    asm("s_nop 1\n\tv_fmac_f32_dpp %0, %1, %2 quad_perm:[%3,%3,%3,%3] row_mask:0xf bank_mask:0xf" : "+v"(acc) : "v"(v), "v"(x), "n"(I));
+// acc[0 .. 4) += lanes 0 .. 3's v * x, acc[4 .. 8) += theirs of w * x.  (The
+// compiler folds the broadcast into a product or a sum, not into a fused one.
+// The wait covers a v or w written just before.)
+__device__ __forceinline__ void add_each_from_quads(float *acc, float v, float w, float x) {
+    asm("s_nop 1\n\t"
+        "v_fmac_f32_dpp %0, %8, %10 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %1, %8, %10 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %2, %8, %10 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %3, %8, %10 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %4, %9, %10 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %5, %9, %10 quad_perm:[1,1,1,1] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %6, %9, %10 quad_perm:[2,2,2,2] row_mask:0xf bank_mask:0xf\n\t"
+        "v_fmac_f32_dpp %7, %9, %10 quad_perm:[3,3,3,3] row_mask:0xf bank_mask:0xf"
+        : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(acc[4]), "+v"(acc[5]), "+v"(acc[6]), "+v"(acc[7])
+        : "v"(v), "v"(w), "v"(x));
 }
-// The same over x[0 .. 4) with lanes 0 .. 3 of v and x[4 .. 8) with those of w.
+// acc += the sum of lanes 0 .. 3's v * x[0 .. 4) and theirs of w * x[4 .. 8).
+// (The wait also covers an x by an exponential.)
 __device__ __forceinline__ void add_from_quads(float &acc, float v, float w, const float *x) {
     asm("s_nop 1\n\t"
         "v_fmac_f32_dpp %0, %1, %3 quad_perm:[0,0,0,0] row_mask:0xf bank_mask:0xf\n\t"
@@ -96,7 +107,7 @@ __device__ __forceinline__ void add_from_quads(float &acc, float v, float w, con
         : "+v"(acc)
         : "v"(v), "v"(w), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
 }
-// lane I's v * x + y, as a product and a sum (see add_from_quad; x may be a
+// lane I's v * x + y, as a product and a sum (x may be a
 // matrix product's result, whose wait only the compiler knows).
 template <int I>
 __device__ __forceinline__ float sum_from_quad(float v, float x, float y) {
@@ -271,7 +282,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 }
             }
         }
-        float qs[NG], unscale;  // scale2 times the sums of the groups' elements; scale2 / the query's power of two
+        float qs[NG], unscale;  // sums of the groups' elements, multiplied; scale2 / the query's power of two
         int begin = k.begin, end = k.end, most_begin = k.begin, least_end = k.end;
 
         const ConstInts table = (ConstInts)(g.a.block_table + row * g.a.table_stride);
@@ -435,11 +446,15 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             const float odd = column_sum(top * 0.f);  // NaN where an element is not finite
             const int up = 15 - __builtin_amdgcn_frexp_expf(column_max(top));
             unscale = ldexpf(g.scale2, -up) + odd;
+            float sums[NG] = {};  // (of the elements as multiplied: no sum of finite ones overflows)
 #pragma unroll
             for (int s = 0; s < W; s++) {
                 float y[8];
 #pragma unroll
-                for (int c = 0; c < 8; c++) y[c] = ldexpf(x[s][c], up);
+                for (int c = 0; c < 8; c++) {
+                    y[c] = ldexpf(x[s][c], up);
+                    sums[s / GS] += y[c];
+                }
                 u32x4 v;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -451,14 +466,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             }
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
-            for (int i = 0; i < NG; i++) {
-                float sum = 0.f;
-#pragma unroll
-                for (int s = i * GS; s < (i + 1) * GS; s++)
-#pragma unroll
-                    for (int c = 0; c < 8; c++) sum += x[s][c];
-                qs[i] = column_sum(sum) * g.scale2;
-            }
+            for (int i = 0; i < NG; i++) qs[i] = column_sum(sums[i]);
             if (tokens > 1) {
                 int64_t b, e;
                 range_of(g, t + j, &b, &e);
@@ -481,7 +489,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             else if (taken == 2 * quarter) __builtin_amdgcn_s_setprio(1);
             else if (taken == 3 * quarter) __builtin_amdgcn_s_setprio(0);
             // scores: lane (col, lg) gets those of its eight keys
-            float x[8], offset[8];
+            float x[8];
             each<NG>([&](auto group) {
                 constexpr int C = group.value;
                 f32x4 acc[2];
@@ -505,20 +513,16 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
                 }
                 each<8>([&](auto i) {
                     constexpr int I = i.value, T = I >> 2;
-                    if constexpr (C == 0) {
-                        x[I] = from_quad<(I & 3)>(sc[T]) * acc[T][I & 3];
-                        offset[I] = from_quad<(I & 3)>(mid[T]) * qs[0];
-                    } else {
-                        x[I] = sum_from_quad<(I & 3)>(sc[T], acc[T][I & 3], x[I]);
-                        add_from_quad<(I & 3)>(offset[I], mid[T], qs[C]);
-                    }
+                    if constexpr (C == 0) x[I] = from_quad<(I & 3)>(sc[T]) * acc[T][I & 3];
+                    else x[I] = sum_from_quad<(I & 3)>(sc[T], acc[T][I & 3], x[I]);
                 });
+                add_each_from_quads(x, mid[0], mid[1], qs[C]);
             });
             __builtin_amdgcn_sched_barrier(0);
             load_k(pass + step);  // (past the end: the last keys again)
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = fmaf(unscale, x[i], offset[i]);
+            for (int i = 0; i < 8; i++) x[i] *= unscale;
 
             const int key0 = (int)key_of(pass, 0);
             const bool masked = (key0 < most_begin) | (key0 > least_end - kTile) | !__all(seen8 == 0xffu);

@@ -32,8 +32,9 @@ def cache_of(codes, scales, lows, pages, P):
     return [torch.from_numpy(rows.reshape(pages, P, 1, -1)).cuda(), torch.from_numpy(pairs.reshape(pages, P, 1, -1, 2)).cuda()]
 
 
-def check(q, key, value, P, scale):
-    """q [H, D] FP64 tensor in its type; key and value (codes, scales, lows) of one request, which q's heads share."""
+def check(q, key, value, P, scale, more=0.0, hidden=()):
+    """q [H, D] in its type; key and value (codes, scales, lows) of one request, which q's heads share.  more: added to d;
+    hidden: elements in which every key is 0, which add nothing to d."""
     n, D = key[0].shape
     pages, dt = -(-n // P), q.dtype
     cache = cache_of(*key, pages, P) + cache_of(*value, pages, P)
@@ -46,7 +47,8 @@ def check(q, key, value, P, scale):
         return wide(lows) + codes * wide(scales), np.abs(wide(lows)) + codes * np.abs(wide(scales))
 
     (k, kmag), (v, vmag), qq = numbers(key), numbers(value), np64(q)
-    s, d = qq @ k.T * scale, (np.abs(qq) @ kmag.T).max(-1, keepdims=True) * (D + 16) * 2.0 ** -24 * abs(scale)
+    kmag[:, list(hidden)] = 0
+    s, d = qq @ k.T * scale, (np.abs(qq) @ kmag.T).max(-1, keepdims=True) * (D + 16) * 2.0 ** -24 * abs(scale) + more
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
     want = p @ v
@@ -91,3 +93,43 @@ def test_outputs_whose_largest_value_is_zero(gpu, D, group, P, dtype):
     codes = np.ones((n, D))
     want, bound = check(torch.tensor(q).to(DT[dtype]).cuda(), key, (codes, np.ones((n, G)), first), P, 1.0)
     assert (np.abs(want) > bound).all()  # (30 2^-18, beside (16 + 31) 2^-24 of 2 and a hundredth of itself)
+
+
+@pytest.mark.parametrize("P", [16, 5])
+@pytest.mark.parametrize("D,group", LAYOUTS)
+def test_queries_whose_elements_sum_past_the_largest_number(gpu, D, group, P):
+    # finite BF16 elements of up to 2^127.9, all of one sign and mixed, whose sums pass FP32's largest number: scores are of ordinary size
+    rng = np.random.default_rng(D + group)
+    q = rng.uniform(1, 3.9, (4, D)) * 2.0 ** 126
+    q[1] = -q[1]
+    q[2, ::2] = -q[2, ::2]
+    q[3, 1:] *= 2.0 ** -rng.integers(0, 12, D - 1)
+    n, G = 40, D // group
+
+    def side():
+        return rng.integers(0, 16, (n, D)), rng.uniform(0.01, 0.02, (n, G)), rng.uniform(-0.2, -0.1, (n, G))
+    check(torch.tensor(q).bfloat16().cuda(), side(), side(), P, 2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype,k", [("fp16", 24), ("fp16", 27), ("fp16", 30), ("fp16", 34), ("bf16", 24), ("bf16", 30), ("bf16", 33), ("bf16", 36)])
+@pytest.mark.parametrize("D,group", LAYOUTS)
+def test_small_elements_beside_a_querys_largest(gpu, D, group, dtype, k):
+    """The largest element meets a 0 in every key, the others are 2^-k of it.
+    Down to 2^-28 (BF16: 2^-31) of the largest they keep all their bits, below
+    that each is off by at most 2^-39 of it; a matrix product of such
+    elements alone adds less than a hundredth of that."""
+    rng = np.random.default_rng(D + group + k)
+    X, G, n = 2.0 ** 15, D // group, 20
+    q = rng.uniform(1, 2, (6, D)) * X * 2.0 ** -k * rng.choice([-1, 1], (6, D))
+    at = [0, D - 1, 5]  # (and a high nibble where vectors have any)
+    codes = rng.integers(0, 16, (n, D))
+    codes[:, at] = 8
+    for h in range(6):
+        q[h, at] = 0
+        q[h, at[h % 3]] = X
+    q = torch.tensor(q).to(DT[dtype]).cuda()
+    key = (codes, np.ones((n, G)), np.full((n, G), -8.0))
+    value = (np.zeros((n, D)), np.zeros((n, G)), rng.standard_normal((n, G)))
+    scale = 1 / (X * 2.0 ** -k * 8 * D ** 0.5)
+    exact = k <= (28 if dtype == "fp16" else 31)
+    check(q, key, value, 16, scale, more=0 if exact else 1.01 * 2.0 ** -39 * X * scale * np.abs(codes - 8).sum(-1).max(), hidden=at)
