@@ -506,6 +506,10 @@ int orth_cache_read_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_
  * keys and values; q and out hold `dtype`.  Queries enter in FP16 with a power
  * of two of their own vector: elements down to 2^-28 of its largest (of BF16
  * ones 2^-31) keep all their bits, smaller ones are off by at most 2^-39 of it.
+ * A softmax weight times a value group's scale is off by at most 2^-24 of
+ * itself or 2^-39 of the largest such product of its token and head, all
+ * groups of the vector included: a group whose scales are below 2^-28 of
+ * another group's has sums off by more than 2^-11 of themselves.
  * The NaN of a group of a key in sight reaches its tokens' outputs, that of a
  * value the group's elements; a query with an element that is not finite gives
  * NaN. */

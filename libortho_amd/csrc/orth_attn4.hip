@@ -21,10 +21,14 @@
 //   values  O[d] = sum_j (p_j scale_j) c_j + sum_j p_j mid_j.  A lane loads
 //           its unit of eight keys; v_perm_b32 pairs the bytes of two keys,
 //           and their c are taken as above.
-//           The weights p scale enter as two FP16 parts, 2^-24 of the weight
-//           or 2^-39 of the largest of their column: the running maximum is
-//           that of score + exponent of the key's largest scale, so that
-//           weights are at most 1 whatever the values' size is.
+//           The weights p scale enter as two FP16 parts, off by 2^-24 of the
+//           weight or 2^-39 of the largest of their column: the running
+//           maximum is that of score + exponent of the key's largest scale, so
+//           that the largest weight is between 1/2 and 1, held as 2^14 to 2^15,
+//           whatever the values' size is.  (One maximum for all groups: one
+//           each would take 8 products and a maximum over keys and lanes a
+//           group more, for groups whose scales are below 2^-28 of another's
+//           of the same head.)
 //
 // Queries are multiplied by the power of two that brings their largest element
 // to 2^14 and beyond, so that BF16 ones fit FP16: elements below 2^-28 of it are
@@ -573,7 +577,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 #pragma unroll
                 for (int tau = 0; tau < 2; tau++) {
                     const f16x2 v = __builtin_bit_cast(f16x2, vp[tau][C]);
-                    sc[tau] = (float)v[0] * 0x1p14f;  // (held so, as FP16)
+                    sc[tau] = (float)v[0] * 0x1p15f;  // (held so, as FP16)
                     mid[tau] = fmaf((float)v[0], 8.f, (float)v[1]);
                 }
                 float weight[8], sum = 0.f;
@@ -633,7 +637,7 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
             float *dst = lds + wave * g.wave_floats + col * row_floats + 4 * lg;
 #pragma unroll
             for (int e = 0; e < 2 * W; e++) {
-                constexpr float f = 0x1p-14f;  // (the weights' 2^14)
+                constexpr float f = 0x1p-15f;  // (the weights' 2^15)
                 const float b = mids[e / (2 * GS)];
                 *reinterpret_cast<f32x4 *>(dst + 16 * e) = f32x4{fmaf(o[e][0], f, b), fmaf(o[e][1], f, b), fmaf(o[e][2], f, b), fmaf(o[e][3], f, b)};
             }

@@ -32,9 +32,10 @@ def cache_of(codes, scales, lows, pages, P):
     return [torch.from_numpy(rows.reshape(pages, P, 1, -1)).cuda(), torch.from_numpy(pairs.reshape(pages, P, 1, -1, 2)).cuda()]
 
 
-def check(q, key, value, P, scale, more=0.0, hidden=()):
+def check(q, key, value, P, scale, more=0.0, hidden=(), lost=0.0):
     """q [H, D] in its type; key and value (codes, scales, lows) of one request, which q's heads share.  more: added to d;
-    hidden: elements in which every key is 0, which add nothing to d."""
+    hidden: elements in which every key is 0, which add nothing to d;
+    lost: added to the bound."""
     n, D = key[0].shape
     pages, dt = -(-n // P), q.dtype
     cache = cache_of(*key, pages, P) + cache_of(*value, pages, P)
@@ -52,7 +53,7 @@ def check(q, key, value, P, scale, more=0.0, hidden=()):
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
     want = p @ v
-    bound = U[dt] * 1.01 * np.abs(want) + TINY[dt] + 2 * d * (p @ np.abs(v)) + (2.0 ** -20 + n * 2.0 ** -24) * (p @ vmag)
+    bound = U[dt] * 1.01 * np.abs(want) + TINY[dt] + 2 * d * (p @ np.abs(v)) + (2.0 ** -20 + n * 2.0 ** -24) * (p @ vmag) + lost
     err = np.abs(got - want)
     assert (err <= bound).all(), (float((err - bound).max()), float(np.abs(want).max()), float(bound.max()))
     return want, bound
@@ -133,3 +134,29 @@ def test_small_elements_beside_a_querys_largest(gpu, D, group, dtype, k):
     scale = 1 / (X * 2.0 ** -k * 8 * D ** 0.5)
     exact = k <= (28 if dtype == "fp16" else 31)
     check(q, key, value, 16, scale, more=0 if exact else 1.01 * 2.0 ** -39 * X * scale * np.abs(codes - 8).sum(-1).max(), hidden=at)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("ratio", [-20, -28, -32])
+@pytest.mark.parametrize("D,group,P", [(128, 32, 16), (128, 64, 5), (96, 32, 16), (256, 128, 16), (64, 32, 8)])
+def test_groups_of_values_of_very_different_scales(gpu, D, group, P, ratio, dtype):
+    """The second group's scales are 2^ratio of the others'.  A weight times a
+    scale is off by 2^-24 of itself or by 2^-39 of the largest of its token
+    and head, whichever is more: a group of 2^-20 of the largest keeps 2^-19
+    of its own sums, one of 2^-28 2^-11, in the formula and in what is tested."""
+    rng = np.random.default_rng(D - ratio)
+    n, G, H = 70, D // group, 3
+    q = torch.tensor(rng.standard_normal((H, D))).to(DT[dtype]).cuda()
+    key = (rng.integers(0, 16, (n, D)), rng.uniform(0.1, 0.3, (n, G)), rng.uniform(-2, -1, (n, G)))
+    scales = rng.uniform(2048, 4096, (n, G))  # (from 2^11 on, so that FP16 holds 2^-32 of them)
+    scales[:, 1] = 2.0 ** np.maximum(11 + ratio, -24) * rng.integers(1, 4, n)
+    lows = -8 * scales
+    value = (rng.integers(0, 16, (n, D)), scales, lows)
+    scale = D ** -0.5
+    # what the smallest group may lose: 2^-39 of the largest product of a weight and a scale, for each key's |u - 8|
+    qq, wide = np64(q), lambda a: np.repeat(np.asarray(a).astype(np.float16).astype(np.float64), group, -1)
+    s = qq @ (wide(key[2]) + key[0] * wide(key[1])).T * scale
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    lost = 1.01 * 2.0 ** -39 * (p * scales.astype(np.float16).astype(np.float64).max(-1)).max(-1)[:, None] * np.abs(value[0] - 8).sum(0)
+    check(q, key, value, P, scale, lost=lost)
