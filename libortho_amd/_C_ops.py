@@ -814,9 +814,16 @@ def int4_cache(pages, page_size, kv_heads, head_dim, group_size=None, device="cu
     every ``group_size`` elements of a vector, FP16 (scale, low) [pages,
     page_size, kv_heads, groups, 2]; code u stands for low + u * scale.
     ``group_size`` is ``head_dim``, or 32, 64 or 128 where that divides it
-    (None: 64 if it does, else ``head_dim``)."""
+    (None: 64 if it does, else ``head_dim``); ``head_dim`` a multiple of 8, at
+    most 256."""
+    _req(8 <= head_dim <= 256 and head_dim % 8 == 0, "head_dim must be a multiple of 8, at most 256")
     group_size = group_size if group_size is not None else 64 if head_dim % 64 == 0 else head_dim
-    _req(group_size > 0 and head_dim % group_size == 0, "group_size must divide head_dim")
+    _req(group_size == head_dim or (group_size in (32, 64, 128) and head_dim % group_size == 0),
+         "group_size must be head_dim, or 32, 64 or 128 where that divides it")
+    _req(1 <= pages < 1 << 31, "pages must be positive, at most 2^31 - 1")
+    _req(page_size >= 1, "page_size must be positive")
+    _req(kv_heads >= 1, "kv_heads must be positive")
+    _req(page_size < 1 << 31 and kv_heads < 1 << 31, "the cache's page_size or kv_heads is too large")
     codes = (pages, page_size, kv_heads, _int4_row_bytes(head_dim))
     scales = (pages, page_size, kv_heads, head_dim // group_size, 2)
     return tuple(torch.zeros(shape, dtype=dtype, device=device)
