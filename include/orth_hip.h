@@ -459,8 +459,10 @@ int orth_paged_attention_hip(const orth_hip_cache_t *cache, const orth_hip_atten
  * rounded to FP16, what passes +-65504 saturates): low = min x, scale =
  * (max x - min x) / 15 rounded to FP16 (the next number below where low + 15 *
  * scale would pass 65504), u = (x - low) / scale to the nearest, halves up; a
- * scale of 0 has codes 0.  A group with an element that is not finite is held
- * as NaN (scale and low NaN). */
+ * scale of 0 has codes 0.  Turned keys and (max x - min x) / 15 are numbers of
+ * 64 bits that are rounded to FP32 and then to FP16, each to the nearest, ties
+ * to even (some last places differ from one rounding's).  A group with an
+ * element that is not finite is held as NaN (scale and low NaN). */
 #define ORTH_INT4_ROW_BYTES(head_dim) \
     ((head_dim) <= 64 ? 32 : (head_dim) <= 96 ? 48 : (head_dim) <= 128 ? 64 : 128)
 typedef struct {
@@ -481,8 +483,8 @@ typedef struct {
 
 /* orth_cache_append_hip for that cache; q, k, v and q_out hold `dtype`
  * (ORTH_DT_F16 or ORTH_DT_BF16).  q is turned as there; k is turned in 64 bits
- * and rounded to FP16 once (a last place may move a code).  Two tokens with
- * one slot leave a mixture of both there. */
+ * and rounded through FP32 to FP16 (a last place may move a code).  Two tokens
+ * with one slot leave a mixture of both there. */
 int orth_cache_append_int4_hip(const orth_hip_int4_cache_t *cache, const orth_hip_append_t *append, int32_t dtype,
                                void *stream);
 

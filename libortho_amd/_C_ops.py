@@ -860,10 +860,10 @@ def _dtype16(t: torch.Tensor, name: str) -> int:
 def cache_append_int4(k, v, k_codes, k_scales, v_codes, v_scales, slots, q=None, positions=None, cos_sin=None,
                       interleaved=False, q_out=None):
     """:func:`cache_append` into a cache of :func:`int4_cache`: k, turned like
-    q, and v are quantised as they are written (float16 or bfloat16; elements
-    past +-65504 saturate, a group with one that is not finite is held as
-    NaN).  q comes back in its own type.  Two tokens with one slot leave a
-    mixture of both there."""
+    q, and v are quantised as they are written (float16 or bfloat16; k turned
+    in 64 bits, then float32, then float16; elements past +-65504 saturate, a
+    group with one that is not finite is held as NaN).  q comes back in its own
+    type.  Two tokens with one slot leave a mixture of both there."""
     T = _lib.torch_ops()
     if T is not None:
         return T.cache_append_int4(k, v, k_codes, k_scales, v_codes, v_scales, slots, q, positions, cos_sin, interleaved, q_out)
@@ -880,9 +880,10 @@ def cache_append_int4(k, v, k_codes, k_scales, v_codes, v_scales, slots, q=None,
 
 def cache_read_int4(k_codes, k_scales, v_codes, v_scales, slots, head_dim, dtype=torch.float16, k_out=None, v_out=None):
     """The keys and values of ``slots`` (int64 [n]) of a cache of
-    :func:`int4_cache`, low + u * scale rounded once to ``dtype`` (float16 or
-    bfloat16): two tensors [n, kv_heads, head_dim], new ones or ``k_out`` and
-    ``v_out``.  A slot that is negative or past the cache reads as zeros."""
+    :func:`int4_cache`, low + u * scale rounded to ``dtype`` (float16 once,
+    bfloat16 from float32): two tensors [n, kv_heads, head_dim], new ones or
+    ``k_out`` and ``v_out``.  A slot that is negative or past the cache reads
+    as zeros."""
     T = _lib.torch_ops()
     if T is not None:
         return T.cache_read_int4(k_codes, k_scales, v_codes, v_scales, slots, head_dim, dtype, k_out, v_out)

@@ -17,9 +17,9 @@ constexpr int64_t kLaunch = 1 << 23;  // workgroups of 256 along x (2^32 threads
 // The codes' layout wants one byte of eight units from a lane, so eight lanes
 // exchange nibbles in three steps and hold a unit each.
 //
-// What is quantised has to be the FP16 number nearest to the turned key, and a
-// code the one nearest to the quotient: a last place of difference moves a
-// code by a whole step.  FP32 decides all but the numbers next to a border,
+// What is quantised has to be the turned key in 64 bits rounded to FP32 and to
+// FP16, and a code the one nearest to the quotient: a last place of difference
+// moves a code by a whole step.  FP32 decides all but the numbers next to a border,
 // and 64 bits those (one key in some 800, one code in some 30,000).
 //
 // An element is read once and, of keys and values, a quarter of it written;
