@@ -53,6 +53,17 @@ struct Keys {
     uint32_t units;
 };
 
+// Numbers that all lanes share, known as such: in scalar registers, also where
+// a division made them by way of vector ones.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
+__device__ __forceinline__ Keys uniform(const Keys &k) {
+    return Keys{__builtin_amdgcn_readfirstlane(k.begin), __builtin_amdgcn_readfirstlane(k.end),
+                __builtin_amdgcn_readfirstlane(k.tile0), __builtin_amdgcn_readfirstlane(k.tiles),
+                (uint32_t)__builtin_amdgcn_readfirstlane((int)k.units)};
+}
+
 // a / b.  (A 64-bit division takes a quarter of a microsecond, and a short
 // call is a chain of such latencies: below 2^22 a product with the reciprocal
 // is off by one at the most.)
@@ -138,13 +149,7 @@ __device__ __forceinline__ Keys tiles_of(const G &g, const Block &b) {
     return tiles_of(g, b.end == 0 ? 0 : b.begin, b.end);
 }
 
-// The keys of the item that starts with token t, and its tokens, as numbers
-// that all lanes are known to share.
-__device__ __forceinline__ Keys uniform(const Keys &k) {
-    return Keys{__builtin_amdgcn_readfirstlane(k.begin), __builtin_amdgcn_readfirstlane(k.end),
-                __builtin_amdgcn_readfirstlane(k.tile0), __builtin_amdgcn_readfirstlane(k.tiles),
-                (uint32_t)__builtin_amdgcn_readfirstlane((int)k.units)};
-}
+// The keys of the item that starts with token t, and its tokens.
 template <class G>
 __device__ __forceinline__ Keys keys_at(const G &g, int64_t t, int lane, int *tokens) {
     *tokens = 1;
@@ -196,6 +201,10 @@ struct Share {
     int item;
     uint32_t unit;
 };
+__device__ __forceinline__ Share uniform(const Share &s) {
+    return Share{(uint64_t)uniform64(s.per), (uint64_t)uniform64(s.cur), (uint64_t)uniform64(s.stop), uniform64(s.t), uniform(s.k),
+                 __builtin_amdgcn_readfirstlane(s.item), (uint32_t)__builtin_amdgcn_readfirstlane((int)s.unit)};
+}
 template <class G>
 __device__ __forceinline__ bool share_of(const G &g, int lane, int items, Share *s) {
     Keys mine[2];

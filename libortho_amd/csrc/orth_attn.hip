@@ -128,6 +128,13 @@ __global__ __launch_bounds__(256, KS > 4 ? 1 : KS > 2 ? 2 : 3) void attend_kerne
 
     Share w;
     if (!share_of(g, lane, items, &w)) return;
+    // (in scalar registers some 20 vector registers fewer are used.  Without
+    // PG8, whose loop needs them for its addresses, that is faster: a prompt of
+    // 2,048 tokens, 8 of 32 heads, FP16, pages of 7, 1,251 us and 1,008, 32
+    // requests of 16 to 2,000 keys, 16 heads of 64, 21.5 and 20.3.  With it the
+    // items' starts and ends get slower: the prompt, BF16, pages of 16, 836 and
+    // 867, the 32 requests 16.6 and 17.0.)
+    if constexpr (!PG8) w = uniform(w);
     const uint64_t first = w.cur, stop = w.stop, per = w.per;
     uint64_t cur = w.cur;
     int64_t t = w.t;

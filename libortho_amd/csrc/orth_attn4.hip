@@ -53,10 +53,6 @@ namespace orth {
 
 namespace {
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
-}
-
 struct Attend4Args : AttendArgs<orth_hip_int4_cache_t> {
     static constexpr bool blocks = true;
     int block;   // tokens that may share a head tile, a power of two
@@ -230,13 +226,13 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
 
     Share w;
     if (!share_of(g, lane, items, &w)) return;
-    const uint64_t first = uniform64(w.cur), stop = uniform64(w.stop), per = uniform64(w.per);
+    w = uniform(w);
+    const uint64_t first = w.cur, stop = w.stop, per = w.per;
     uint64_t cur = w.cur;
     int64_t t = w.t;
-    Keys k = uniform(w.k);
-    int item = __builtin_amdgcn_readfirstlane(w.item), tokens = 1;
-    uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)w.unit);
-    cur = uniform64(cur), t = uniform64(t);
+    Keys k = w.k;
+    int item = w.item, tokens = 1;
+    uint32_t unit = w.unit;
     if (g.block > 1) k = keys_at(g, t, lane, &tokens);
 
     // A SIMD prefers its oldest wave, which then ends long before the others
