@@ -31,14 +31,14 @@
 // (orth_attend.h).
 //
 // Measured (one MI355X, a call among others, inputs from HBM): 128 requests
-// of 2,048 to 16,384 keys, 8 of 64 heads of 128, BF16: 594 us, 5.6 TB/s (a
-// kernel that only reads reaches 5.7); 32 ragged requests up to 4,096 keys, 32
-// heads, FP16: 73.8 us, 4.6 TB/s; one of 32,768 keys, 8 of 32 heads: 37.3 us
+// of 2,048 to 16,384 keys, 8 of 64 heads of 128, BF16: 585 us, 5.7 TB/s (what
+// a kernel that only reads reaches); 32 ragged requests up to 4,096 keys, 32
+// heads, FP16: 73.2 us, 4.6 TB/s; one of 32,768 keys, 8 of 32 heads: 37.0 us
 // (32 the keys, 5 the join of 64 pieces a key head), 3.6 TB/s; one of 190
-// keys, 32 heads: 8.9 us, a chain of latencies (position 1.2, share 0.7, table
+// keys, 32 heads: 8.7 us, a chain of latencies (position 1.2, share 0.7, table
 // 1.6, keys 2, join 1).  HBM reads by counter: 3.37 GB, 344 MB and 135 MB for
 // the first three, as their keys and values.  Several tokens of one request
-// read its keys each for itself (2,048 tokens of one prompt: 853 us).
+// read its keys each for itself (2,048 tokens of one prompt: 836 us).
 // A wave per query head on the vector unit (no matrix products, no split)
 // took 35,500, 7,900, 57,500 and 164 us.
 #include "orth_attend.h"

@@ -1,4 +1,5 @@
-// Attention of single tokens over the cache in 4 bits.
+// Attention over the cache in 4 bits: single tokens, and several tokens of a
+// request (a prompt, a draft) together.
 //
 // One pass over the keys with a running maximum and sum of the softmax, as
 // over the cache in 16 bits (orth_attn.hip): a wave takes 32 keys from
@@ -32,17 +33,18 @@
 //
 // Queries are multiplied by the power of two that brings their largest element
 // to 2^14 and beyond, so that BF16 ones fit FP16: elements below 2^-28 of it are
-// subnormal there, multiples of 2^-24.  Scale and low of the tile's
-// keys and values are held by four lanes of a score's column each, two keys and
-// two values a lane, and broadcast within quads of lanes by DPP.
+// subnormal there, multiples of 2^-24.  Scale and low of the tile's keys and
+// values are held by four lanes of a score's column each, two keys and two
+// values a lane, and broadcast within quads of lanes by DPP.
 //
 // Bound by memory and instructions about equally where there are many keys
-// (128 requests of 2,048 to 16,384 keys, 8 of 64 heads, 943 MB: 232 us, 4.1
+// (128 requests of 2,048 to 16,384 keys, 8 of 64 heads, 943 MB: 239 us, 3.9
 // TB/s).  A head's row of a slot is half a line of 128 bytes, so the waves of
 // neighbouring heads keep step (a barrier a tile) and find each other's lines
-// in the L1 (without: 258 us, 1,258 MB read; 1,088 with it, the rest (scale,
-// low) pairs whose lines hold the heads of two workgroups).  Few keys: a chain
-// of latencies (190 keys, 32 heads: 13 us).
+// in the L1 (without it some 11% slower, 1,258 MB read; 1,088 with it, the rest
+// (scale, low) pairs whose lines hold the heads of two workgroups).  Few keys:
+// a chain of latencies (190 keys, 32 heads: 13 us).  A prompt of 2,048 tokens, 8
+// of 32 heads: 288 us.
 // Two tiles of keys in one product where no more than eight columns are used,
 // and one softmax for both, was 2% faster at the largest call and up to 15%
 // slower at the others; four workgroups a CU 3% slower than three.
@@ -208,7 +210,9 @@ constexpr int kResident = W > 4 ? (PG16 ? 2 : 1) : 3;
 // W: bytes of a unit; GS: steps of 32 elements of a group.
 // PG16: page_size is a multiple of 16, so 16 keys from a multiple of 16 lie in
 // one page: a scalar table entry and scalar addresses serve them, and lanes
-// add offsets that stay the same for the whole item.
+// add offsets that stay the same for the whole item.  (Without it every key has
+// an entry and an address of its own: 128 requests 411 us in pages of 28, 239
+// in pages of 32; 190 keys 16 and 13.)
 template <int W, int GS, bool PG16>
 __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Attend4Args g) {
     constexpr int NG = W / GS, VD = (W + 3) / 4;
@@ -238,8 +242,8 @@ __global__ __launch_bounds__(256, (kResident<W, PG16>)) void attend4_kernel(Atte
     // A SIMD prefers its oldest wave, which then ends long before the others
     // and leaves them alone with their latencies (shares of one length ended
     // between 116 and 274 us): a wave that is through a quarter of its share
-    // gives way to those that are not (128 requests: 239 us without, 231 with;
-    // 128 tokens of four prompts 102 and 95, 32 ragged requests 41.0 and 39.6).
+    // gives way to those that are not (128 requests: 251 us without, 239 with;
+    // 128 tokens of four prompts 110 and 104, 32 ragged requests 42.5 and 41.5).
     const uint32_t quarter = (uint32_t)(stop - first) * kPair / 4 + 1;
     uint32_t taken = 0;
     __builtin_amdgcn_s_setprio(3);
@@ -673,7 +677,9 @@ Attend4Args attend4_args(const orth_hip_int4_cache_t &c, const orth_hip_attend_t
     g.gtiles = (g.group + 15) / 16;
     g.groups = c.head_dim / c.group_size;
     // Neighbouring tokens share a product where some request must have several:
-    // more tokens than requests.
+    // more tokens than requests.  (A table of more rows than tokens may have
+    // several of one request too, which the host cannot see: 128 tokens of four
+    // prompts 103 us with up to 511 rows, 249 with 512.)
     g.block = 1;
     if (a.rows && a.tokens > a.table_rows)
         while (2 * g.block * g.group <= 16) g.block *= 2;
@@ -681,9 +687,10 @@ Attend4Args attend4_args(const orth_hip_int4_cache_t &c, const orth_hip_attend_t
     // The pieces of a full tile are twice as long, so there neighbouring heads
     // go together from two items a CU on, else from one for four CUs (8 key
     // heads with 16 columns each; one, two and four heads a workgroup: 1,024
-    // items of a head, 128 tokens of four prompts 108, 112 and 135 us, 8 tokens
-    // of 64 prompts 143, 117 and 140; 128 requests 132, 105 and 126; 4,096
-    // items, 512 tokens of four prompts: 330, 306 and 305).
+    // items of a head, 128 tokens of four prompts 108, 110 and 136 us, 8 tokens
+    // of 64 prompts 130, 106 and 116; 128 requests of 2,048 to 16,384 keys, the
+    // call that would rather have four, 395, 283 and 266; 4,096 items, 512
+    // tokens of four prompts: 336, 309 and 309).
     attend_tiles(g, g.gt > 8 ? 2 * cus : cus / 4, (a.tokens + g.block - 1) / g.block);
     const int resident = by_sixteen(c) ? c.head_dim > 128 ? kResident<8, true> : kResident<4, true>
                                        : c.head_dim > 128 ? kResident<8, false> : kResident<4, false>;
